@@ -1,0 +1,78 @@
+"""A cache in 4 bits, what needs no GPU: the plain implementation, and the refusals of the kernel library's entries (all sizes are checked
+before anything is launched)."""
+import ctypes
+from fractions import Fraction
+
+import pytest
+import torch
+
+import plain_packed as plain
+
+
+def test_plain_quantisation_of_known_numbers():
+    assert plain.quantise_group([0.0, 15.0, 7.4, 7.5, 8.5, 1.0]) == (1.0, 0.0, [0, 15, 7, 8, 8, 1])          # ties to even
+    assert plain.quantise_group([2.0] * 4) == (0.0, 2.0, [0] * 4)
+    step, zero, codes = plain.quantise_group([1.0, 1.001953125])       # the least number, and a range below bfloat16's spacing at 1
+    assert zero == 1.0 and codes == [0, 15] and step == float(plain._bfloat16(Fraction(1.001953125 - 1.0) / 15))
+    assert plain._bfloat16(Fraction(257)) == 256 and plain._bfloat16(Fraction(259)) == 260
+    assert all(v != v for v in plain.quantise_group([1.0, float("inf")])[:2])
+
+
+def test_a_number_read_back_is_within_half_a_step():
+    x = torch.randn(20, 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+    codes, pairs = plain.quantise(x, 64)
+    off = (plain.values(codes, pairs).view(20, 2, 64) - x.double().view(20, 2, 64)).abs()
+    step = pairs[..., 0].view(20, 2, 1)
+    # half a step, and where the step was rounded down, by at most 2^-8 of itself, the last code may lie 15 · 2^-8 of a step further off
+    assert bool((off <= step * (0.5 + 15 * 2.0 ** -8)).all())
+
+
+@pytest.mark.parametrize("dim,group", [(16, 16), (32, 32), (48, 16), (64, 64), (80, 16), (96, 32), (128, 64), (192, 64), (256, 64), (24, 0), (0, 0),
+                                       (-64, 0), (272, 0)])
+def test_groups(dim, group):
+    from vlrf_b200.csrc import library, ops
+    assert ops.packed_group(dim) == group and library().vlrf_packed_group(dim) == group
+    if group:
+        assert plain.group_of(dim) == group
+
+
+def pointers(n):
+    return [ctypes.c_void_p(4096)] * n
+
+
+@pytest.mark.parametrize("change", [dict(dh=24), dict(dh=512), dict(T=-1), dict(Hkv=0), dict(BT=0), dict(max_blocks=0), dict(dtype=2), dict(dev_err=None),
+                                    dict(T=2 ** 30, Hkv=64)])
+def test_append_and_read_refuse(change):
+    from vlrf_b200.csrc import library
+    lib = library()
+    a = dict(dict(dtype=0, T=3, Hkv=2, dh=64, BT=64, max_blocks=4, dev_err=ctypes.c_void_p(4096)), **change)
+    assert lib.vlrf_packed_append(*pointers(1), a["dtype"], 384, 128, 256, *pointers(4), 10, *pointers(1), a["max_blocks"], *pointers(2), a["T"], a["Hkv"],
+                                  a["dh"], a["BT"], a["dev_err"], None) != 0
+    assert b"packed_append" in lib.vlrf_last_error()
+    assert lib.vlrf_packed_read(*pointers(4), 10, *pointers(1), a["max_blocks"], *pointers(3), 128, *pointers(1), 128, a["dtype"], a["T"], a["Hkv"], a["dh"],
+                                a["BT"], a["dev_err"], None) != 0
+    assert b"packed_read" in lib.vlrf_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(dh=24), dict(dh=512), dict(T=-1), dict(H=3), dict(H=0), dict(BT=48), dict(BT=0), dict(max_blocks=0), dict(dtype=2),
+                                    dict(window=-1), dict(dev_err=None)])
+def test_attention_refuses(change):
+    from vlrf_b200.csrc import library
+    lib = library()
+    a = dict(dict(dtype=0, T=3, H=4, Hkv=2, dh=64, BT=64, max_blocks=4, window=0, dev_err=ctypes.c_void_p(4096)), **change)
+    assert lib.vlrf_attn_packed(*pointers(1), a["dtype"], 384, 0, *pointers(4), 10, *pointers(1), a["max_blocks"], *pointers(3), 256, a["T"], a["H"], a["Hkv"],
+                                a["dh"], a["BT"], 0.125, a["window"], a["dev_err"], None) != 0
+    assert b"attn_packed" in lib.vlrf_last_error()
+
+
+def test_no_cpu_path():
+    from vlrf_b200.csrc import KernelError, ops
+    cache = ops.PackedKV.zeros(3, 2, 64, 64, "cpu")
+    assert cache.bytes() == 3 * 2 * 64 * (64 + 8)
+    t = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(KernelError):
+        ops.kv_append_packed(torch.zeros(4, 384), 128, 256, cache, t.view(1, 4), t, t, 4, 2, 64, t)
+    with pytest.raises(KernelError):
+        ops.kv_read_packed(cache, t.view(1, 4), t, t, torch.zeros(4, 128), torch.zeros(4, 128), 4, t)
+    with pytest.raises(KernelError):
+        ops.attention_packed(torch.zeros(4, 384), 0, cache, t.view(1, 4), t, t, torch.zeros(4, 128), 4, 2, 2, 64, 0.125, 0, t)

@@ -1,0 +1,304 @@
+"""The kernels over a paged cache of keys and values in 4 bits against exact rational arithmetic and float64.
+
+Tolerances, from the arithmetic.  Codes, steps and zeros: none, every rounding is that of an exact quotient.  Numbers read back: none, zero +
+step · code is one rounding.  Attention: a result is a mean of values with weights softmax(s).  With u = 2^-24, a score is a sum of
+dim products in float32, off by at most e_s = (dim + 16) u · scale · Σ |q| (|zero| + 15 step); weights are then off by a factor of at most
+exp(2 e_s), their exponentials and sums by (keys + 32) u.  bfloat16 has eight significant bits: numbers of the binade from 1 on are 2^-7 apart, so
+a rounding to it is off by at most 2^-8 of the number.  On the tensor cores a weight times a step is rounded to it, which moves a result by
+at most 2^-8 · 15 step of the values' groups; and a bfloat16 result is rounded once."""
+import math
+
+import pytest
+import torch
+
+import plain_packed as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U, HALF_STEP = 2.0 ** -24, 2.0 ** -8
+
+
+def err_word():
+    return torch.zeros(1, dtype=torch.int32, device=DEV)
+
+
+class Pages:
+    """Sequences of given lengths in shuffled blocks of a cache full of another owner's leftovers (NaN among them)."""
+
+    def __init__(self, lengths, kv_heads, dim, seed=0, spare=3):
+        from vlrf_b200.csrc import ops
+        gen = torch.Generator().manual_seed(seed)
+        need = [-(-n // 64) for n in lengths]
+        self.n_blocks = sum(need) + spare
+        order = torch.randperm(self.n_blocks, generator=gen)
+        self.table = torch.full((len(lengths), max(need + [1]) + 1), -1, dtype=torch.int32)
+        at = 0
+        for i, n in enumerate(need):
+            self.table[i, :n] = order[at:at + n].int()
+            at += n
+        groups = dim // plain.group_of(dim)
+        shape = (self.n_blocks, kv_heads, 64)
+        self.host = {}
+        for name, size in (("k", 1.3), ("v", 0.7)):
+            self.host[name] = torch.randint(0, 256, shape + (dim // 2,), generator=gen, dtype=torch.uint8)
+            step = torch.rand(shape + (groups,), generator=gen) * 0.3 * size + 0.01
+            zero = -7.5 * step + torch.randn(shape + (groups,), generator=gen) * 0.4
+            self.host[name + "_pairs"] = torch.stack([step, zero], -1).bfloat16()
+        # what lies behind a sequence's last token, and in blocks of nobody: not a number
+        owned = torch.zeros(shape[:1] + (64,), dtype=torch.bool)
+        for i, n in enumerate(lengths):
+            for p in range(n):
+                owned[self.table[i, p // 64], p % 64] = True
+        for name in ("k_pairs", "v_pairs"):
+            self.host[name][~owned[:, None, :].expand(shape)] = float("nan")
+        self.cache = ops.PackedKV(*[self.host[n].to(DEV) for n in ("k", "k_pairs", "v", "v_pairs")])
+        self.lengths = lengths
+
+    def context(self, i):
+        n = self.lengths[i]
+        place = torch.arange(n)
+        blocks = self.table[i].long()[place // 64]
+        return [plain.unpacked(self.host[name], self.host[name + "_pairs"])[blocks, :, place % 64] for name in ("k", "v")]
+
+    def reach(self, i, name):
+        """|zero| + 15 step of sequence i's tokens, per entry, and 15 step alone."""
+        n = self.lengths[i]
+        place = torch.arange(n)
+        blocks = self.table[i].long()[place // 64]
+        pairs = self.host[name + "_pairs"][blocks, :, place % 64].double()
+        return (pairs[..., 1].abs() + 15 * pairs[..., 0]), 15 * pairs[..., 0]
+
+
+def bound(pages, i, pos, first, q, scale, want, dtype, tensor_cores):
+    """The derivation above, for one token: [heads, 1]."""
+    share = q.shape[0] // pages.context(i)[0].shape[1]
+    rk, _ = pages.reach(i, "k")
+    rv, sv = pages.reach(i, "v")
+    dim = q.shape[1]
+    group = dim // rk.shape[-1]
+    out = []
+    for h in range(q.shape[0]):
+        k_reach = rk[first:pos + 1, h // share].repeat_interleave(group, -1)
+        e_s = (dim + 16) * U * scale * float((k_reach * q[h].abs()).sum(-1).max())
+        v_max, s_max = float(rv[first:pos + 1, h // share].max()), float(sv[first:pos + 1, h // share].max())
+        rel = math.expm1(2 * e_s) + (pos + 1 - first + 32) * U
+        out.append(2 * rel * v_max + (HALF_STEP * s_max if tensor_cores else 0.0))
+    tol = torch.tensor(out, dtype=torch.float64)[:, None].expand_as(want)
+    if dtype == torch.bfloat16:
+        tol = tol + HALF_STEP * (want.abs() + tol)
+    return tol
+
+
+# ---- append and read ---------------------------------------------------------------------------------------------------
+
+def rows_of(T, width, dtype, seed, kind="plain"):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn((T, width), generator=gen) * 1.5 + torch.randn((1, width), generator=gen)
+    if kind == "grid":                         # quotients on the borders: ties
+        x = torch.randint(-31, 32, (T, width), generator=gen).float() * 0.25
+    if kind == "wild":                         # many sizes in one row, down to subnormal
+        x = x * torch.exp2(torch.randint(-130, 60, (T, 1), generator=gen).float())
+    if kind == "flat":
+        x = torch.full((T, width), 1.0) * torch.randn((T, 1), generator=gen)
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["plain", "grid", "wild", "flat"])
+@pytest.mark.parametrize("heads,kv_heads,dim,new,past", [
+    (12, 12, 64, [1], [515]), (4, 2, 128, [3, 1, 70], [0, 63, 60]), (3, 3, 32, [5, 66], [62, 0]), (5, 5, 16, [9], [0]), (2, 1, 80, [65], [1]),
+    (3, 1, 256, [2], [64]), (2, 2, 192, [4], [0]), (6, 3, 96, [7, 1], [128, 0])])
+def test_append_holds_the_exact_codes_and_reads_back(dtype, kind, heads, kv_heads, dim, new, past):
+    from vlrf_b200.csrc import ops
+    T, width = sum(new), (heads + 2 * kv_heads) * dim
+    pages = Pages([a + b for a, b in zip(new, past)], kv_heads, dim, seed=dim)
+    rows = rows_of(T, width, dtype, seed=T + dim, kind=kind)
+    slot = torch.tensor([i for i, a in enumerate(new) for _ in range(a)], dtype=torch.int32)
+    pos = torch.tensor([b + j for a, b in zip(new, past) for j in range(a)], dtype=torch.int32)
+    k_off, v_off = heads * dim, (heads + kv_heads) * dim
+    e = err_word()
+    ops.kv_append_packed(rows.to(DEV), k_off, v_off, pages.cache, pages.table.to(DEV), slot.to(DEV), pos.to(DEV), T, kv_heads, dim, e)
+    assert int(e.item()) == 0
+    want = {name: plain.quantise(rows[:, at:at + kv_heads * dim], dim) for name, at in (("k", k_off), ("v", v_off))}
+    got = {n: getattr(pages.cache, n).cpu() for n in ("k", "k_pairs", "v", "v_pairs")}
+    touched = torch.zeros((pages.n_blocks, 64), dtype=torch.bool)
+    for t in range(T):
+        blk, at = int(pages.table[slot[t], pos[t] // 64]), int(pos[t] % 64)
+        touched[blk, at] = True
+        for name in ("k", "v"):
+            codes = torch.stack([got[name][blk, :, at] & 15, got[name][blk, :, at] >> 4], -1).flatten(-2)
+            pairs = got[name + "_pairs"][blk, :, at]
+            assert torch.equal(pairs.double(), want[name][1][t]), (name, t)
+            assert torch.equal(codes.long(), want[name][0][t]), (name, t)
+    for name in got:                           # everything else is as it was
+        same = ~touched[:, None, :].expand(got[name].shape[:3])
+        assert torch.equal(got[name][same].view(torch.uint8), pages.host[name][same].view(torch.uint8))
+    for out_dtype in (torch.float32, torch.bfloat16):
+        out = [torch.full((T, kv_heads * dim), 7.0, dtype=out_dtype, device=DEV) for _ in range(2)]
+        ops.kv_read_packed(pages.cache, pages.table.to(DEV), slot.to(DEV), pos.to(DEV), out[0], out[1], T, e)
+        for o, name in zip(out, ("k", "v")):
+            assert torch.equal(o.cpu(), plain.values(*want[name]).reshape(T, -1).float().to(out_dtype))
+    assert int(e.item()) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_group_that_is_not_finite_reads_back_as_nan_and_no_other(dtype):
+    from vlrf_b200.csrc import ops
+    pages = Pages([8], 2, 128)
+    rows = rows_of(8, 3 * 256, dtype, seed=1)
+    rows[2, 256 + 70] = float("nan")           # keys, head 0, second group
+    rows[3, 512 + 128] = float("inf")          # values, head 1, first group
+    rows[4, 256] = -float("inf")
+    rows[5, 256:320] = torch.tensor([-3.0e38, 3.0e38] * 32).to(dtype)      # finite numbers, a range that is not
+    slot, pos = torch.zeros(8, dtype=torch.int32, device=DEV), torch.arange(8, dtype=torch.int32, device=DEV)
+    e = err_word()
+    ops.kv_append_packed(rows.to(DEV), 256, 512, pages.cache, pages.table.to(DEV), slot, pos, 8, 2, 128, e)
+    out = [torch.empty(8, 256, device=DEV) for _ in range(2)]
+    ops.kv_read_packed(pages.cache, pages.table.to(DEV), slot, pos, out[0], out[1], 8, e)
+    nan = [torch.zeros(8, 256, dtype=torch.bool) for _ in range(2)]
+    nan[0][2, 64:128] = nan[0][4, :64] = nan[0][5, :64] = nan[1][3, 128:192] = True
+    for o, n in zip(out, nan):
+        assert torch.equal(torch.isnan(o.cpu()), n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_append_and_read_with_strides_and_odd_alignment(dtype, shift):
+    """Columns that begin anywhere in wider rows, in and out."""
+    from vlrf_b200.csrc import ops
+    T, kv_heads, dim = 37, 3, 64
+    pages = Pages([T], kv_heads, dim)
+    wide = torch.full((T, 700), float("nan"), dtype=dtype)
+    rows = rows_of(T, 2 * 192, dtype, seed=5)
+    wide[:, shift:shift + 384] = rows
+    dev = wide.to(DEV)
+    slot, pos = torch.zeros(T, dtype=torch.int32, device=DEV), torch.arange(T, dtype=torch.int32, device=DEV)
+    e = err_word()
+    ops.kv_append_packed(dev[:, shift:shift + 384], 0, 192, pages.cache, pages.table.to(DEV), slot, pos, T, kv_heads, dim, e)
+    out = torch.full((T, 700), 9.0, dtype=dtype, device=DEV)
+    ops.kv_read_packed(pages.cache, pages.table.to(DEV), slot, pos, out[:, shift:shift + 192], out[:, 300 + shift:492 + shift], T, e)
+    want = [plain.values(*plain.quantise(rows[:, at:at + 192], dim)).reshape(T, -1).float().to(dtype) for at in (0, 192)]
+    got = out.cpu()
+    assert torch.equal(got[:, shift:shift + 192], want[0]) and torch.equal(got[:, 300 + shift:492 + shift], want[1])
+    got[:, shift:shift + 192] = got[:, 300 + shift:492 + shift] = 9.0
+    assert bool((got == 9.0).all()) and int(e.item()) == 0
+
+
+def test_padding_rows_and_blocks_that_are_not_mapped():
+    from vlrf_b200.csrc import ops
+    pages = Pages([70, 5], 2, 64)
+    before = {n: getattr(pages.cache, n).clone() for n in ("k", "k_pairs", "v", "v_pairs")}
+    rows = rows_of(4, 3 * 128, torch.bfloat16, seed=2).to(DEV)
+    table = pages.table.to(DEV)
+    slot = torch.tensor([-1, -1, -1, -1], dtype=torch.int32, device=DEV)
+    pos = torch.tensor([3, 900, 0, 12], dtype=torch.int32, device=DEV)
+    e = err_word()
+    ops.kv_append_packed(rows, 128, 256, pages.cache, table, slot, pos, 4, 2, 64, e)
+    assert all(torch.equal(getattr(pages.cache, n).view(torch.uint8), before[n].view(torch.uint8)) for n in before) and int(e.item()) == 0
+    out = [torch.full((4, 128), 5.0, device=DEV) for _ in range(2)]
+    ops.kv_read_packed(pages.cache, table, slot, pos, out[0], out[1], 4, e)
+    assert all(bool((o == 0).all()) for o in out) and int(e.item()) == 0
+    # positions without a block, beyond the table, negative; block numbers outside the cache: an error bit, nothing written
+    bad = pages.table.clone()
+    bad[0, 0] = pages.n_blocks
+    for where, at in ((pages.table, 130), (pages.table, 10_000), (pages.table, -1), (bad, 3)):
+        e = err_word()
+        slot = torch.zeros(1, dtype=torch.int32, device=DEV)
+        pos = torch.tensor([at], dtype=torch.int32, device=DEV)
+        ops.kv_append_packed(rows, 128, 256, pages.cache, where.to(DEV), slot, pos, 1, 2, 64, e)
+        assert int(e.item()) == 4
+        e = err_word()
+        ops.kv_read_packed(pages.cache, where.to(DEV), slot, pos, out[0], out[1], 1, e)
+        assert int(e.item()) == 4 and bool((out[0][0] == 0).all())
+        assert all(torch.equal(getattr(pages.cache, n).view(torch.uint8), before[n].view(torch.uint8)) for n in before)
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------
+
+def run_tokens(fn, pages, new, heads, kv_heads, dim, dtype, window, scale=None, seed=3, sharp=1.5, tensor_cores=False, check=True):
+    """Sequence i's last new[i] tokens attend; `fn(qkv, q_off, table, slot, pos, out, scale, dev_err)`."""
+    gen = torch.Generator().manual_seed(seed)
+    T = sum(new)
+    scale = 1 / math.sqrt(dim) if scale is None else scale
+    qkv = (torch.randn((T, (heads + 2 * kv_heads) * dim), generator=gen) * sharp).to(dtype)
+    slot = torch.tensor([i for i, a in enumerate(new) for _ in range(a)], dtype=torch.int32)
+    pos = torch.tensor([n - a + j for a, n in zip(new, pages.lengths) for j in range(a)], dtype=torch.int32)
+    out = torch.full((T, heads * dim), 3.0, dtype=dtype, device=DEV)
+    e = err_word()
+    fn(qkv.to(DEV), 0, pages.table.to(DEV), slot.to(DEV), pos.to(DEV), out, scale, e)
+    assert int(e.item()) == 0
+    if not check:
+        return out
+    contexts = [pages.context(i) for i in range(len(new))]
+    worst = 0.0
+    for t in range(T):
+        i, p = int(slot[t]), int(pos[t])
+        q = qkv[t, :heads * dim].double().view(heads, dim)
+        want = plain.attend(q, contexts[i][0], contexts[i][1], scale, window, p)
+        tol = bound(pages, i, p, max(0, p - window + 1) if window else 0, q, scale, want, dtype, tensor_cores)
+        off = (out[t].double().cpu().view(heads, dim) - want).abs()
+        assert bool((off <= tol).all()), (t, i, p, float(off.max()), float(tol.max()))
+        worst = max(worst, float((off / tol).max()))
+    return out, worst
+
+
+SHAPES = [(3, 3, 64), (8, 2, 128), (4, 1, 32), (5, 5, 16), (2, 2, 80), (6, 3, 96), (2, 1, 256), (2, 2, 192), (12, 1, 64), (24, 1, 128)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,dim", SHAPES)
+@pytest.mark.parametrize("window", [0, 1, 37])
+def test_general_attention(dtype, heads, kv_heads, dim, window):
+    from vlrf_b200.csrc import ops
+    pages = Pages([1, 64, 65, 200], kv_heads, dim, seed=heads)
+    run_tokens(lambda qkv, q_off, table, slot, pos, out, scale, e: ops.attention_packed(
+        qkv, q_off, pages.cache, table, slot, pos, out, slot.numel(), heads, kv_heads, dim, scale, window, e),
+        pages, [1, 1, 2, 5], heads, kv_heads, dim, dtype, window)
+
+
+def test_general_attention_skips_padding_and_reports_missing_blocks():
+    from vlrf_b200.csrc import ops
+    pages = Pages([100], 2, 64)
+    qkv = torch.randn(3, 6 * 64, device=DEV)
+    out = torch.full((3, 128), 8.0, device=DEV)
+    slot, pos = torch.tensor([-1, 0, -1], dtype=torch.int32, device=DEV), torch.tensor([5, 99, 0], dtype=torch.int32, device=DEV)
+    e = err_word()
+    ops.attention_packed(qkv, 0, pages.cache, pages.table.to(DEV), slot, pos, out, 3, 2, 2, 64, 0.125, 0, e)
+    assert bool((out[0] == 8).all()) and bool((out[2] == 8).all()) and not bool((out[1] == 8).all()) and int(e.item()) == 0
+    pos[1] = 200                              # beyond the sequence's blocks
+    ops.attention_packed(qkv, 0, pages.cache, pages.table.to(DEV), slot, pos, out, 3, 2, 2, 64, 0.125, 0, e)
+    assert int(e.item()) == 4
+
+
+def test_refusals():
+    from vlrf_b200.csrc import KernelError, ops
+    pages = Pages([70], 2, 64)
+    rows, table = torch.randn(4, 6 * 64, device=DEV), pages.table.to(DEV)
+    slot, pos, e = torch.zeros(4, dtype=torch.int32, device=DEV), torch.arange(4, dtype=torch.int32, device=DEV), err_word()
+    out = torch.empty(4, 128, device=DEV)
+
+    def append(**kw):
+        a = dict(qkv=rows, k_off=128, v_off=256, cache=pages.cache, block_table=table, tok_slot=slot, tok_pos=pos, n_tokens=4, n_kv_heads=2,
+                 head_dim=64, dev_err=e)
+        ops.kv_append_packed(**dict(a, **kw))
+
+    def attend(**kw):
+        a = dict(qkv=rows, q_off=0, cache=pages.cache, block_table=table, tok_slot=slot, tok_pos=pos, out=out, n_tokens=4, n_heads=2, n_kv_heads=2,
+                 head_dim=64, scale=0.125, window=0, dev_err=e)
+        ops.attention_packed(**dict(a, **kw))
+
+    append(); attend()
+    c = pages.cache
+    for call, kw in [(append, dict(qkv=rows.half())), (append, dict(qkv=rows.cpu())), (append, dict(k_off=-1)), (append, dict(v_off=257)),
+                     (append, dict(n_tokens=5)), (append, dict(head_dim=32)), (append, dict(head_dim=72)), (append, dict(n_kv_heads=1)),
+                     (append, dict(cache=None)), (append, dict(cache=ops.PackedKV(c.k, c.k_pairs.float(), c.v, c.v_pairs))),
+                     (append, dict(cache=ops.PackedKV(c.k, c.k_pairs, c.v[:1], c.v_pairs))), (append, dict(tok_pos=pos.long())),
+                     (append, dict(block_table=table[0])), (append, dict(qkv=rows.t())),
+                     (attend, dict(out=out.bfloat16())), (attend, dict(n_heads=3)), (attend, dict(q_off=400)), (attend, dict(window=-1)),
+                     (attend, dict(out=out[:3])), (attend, dict(qkv=rows[:2])), (attend, dict(cache=ops.PackedKV(c.k.cpu(), c.k_pairs, c.v, c.v_pairs)))]:
+        with pytest.raises(KernelError):
+            call(**kw)
+    with pytest.raises(KernelError):
+        ops.kv_read_packed(c, table, slot, pos, out[:, :64], out, 4, e)
+    with pytest.raises(KernelError):
+        ops.PackedKV.zeros(3, 2, 64, 24, DEV)

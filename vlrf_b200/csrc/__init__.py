@@ -190,6 +190,13 @@ _SIGNATURES = {
     "vlrf_attn_latent_mma": [_c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p,
                              _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p,
                              _c_void_p, _c_float, _c_void_p, _c_void_p],
+    "vlrf_packed_group": [_c_int],
+    "vlrf_packed_append": [_c_void_p, _c_int, _c_int, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
+                           _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    "vlrf_packed_read": [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int,
+                         _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    "vlrf_attn_packed": [_c_void_p, _c_int, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
+                         _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p],
     "vlrf_moe_route": [_c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                        _c_void_p, _c_int, _c_void_p],
     "vlrf_moe_route_scored": [_c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p,

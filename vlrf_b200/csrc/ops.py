@@ -6,6 +6,7 @@ no function has a CPU or library fallback.
 """
 from __future__ import annotations
 
+import dataclasses
 import os
 
 import torch
@@ -886,6 +887,148 @@ def attention_latent(qp, cache, C: int, R: int, block_table, tok_slot, tok_pos, 
     call("vlrf_attn_latent", _ptr(qp), dtype_code(qp.dtype), qp.shape[1], _ptr(cache), cache.shape[2], C, R, _ptr(block_table),
          block_table.shape[1], _ptr(tok_slot), _ptr(tok_pos), _ptr(out), out.shape[1], n_tokens, n_heads, cache.shape[1],
          float(scale), int(window), _ptr(sink), float(out_scale), _ptr(dev_err), _stream())
+
+
+# ---- a cache of keys and values in 4 bits -------------------------------------------------------------------------------
+
+def packed_group(head_dim: int) -> int:
+    """How many neighbouring entries of a head share a step and a zero in a cache of 4 bits: 64, 32 or 16; 0 where the head size is not
+    taken (those taken are the multiples of 16 up to 256)."""
+    if head_dim <= 0 or head_dim % HEAD_DIM_STEP != 0 or head_dim > HEAD_DIM_MAX:
+        return 0
+    return 64 if head_dim % 64 == 0 else 32 if head_dim % 32 == 0 else 16
+
+
+@dataclasses.dataclass(frozen=True)
+class PackedKV:
+    """One layer's paged keys and values in 4 bits a number (see the kernel library's header): codes uint8 [block, kv_head,
+    block_tokens, head_dim/2], entry 2c in the low half of byte c; pairs bfloat16 [block, kv_head, block_tokens, groups, 2], the step
+    and the zero of every group of `packed_group(head_dim)` entries.  A number is zero + step · code."""
+    k: torch.Tensor
+    k_pairs: torch.Tensor
+    v: torch.Tensor
+    v_pairs: torch.Tensor
+
+    @classmethod
+    def zeros(cls, n_blocks: int, n_kv_heads: int, block_tokens: int, head_dim: int, device) -> "PackedKV":
+        """A cache that reads back as zeros."""
+        group = packed_group(head_dim)
+        if group == 0:
+            raise KernelError(f"a cache in 4 bits takes head sizes that are multiples of {HEAD_DIM_STEP} up to {HEAD_DIM_MAX}, not {head_dim}")
+        at = (n_blocks, n_kv_heads, block_tokens)
+        codes = [torch.zeros(at + (head_dim // 2,), dtype=torch.uint8, device=device) for _ in range(2)]
+        pairs = [torch.zeros(at + (head_dim // group, 2), dtype=torch.bfloat16, device=device) for _ in range(2)]
+        return cls(codes[0], pairs[0], codes[1], pairs[1])
+
+    def bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.k_pairs, self.v, self.v_pairs))
+
+
+def _packed_args(what: str, cache: PackedKV, n_kv_heads: int, head_dim: int, *others) -> list:
+    """The cache's pointers and number of blocks, checked; `others`: tensors that must live on its device."""
+    if not isinstance(cache, PackedKV):
+        raise KernelError(f"{what}: the cache is a PackedKV, not {type(cache).__name__}")
+    group = packed_group(head_dim)
+    if group == 0:
+        raise KernelError(f"{what}: a cache in 4 bits takes head sizes that are multiples of {HEAD_DIM_STEP} up to {HEAD_DIM_MAX}, not {head_dim}")
+    for name, t, dtype in (("k", cache.k, torch.uint8), ("k_pairs", cache.k_pairs, torch.bfloat16), ("v", cache.v, torch.uint8),
+                           ("v_pairs", cache.v_pairs, torch.bfloat16)):
+        _dev(t, f"{what}: {name}", dtype)
+        if t.data_ptr() % 16 != 0:
+            raise KernelError(f"{what}: {name} must begin on 16 bytes")
+    shape = tuple(cache.k.shape)
+    if len(shape) != 4 or shape[1] != n_kv_heads or shape[3] * 2 != head_dim or tuple(cache.v.shape) != shape \
+            or tuple(cache.k_pairs.shape) != shape[:3] + (head_dim // group, 2) or cache.v_pairs.shape != cache.k_pairs.shape:
+        raise KernelError(f"{what}: cache shape does not match the heads")
+    _same_device(what, cache.k, cache.k_pairs, cache.v, cache.v_pairs, *others)
+    return [_ptr(cache.k), _ptr(cache.k_pairs), _ptr(cache.v), _ptr(cache.v_pairs), shape[0]]
+
+
+def _same_device(what: str, *tensors) -> None:
+    """All on one device, and that the current one: a launch goes to the current device's stream."""
+    devices = {t.device for t in tensors}
+    if len(devices) != 1 or next(iter(devices)).index != torch.cuda.current_device():
+        raise KernelError(f"{what}: every tensor must live on the current CUDA device")
+
+
+def _packed_table(what: str, block_table, tok_slot, tok_pos, dev_err, n_tokens: int) -> None:
+    _dev(block_table, f"{what}: block_table", torch.int32); _dev(tok_slot, f"{what}: tok_slot", torch.int32)
+    _dev(tok_pos, f"{what}: tok_pos", torch.int32); _dev(dev_err, f"{what}: dev_err", torch.int32)
+    if block_table.dim() != 2 or block_table.shape[1] == 0:
+        raise KernelError(f"{what}: the block table is [slots, blocks]")
+    if n_tokens < 0 or min(tok_slot.shape[0], tok_pos.shape[0]) < n_tokens:
+        raise KernelError(f"{what}: fewer slots or positions than tokens")
+
+
+def kv_append_packed(qkv, k_off: int, v_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, n_tokens: int, n_kv_heads: int,
+                     head_dim: int, dev_err) -> None:
+    """Quantise the K and V columns of qkv rows (float32 or bfloat16; qkv may be a range of columns of wider rows) into one layer's paged
+    cache of 4 bits.  Rows with slot −1 are skipped."""
+    what = "kv_append_packed"
+    _rows(qkv, f"{what}: qkv")
+    code = dtype_code(qkv.dtype)
+    _packed_table(what, block_table, tok_slot, tok_pos, dev_err, n_tokens)
+    args = _packed_args(what, cache, n_kv_heads, head_dim, qkv, block_table, tok_slot, tok_pos, dev_err)
+    if qkv.shape[0] < n_tokens:
+        raise KernelError(f"{what}: fewer rows than tokens")
+    if min(k_off, v_off) < 0 or max(k_off, v_off) + n_kv_heads * head_dim > qkv.shape[1]:
+        raise KernelError(f"{what}: K/V columns lie outside the row")
+    call("vlrf_packed_append", _ptr(qkv), code, qkv.stride(0), int(k_off), int(v_off), *args, _ptr(block_table), block_table.shape[1],
+         _ptr(tok_slot), _ptr(tok_pos), n_tokens, n_kv_heads, head_dim, cache.k.shape[2], _ptr(dev_err), _stream())
+
+
+def kv_read_packed(cache: PackedKV, block_table, tok_slot, tok_pos, out_k, out_v, n_tokens: int, dev_err) -> None:
+    """The tokens' keys and values out of a cache of 4 bits as plain rows [T, kv_heads·head_dim], float32 or bfloat16 (out_k and out_v
+    may be ranges of columns of wider rows); rows of padding tokens are zeros."""
+    what = "kv_read_packed"
+    if not isinstance(cache, PackedKV) or cache.k.dim() != 4:
+        raise KernelError(f"{what}: the cache is a PackedKV")
+    n_kv_heads, head_dim = cache.k.shape[1], 2 * cache.k.shape[3]
+    _rows(out_k, f"{what}: out_k"); _rows(out_v, f"{what}: out_v", out_k.dtype)
+    code = dtype_code(out_k.dtype)
+    _packed_table(what, block_table, tok_slot, tok_pos, dev_err, n_tokens)
+    args = _packed_args(what, cache, n_kv_heads, head_dim, out_k, out_v, block_table, tok_slot, tok_pos, dev_err)
+    if min(out_k.shape[1], out_v.shape[1]) != n_kv_heads * head_dim or max(out_k.shape[1], out_v.shape[1]) != n_kv_heads * head_dim \
+            or min(out_k.shape[0], out_v.shape[0]) < n_tokens:
+        raise KernelError(f"{what}: the output does not match")
+    call("vlrf_packed_read", *args, _ptr(block_table), block_table.shape[1], _ptr(tok_slot), _ptr(tok_pos), _ptr(out_k), out_k.stride(0),
+         _ptr(out_v), out_v.stride(0), code, n_tokens, n_kv_heads, head_dim, cache.k.shape[2], _ptr(dev_err), _stream())
+
+
+def attention_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, out, n_tokens: int, n_heads: int, n_kv_heads: int,
+                     head_dim: int, scale: float, window: int, dev_err) -> None:
+    """Each token's query attends the keys 0…position of its slot in a cache of 4 bits (window > 0: the last `window` of them), any mix of
+    tokens; rows with slot −1 are left as they are.  qkv and out may be ranges of columns of wider rows."""
+    args = _attention_packed_args("attention_packed", qkv, q_off, cache, block_table, tok_slot, tok_pos, out, n_tokens, n_heads, n_kv_heads,
+                                  head_dim, window, dev_err)
+    call("vlrf_attn_packed", _ptr(qkv), dtype_code(qkv.dtype), qkv.stride(0), int(q_off), *args, _ptr(block_table), block_table.shape[1],
+         _ptr(tok_slot), _ptr(tok_pos), _ptr(out), out.stride(0), n_tokens, n_heads, n_kv_heads, head_dim, cache.k.shape[2], float(scale),
+         int(window), _ptr(dev_err), _stream())
+
+
+def _attention_packed_args(what: str, qkv, q_off: int, cache, block_table, tok_slot, tok_pos, out, n_tokens: int, n_heads: int,
+                           n_kv_heads: int, head_dim: int, window: int, dev_err) -> list:
+    _rows(qkv, f"{what}: qkv"); _rows(out, f"{what}: out", qkv.dtype)
+    dtype_code(qkv.dtype)
+    _packed_table(what, block_table, tok_slot, tok_pos, dev_err, n_tokens)
+    args = _packed_args(what, cache, n_kv_heads, head_dim, qkv, out, block_table, tok_slot, tok_pos, dev_err)
+    if n_heads <= 0 or n_heads % n_kv_heads != 0:
+        raise KernelError(f"{what}: {n_heads} heads cannot share {n_kv_heads} key/value heads")
+    if out.shape[1] < n_heads * head_dim or out.shape[0] < n_tokens or qkv.shape[0] < n_tokens:
+        raise KernelError(f"{what}: output does not match")
+    if q_off < 0 or q_off + n_heads * head_dim > qkv.shape[1]:
+        raise KernelError(f"{what}: Q columns lie outside the row")
+    if window < 0:
+        raise KernelError(f"{what}: a window is positive, or 0 for none")
+    return args
+
+
+def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ctx, n_heads: int, n_kv_heads: int, head_dim: int,
+                          scale: float, window: int = 0) -> None:
+    """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
+    already holds the step's own keys and values."""
+    attention_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
+                     window, ctx.dev_err)
 
 
 # ---- routed experts --------------------------------------------------------------------------------------------------

@@ -448,6 +448,27 @@ int vlrf_attn_latent_mma(const void* qp, int ld_q, const void* cache, int row_w,
                          int n_seqs, int max_new, int H, int BT, float scale, int window, int n_split, float* partials,
                          const float* sink, float out_scale, int* dev_err, cudaStream_t stream);
 
+// ---- a cache of keys and values in 4 bits (packed_kv.cu, attention_packed.cu) ------------------------
+// A token's row of dh numbers of a head is cut into groups of vlrf_packed_group(dh) (64, 32 or 16; 0: a head size that is not taken:
+// those taken are the multiples of 16 up to 256).  A group is held as zero = its least number, rounded to bfloat16, step = (its largest −
+// zero) / 15, rounded once to bfloat16, and codes = (number − zero) / step, rounded once to 0 … 15; it reads back as zero + step ·
+// code.  A group with a number that is not finite reads back as NaN throughout.  The cache of one layer: codes Kq, Vq uint8 [n_blocks][Hkv]
+// [BT][dh/2] (entry 2c in the low half of byte c), pairs Kp, Vp bfloat16 [n_blocks][Hkv][BT][dh/group][2] (step, zero).  Block numbers
+// outside 0 … n_blocks − 1 are blocks that are not mapped (VLRF_DEVERR_NO_BLOCK).
+int vlrf_packed_group(int dh);
+// The new tokens' K and V columns into the cache; rows with slot −1 are skipped.
+int vlrf_packed_append(const void* qkv, int dtype, int ld, int k_off, int v_off, void* Kq, void* Kp, void* Vq, void* Vp, int n_blocks,
+                       const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, int T, int Hkv, int dh, int BT,
+                       int* dev_err, cudaStream_t stream);
+// The tokens' keys and values as plain rows out_k, out_v [T][Hkv·dh] of `dtype` (row strides ld_k, ld_v); rows of padding tokens are zeros.
+int vlrf_packed_read(const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table, int max_blocks,
+                     const int* tok_slot, const int* tok_pos, void* out_k, int ld_k, void* out_v, int ld_v, int dtype, int T, int Hkv,
+                     int dh, int BT, int* dev_err, cudaStream_t stream);
+// Attention as vlrf_attn_generic's, over the numbers that the cache stands for: any mix of tokens, float32 or bfloat16.
+int vlrf_attn_packed(const void* qkv, int dtype, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp,
+                     int n_blocks, const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out,
+                     int T, int H, int Hkv, int dh, int BT, float scale, int window, int* dev_err, cudaStream_t stream);
+
 // ---- routed experts (moe.cu) ---------------------------------------------------------------------------------------
 // z: float32 router logits [T][ld_z] (column E: the logit of a shared expert's gate, if shared_gate).  ids, wts, rank
 // [T][top]: the chosen experts (largest logits, ties to the lower index; −1 for padding rows), the softmax over the
