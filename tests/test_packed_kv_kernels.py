@@ -270,6 +270,75 @@ def test_general_attention_skips_padding_and_reports_missing_blocks():
     assert int(e.item()) == 4
 
 
+DECODE_SHAPES = [(3, 3, 64), (8, 2, 128), (2, 1, 256), (2, 2, 192), (12, 1, 64), (24, 1, 128), (40, 2, 64), (10, 1, 256)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", DECODE_SHAPES)
+@pytest.mark.parametrize("window", [0, 1, 70])
+@pytest.mark.parametrize("n_split", [1, 3, 16])
+def test_decode_attention_on_the_tensor_cores(heads, kv_heads, dim, window, n_split):
+    """Contexts of one token, of whole blocks, of a token more, longer than all stages of a warp's ring; more parts than tiles."""
+    from vlrf_b200.csrc import ops
+    pages = Pages([1, 64, 65, 130, 2000, 7], kv_heads, dim, seed=heads)
+    run_tokens(lambda qkv, q_off, table, slot, pos, out, scale, e: ops.attention_decode_packed(
+        qkv, q_off, pages.cache, table, slot, pos, out, slot.numel(), heads, kv_heads, dim, scale, window, n_split, e),
+        pages, [1] * 6, heads, kv_heads, dim, torch.bfloat16, window, tensor_cores=True)
+
+
+@pytest.mark.parametrize("scale,sharp", [(1.0, 4.0), (1e-4, 1.0), (0.125, 1e-20), (0.125, 1e4)])
+def test_decode_attention_with_sharp_and_flat_scores(scale, sharp):
+    """Scores of many sizes: one key takes all, all alike; queries near the ends of what they may be."""
+    from vlrf_b200.csrc import ops
+    pages = Pages([300, 900], 2, 64, seed=4)
+    run_tokens(lambda qkv, q_off, table, slot, pos, out, scale, e: ops.attention_decode_packed(
+        qkv, q_off, pages.cache, table, slot, pos, out, 2, 4, 2, 64, scale, 0, 2, e),
+        pages, [1, 1], 4, 2, 64, torch.bfloat16, 0, scale=scale, sharp=sharp, tensor_cores=True)
+
+
+def test_decode_attention_skips_padding_reports_missing_blocks_and_repeats_itself():
+    from vlrf_b200.csrc import ops
+    pages = Pages([500, 40, 1300], 3, 64)
+    qkv = torch.randn(5, 9 * 64, device=DEV).bfloat16()
+    slot = torch.tensor([-1, 2, 0, -1, 1], dtype=torch.int32, device=DEV)
+    pos = torch.tensor([5, 1299, 499, 0, 39], dtype=torch.int32, device=DEV)
+    table, e = pages.table.to(DEV), err_word()
+    outs = []
+    for n_split in (1, 4, 4):
+        out = torch.full((5, 192), 8.0, device=DEV, dtype=torch.bfloat16)
+        ops.attention_decode_packed(qkv, 0, pages.cache, table, slot, pos, out, 5, 3, 3, 64, 0.125, 0, n_split, e)
+        assert bool((out[0] == 8).all()) and bool((out[3] == 8).all()) and int(e.item()) == 0
+        outs.append(out)
+    assert torch.equal(outs[1], outs[2])
+    bad = table.clone()
+    bad[2, 7], bad[0, 1] = -1, pages.n_blocks        # a page in the middle that is not mapped, one outside the cache
+    ops.attention_decode_packed(qkv, 0, pages.cache, bad, slot, pos, outs[1], 5, 3, 3, 64, 0.125, 0, 4, e)
+    assert int(e.item()) == 4 and torch.equal(outs[1][4], outs[2][4])
+    pos[1] = 100_000
+    e.zero_()
+    ops.attention_decode_packed(qkv, 0, pages.cache, table, slot, pos, outs[1], 5, 3, 3, 64, 0.125, 0, 4, e)
+    assert int(e.item()) == 4
+
+
+def test_numbers_that_are_not_finite_show_in_their_rows_only():
+    """A visible key or value that is not a number makes its sequence's head NaN; hidden ones nothing (the pages' leftovers are NaN everywhere)."""
+    from vlrf_b200.csrc import ops
+    pages = Pages([200, 200], 2, 64)
+    blk = int(pages.table[0, 1])
+    pages.cache.k_pairs[blk, 0, 5] = float("nan")
+    blk = int(pages.table[1, 0])
+    pages.cache.v_pairs[blk, 1, 60] = float("nan")
+    qkv = torch.randn(2, 6 * 64, device=DEV).bfloat16()
+    slot, pos = torch.arange(2, dtype=torch.int32, device=DEV), torch.full((2,), 199, dtype=torch.int32, device=DEV)
+    for n_split, window in ((1, 0), (3, 0), (1, 50), (2, 140)):
+        out, general = [torch.zeros(2, 128, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+        ops.attention_decode_packed(qkv, 0, pages.cache, pages.table.to(DEV), slot, pos, out, 2, 2, 2, 64, 0.125, window, n_split, err_word())
+        ops.attention_packed(qkv, 0, pages.cache, pages.table.to(DEV), slot, pos, general, 2, 2, 2, 64, 0.125, window, err_word())
+        nan = torch.zeros(2, 128, dtype=torch.bool)
+        nan[0, :64] = window == 0 or window == 140   # position 69
+        nan[1, 64:] = window in (0, 140)             # position 60
+        assert torch.equal(torch.isnan(out.cpu()), nan) and torch.equal(torch.isnan(general.cpu()), nan), (n_split, window)
+
+
 def test_refusals():
     from vlrf_b200.csrc import KernelError, ops
     pages = Pages([70], 2, 64)

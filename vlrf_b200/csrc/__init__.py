@@ -197,6 +197,9 @@ _SIGNATURES = {
                          _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
     "vlrf_attn_packed": [_c_void_p, _c_int, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
                          _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p],
+    "vlrf_attn_packed_decode_takes": [_c_int] * 7,
+    "vlrf_attn_packed_decode": [_c_void_p, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
+                                _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_void_p],
     "vlrf_moe_route": [_c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                        _c_void_p, _c_int, _c_void_p],
     "vlrf_moe_route_scored": [_c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p,

@@ -1023,10 +1023,49 @@ def _attention_packed_args(what: str, qkv, q_off: int, cache, block_table, tok_s
     return args
 
 
+#: cached numbers in 4 bits on the tensor cores where the kernels take the sizes (off: the general kernel takes every step)
+PACKED_ATTENTION_MMA = True
+
+
+def _packed_decode_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
+    if qkv.dtype != torch.bfloat16 or not PACKED_ATTENTION_MMA or qkv.data_ptr() % 16 != 0 or out.data_ptr() % 16 != 0:
+        return False
+    from . import library
+    return bool(library().vlrf_attn_packed_decode_takes(n_heads, n_kv_heads, head_dim, cache.k.shape[2], qkv.stride(0), q_off, out.stride(0)))
+
+
+def packed_decode_splits(n_rows: int, n_heads: int, n_kv_heads: int, max_context: int, window: int = 0) -> int:
+    """Into how many parts a decode step over a cache of 4 bits cuts each context."""
+    forced = os.environ.get("VLRF_B200_DECODE_SPLITS")
+    if forced:
+        return max(1, min(16, int(forced)))
+    reach = min(max_context, window + 63) if window > 0 else max_context
+    share = n_heads // n_kv_heads
+    ctas = max(1, n_rows * n_kv_heads * (-(-share // 16)))
+    return max(1, min(16, (2 * sm_count()) // ctas, -(-reach // 256)))
+
+
+def attention_decode_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, out, n_rows: int, n_heads: int, n_kv_heads: int,
+                            head_dim: int, scale: float, window: int, n_split: int, dev_err) -> None:
+    """One bfloat16 query per row and head attends the keys 0…position of its slot in a cache of 4 bits, on the tensor cores; the context is
+    cut into n_split parts.  Rows with slot −1 are left as they are."""
+    what = "attention_decode_packed"
+    args = _attention_packed_args(what, qkv, q_off, cache, block_table, tok_slot, tok_pos, out, n_rows, n_heads, n_kv_heads, head_dim, window, dev_err)
+    if qkv.dtype != torch.bfloat16:
+        raise KernelError(f"{what}: bfloat16 only")
+    call("vlrf_attn_packed_decode", _ptr(qkv), qkv.stride(0), int(q_off), *args, _ptr(block_table), block_table.shape[1], _ptr(tok_slot), _ptr(tok_pos),
+         _ptr(out), out.stride(0), n_rows, n_heads, n_kv_heads, head_dim, cache.k.shape[2], float(scale), int(window), int(n_split), _ptr(dev_err),
+         _stream())
+
+
 def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ctx, n_heads: int, n_kv_heads: int, head_dim: int,
                           scale: float, window: int = 0) -> None:
     """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
     already holds the step's own keys and values."""
+    if ctx.max_new == 1 and _packed_decode_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
+        attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
+                                window, packed_decode_splits(ctx.n_tokens, n_heads, n_kv_heads, ctx.max_context, window), ctx.dev_err)
+        return
     attention_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
                      window, ctx.dev_err)
 

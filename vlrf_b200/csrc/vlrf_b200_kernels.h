@@ -448,7 +448,7 @@ int vlrf_attn_latent_mma(const void* qp, int ld_q, const void* cache, int row_w,
                          int n_seqs, int max_new, int H, int BT, float scale, int window, int n_split, float* partials,
                          const float* sink, float out_scale, int* dev_err, cudaStream_t stream);
 
-// ---- a cache of keys and values in 4 bits (packed_kv.cu, attention_packed.cu) ------------------------
+// ---- a cache of keys and values in 4 bits (packed_kv.cu, attention_packed.cu, attention_packed_decode.cu) -----
 // A token's row of dh numbers of a head is cut into groups of vlrf_packed_group(dh) (64, 32 or 16; 0: a head size that is not taken:
 // those taken are the multiples of 16 up to 256).  A group is held as zero = its least number, rounded to bfloat16, step = (its largest −
 // zero) / 15, rounded once to bfloat16, and codes = (number − zero) / step, rounded once to 0 … 15; it reads back as zero + step ·
@@ -468,6 +468,12 @@ int vlrf_packed_read(const void* Kq, const void* Kp, const void* Vq, const void*
 int vlrf_attn_packed(const void* qkv, int dtype, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp,
                      int n_blocks, const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out,
                      int T, int H, int Hkv, int dh, int BT, float scale, int window, int* dev_err, cudaStream_t stream);
+// A decode step of it on the tensor cores, bfloat16, head sizes 64, 128, 192 and 256, blocks of 64: one query a row (slot −1: skipped), every
+// context in n_split (up to 16) parts that meet in a cluster.
+int vlrf_attn_packed_decode_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out);
+int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
+                            const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows,
+                            int H, int Hkv, int dh, int BT, float scale, int window, int n_split, int* dev_err, cudaStream_t stream);
 
 // ---- routed experts (moe.cu) ---------------------------------------------------------------------------------------
 // z: float32 router logits [T][ld_z] (column E: the logit of a shared expert's gate, if shared_gate).  ids, wts, rank
