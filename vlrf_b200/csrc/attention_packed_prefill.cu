@@ -1,0 +1,581 @@
+// Prompt attention over a cache of keys and values in 4 bits (packed_kv.cuh) on the tcgen05 tensor cores: ragged, causal, with or without a
+// window, bfloat16, head sizes 64 and 128.
+//
+// A CTA takes GROUPS · 128 consecutive new tokens of one sequence and one head and walks the keys they see in blocks of BK (128 keys of
+// 64 numbers, 64 of 128) up to the diagonal.  Its warps have fixed jobs:
+//   producers      codes and pairs of a block from the cache into registers, a tile ahead; from there zero + step · code as bfloat16 (one rounding)
+//                  into a ring of four shared-memory slots, K and V in turn, in the 128-byte swizzle that the MMA reads.  A code becomes
+//                  a bfloat16 by a mask under the exponent of 128, less 128 (exact), two at a time; pairs of entries i and i + 4 of eight
+//                  stay neighbours, so the numbers of a row lie permuted, those of the queries likewise (the sum does not care), and the
+//                  result is put in order where it is written.  Rows that no query may see, behind the sequence's last token or in
+//                  blocks wholly before the window, are zeros and are not read;
+//   the MMA warp   S = Q·Kᵀ into tensor memory and, once the probabilities are there, O += P·V (P is the operand in tensor memory, V
+//                  is read as it lies, head dimension contiguous);
+//   softmax warps  eight a group of 128 queries: a query is one lane of tensor memory, and two threads have a half of a block's keys each;
+//                  running maximum and sum in float32, O scaled where a maximum grew.
+// With GROUPS = 2 two groups share every block that the producers take apart.
+//
+// Keys and values enter the products as bfloat16, so each is off by at most 2^-8 of itself beyond the cache's own rounding, as are the weights; scores,
+// sums and results stay in float32.  A value that is not a number must not meet the weight 0 of a query that does not see it (0 · NaN is
+// not 0): its row of V becomes zeros, and its key's row of K NaN instead, which the mask hides from the same queries; so a head's row that
+// sees it is NaN throughout.
+// Every wait is bounded; a CTA that gives up sets the device error word, waits (bounded) for its MMAs, frees its tensor memory and leaves.
+#include <type_traits>
+#include "common.cuh"
+#include "packed_kv.cuh"
+#include "tcgen05.cuh"
+
+namespace {
+constexpr int PP_CB = 64, PP_SLOTS = 4, PP_TILE = 16384;            // tokens of a cache block; slots of the ring, bytes of each
+constexpr int PP_PART_BLOCKS = 3, PP_MAX_PARTS = 16;
+constexpr __host__ __device__ int pp_bk(int DH) { return DH == 64 ? 128 : 64; }
+constexpr __host__ __device__ int pp_producers(int GROUPS) { return 2 * GROUPS; }
+constexpr __host__ __device__ int pp_threads(int GROUPS) { return (GROUPS * 8 + pp_producers(GROUPS) + 1) * 32; }
+constexpr __host__ __device__ int pp_part_floats(int DH) { return DH * 128 + 256; }
+
+__device__ __forceinline__ float pp_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// MN-major tile: rows of 64 elements (128 bytes, swizzled) are the operand's N, a row a step of its K; groups of 8 rows 1024 bytes apart, chunks of
+// 64 along N `chunk` bytes apart
+__device__ __forceinline__ uint64_t pp_desc_mn(const void* tile, uint32_t chunk) {
+    uint64_t d = 0;
+    d |= (uint64_t)((tsm(tile) >> 4) & 0x3FFF);
+    d |= (uint64_t)(chunk >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__host__ __device__ constexpr uint32_t pp_idesc_mn(int M, int N) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void pp_mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void pp_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+// eight codes of a word as bfloat16 numbers: entries (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ uint4 pp_numbers(uint32_t w, __nv_bfloat162 step, __nv_bfloat162 zero) {
+    uint32_t r[4];
+    const uint32_t magic = 0x43004300u;                             // 128, twice
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = ((w >> (4 * i)) & PK_LOW) | magic;
+        const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&magic));
+        const __nv_bfloat162 v = __hfma2(c, step, zero);
+        r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <int DH, int GROUPS>
+__global__ void __launch_bounds__(pp_threads(GROUPS), GROUPS == 1 ? 2 : 1)
+attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_off, const unsigned char* __restrict__ Kq, const uint32_t* __restrict__ Kp,
+                           const unsigned char* __restrict__ Vq, const uint32_t* __restrict__ Vp, int n_blocks, const int* __restrict__ block_table,
+                           int max_blocks, const int* __restrict__ seq_slot, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
+                           __nv_bfloat16* __restrict__ out, int ld_out, int H, int Hkv, float scale, int window, int n_parts, float* __restrict__ partials,
+                           int* __restrict__ counters, int n_tiles, int* __restrict__ dev_err) {
+    constexpr int BK = pp_bk(DH), ROWS = GROUPS * 128, NG = DH / 64, NPROD = pp_producers(GROUPS), SOFT = GROUPS * 8;
+    constexpr int Q_BYTES = 128 * DH * 2, ATOM_Q = 16384, ATOM_KV = BK * 128;    // a 64-number chunk of 128 queries / of a block
+    constexpr int HK = BK / 2, NC = HK / 32, HD = DH / 2;           // keys, chunks of 32 keys, and columns of O of a softmax thread
+    extern __shared__ unsigned char pp_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pp_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* q_tiles = smem;                                  // [GROUPS][NG][128][128 B]
+    unsigned char* kv_tiles = smem + GROUPS * Q_BYTES;              // [PP_SLOTS][NG][BK][128 B]: K_0, V_0, K_1, V_1, …
+    float* s_part = reinterpret_cast<float*>(kv_tiles + PP_SLOTS * PP_TILE);     // [GROUPS][2][2][128]
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(s_part + GROUPS * 512);       // [GROUPS]
+    uint64_t* full = q_full + GROUPS;
+    uint64_t* empty = full + PP_SLOTS;
+    uint64_t* s_full = empty + PP_SLOTS;                            // [GROUPS] each from here
+    uint64_t* s_read = s_full + GROUPS;
+    uint64_t* p_full = s_read + GROUPS;
+    uint64_t* o_full = p_full + GROUPS;
+    uint64_t* drained = o_full + GROUPS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
+    int* s_never = s_abort + 1;                                     // stays 0: for waits that nothing calls off
+    int* s_last = s_never + 1;                                      // [GROUPS]: whether this CTA merges its tile's parts
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // z is the slowest index of the order in which CTAs are started: first parts first, and within a part long tiles first
+    const int part = blockIdx.z / n_tiles, qt = n_tiles - 1 - blockIdx.z % n_tiles, seq = blockIdx.y, h = blockIdx.x;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < PP_SLOTS; ++i) { tbar_init(&full[i], NPROD); tbar_init(&empty[i], 1); }
+        for (int g = 0; g < GROUPS; ++g) {
+            tbar_init(&q_full[g], 8);
+            tbar_init(&s_full[g], 1);
+            tbar_init(&s_read[g], 8);
+            tbar_init(&p_full[g], 8);
+            tbar_init(&o_full[g], 1);
+            s_last[g] = 1;
+        }
+        tbar_init(drained, 1);
+        *s_abort = 0;
+        *s_never = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    constexpr uint32_t TMEM_COLS = 256 * GROUPS;                    // a group: S BK columns, O DH, P BK / 2 (two bfloat16 a column)
+    if (warp == SOFT) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tsm(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    const int row0 = seq_start[seq], n_new = seq_start[seq + 1] - row0, slot = seq_slot[seq], pos0 = seq_pos0[seq];
+    const int hk = h / (H / Hkv);
+    const int t_first = qt * ROWS, q_first = pos0 + t_first;        // the tile's first query, in the step and in the sequence
+    const int n_rows = min(n_new - t_first, ROWS), q_last = q_first + n_rows - 1;
+    const int first_key = window > 0 ? max(0, q_first - window + 1) : 0;
+    const int kb_first = first_key / BK, n_kb = q_last / BK - kb_first + 1;
+    // the tile's key blocks are dealt to tile_parts CTAs; the others of its n_parts have nothing to do
+    const int tile_parts = max(1, min(n_parts, (n_kb + PP_PART_BLOCKS - 1) / PP_PART_BLOCKS));
+    const bool active = n_rows > 0 && slot >= 0 && pos0 >= 0 && part < tile_parts;      // uniform over the CTA
+    const int my_first = kb_first + part * n_kb / tile_parts;
+    const int my_n = active ? kb_first + (part + 1) * n_kb / tile_parts - my_first : 0, my_end = my_first + my_n;
+    // the blocks of group g: lo … hi − 1 (a group without rows: none)
+    int lo[GROUPS], hi[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        const int qf = q_first + g * 128, rows = min(n_rows - g * 128, 128);
+        lo[g] = max(my_first, (window > 0 ? max(0, qf - window + 1) : 0) / BK);
+        hi[g] = rows > 0 ? min(my_end, (qf + rows - 1) / BK + 1) : lo[g];
+        hi[g] = my_n > 0 ? max(hi[g], lo[g]) : lo[g];
+    }
+    const int* table = block_table + (size_t)max(slot, 0) * max_blocks;
+
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= SOFT && warp < SOFT + NPROD) {
+        // ---- producers: warp p has rows p · PR … of every block
+        constexpr int PR = BK / NPROD, UNITS = PR * (DH / 32) / 32; // a unit: 32 entries of a row (16 bytes of codes); so many a lane
+        const int p = warp - SOFT;
+        const int n_exist = pos0 + n_new;                           // tokens that the cache holds
+        uint4 codes[UNITS];
+        uint32_t pairs[UNITS];
+        // tile t of this CTA: block my_first + t / 2, K or V
+        auto fetch = [&](int t) {
+            const int k0 = (my_first + (t >> 1)) * BK;
+            const unsigned char* src = (t & 1) ? Vq : Kq;
+            const uint32_t* psrc = (t & 1) ? Vp : Kp;
+            const int cb = (k0 + p * PR) / PP_CB;                   // (a warp's rows lie in one cache block)
+            const bool wanted = k0 + p * PR < n_exist && (cb + 1) * PP_CB > first_key;
+            const int blk = wanted ? packed_block(table, max_blocks, n_blocks, cb) : -1;
+            if (wanted && blk < 0 && lane == 0) atomicOr(dev_err, VLRF_DEVERR_NO_BLOCK);
+            const size_t at = ((size_t)max(blk, 0) * Hkv + hk) * PP_CB + (k0 + p * PR) % PP_CB;
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const int u = i * 32 + lane, r = u / (DH / 32), c = u % (DH / 32);
+                codes[i] = make_uint4(0u, 0u, 0u, 0u);
+                pairs[i] = 0u;
+                if (blk >= 0 && k0 + p * PR + r < n_exist) {
+                    codes[i] = *reinterpret_cast<const uint4*>(src + (at + r) * (DH / 2) + c * 16);
+                    pairs[i] = psrc[(at + r) * NG + c / 2];
+                    // (NaN in a value's pair, both halves of it: zeros in V, NaN in K)
+                    const uint32_t other = (t & 1) ? pairs[i] : Vp[(at + r) * NG + c / 2];
+                    if ((other & 0x7fffu) > 0x7f80u) pairs[i] = (t & 1) ? 0u : 0x7fff7fffu;
+                }
+            }
+        };
+        bool ok = true;
+        if (my_n > 0) fetch(0);
+        for (int t = 0; t < 2 * my_n; ++t) {
+            const int sl = t % PP_SLOTS, use = t / PP_SLOTS;
+            if (use >= 1 && !tbar_wait_warp(&empty[sl], (uint32_t)((use - 1) & 1), s_abort)) { ok = false; break; }
+            unsigned char* tile = kv_tiles + (size_t)sl * PP_TILE;
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const int u = i * 32 + lane, r = p * PR + u / (DH / 32), c = u % (DH / 32);
+                const uint32_t s2 = __byte_perm(pairs[i], 0, 0x1010), z2 = __byte_perm(pairs[i], 0, 0x3232);
+                const __nv_bfloat162 step = *reinterpret_cast<const __nv_bfloat162*>(&s2), zero = *reinterpret_cast<const __nv_bfloat162*>(&z2);
+                unsigned char* dst = tile + (c >> 1) * ATOM_KV + r * 128;
+                const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<uint4*>(dst + ((((c & 1) * 4 + j) ^ (r & 7)) << 4)) = pp_numbers(w[j], step, zero);
+            }
+            if (t + 1 < 2 * my_n) fetch(t + 1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the MMA reads them
+            __syncwarp();
+            if (lane == 0) tbar_arrive(&full[sl]);
+        }
+        if (!ok) atomicExch(s_abort, 1);
+    } else if (warp == SOFT + NPROD) {
+        // ---- MMAs
+        if (my_n > 0) {
+            constexpr uint32_t idesc_s = umma_idesc_bf16(128, BK), idesc_o = pp_idesc_mn(128, DH);
+            const uint64_t dq0 = umma_desc_k128(q_tiles), dk0 = umma_desc_k128(kv_tiles), dv0 = pp_desc_mn(kv_tiles, ATOM_KV);
+            bool ok = true;
+            auto issue_s = [&](int j) -> bool {                     // S_j = Q · K_jᵀ of every group that sees block j
+                const uint32_t t = 2u * (j - my_first), sl = t % PP_SLOTS;
+                if (!tbar_wait_warp(&full[sl], (t / PP_SLOTS) & 1u, s_abort)) return false;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    if (j < lo[g] || j >= hi[g]) continue;
+                    const int i = j - lo[g];
+                    if (!tbar_wait_warp(i == 0 ? &q_full[g] : &s_read[g], i == 0 ? 0u : (uint32_t)((i - 1) & 1), s_abort)) return false;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < DH / 16; ++k)
+                            umma_bf16(tmem + g * 256, dq0 + (uint64_t)((g * Q_BYTES + (k >> 2) * ATOM_Q) >> 4) + 2 * (k & 3),
+                                      dk0 + (uint64_t)((sl * PP_TILE + (k >> 2) * ATOM_KV) >> 4) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
+                        umma_commit(&s_full[g]);
+                    }
+                    __syncwarp();
+                }
+                if (elect_one()) umma_commit(&empty[sl]);
+                __syncwarp();
+                return true;
+            };
+            ok = issue_s(my_first);
+            for (int j = my_first; j < my_end && ok; ++j) {
+                if (j + 1 < my_end && !issue_s(j + 1)) { ok = false; break; }
+                const uint32_t t = 2u * (j - my_first) + 1, sl = t % PP_SLOTS;
+                if (!tbar_wait_warp(&full[sl], (t / PP_SLOTS) & 1u, s_abort)) { ok = false; break; }
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    if (!ok || j < lo[g] || j >= hi[g]) continue;
+                    const int i = j - lo[g];
+                    if (!tbar_wait_warp(&p_full[g], (uint32_t)(i & 1), s_abort)) { ok = false; continue; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k)           // 16 keys a step: 8 columns of P, 16 rows of V
+                            pp_mma_ta(tmem + g * 256 + BK, tmem + g * 256 + BK + DH + 8u * k, dv0 + (uint64_t)((sl * PP_TILE + k * 16 * 128) >> 4), idesc_o,
+                                      (i > 0 || k > 0) ? 1u : 0u);
+                        umma_commit(&o_full[g]);
+                    }
+                    __syncwarp();
+                }
+                if (elect_one()) umma_commit(&empty[sl]);
+                __syncwarp();
+            }
+            if (!ok) atomicExch(s_abort, 1);
+        }
+    } else if (active) {
+        // ---- softmax warps: a lane of tensor memory is a query row; warps q and q + 4 of a group have a half of a block's keys each
+        const int g = warp >> 3, q = warp & 3, half = (warp >> 2) & 1, r = q * 32 + lane;
+        const int my_lo = GROUPS == 1 || g == 0 ? lo[0] : lo[GROUPS - 1], my_hi = GROUPS == 1 || g == 0 ? hi[0] : hi[GROUPS - 1], n_i = my_hi - my_lo;
+        const int group_first = q_first + g * 128, q_pos = group_first + r;
+        const int group_rows = n_rows - g * 128;                    // (may be none, or more than 128)
+        const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
+        const uint32_t tmem_s = tmem + g * 256 + lane_addr, tmem_o = tmem_s + BK, tmem_p = tmem_o + DH;
+        unsigned char* q_tile = q_tiles + g * Q_BYTES;
+        float* sp = s_part + g * 512;
+        const float sl2 = scale * 1.4426950408889634f;              // scores in units of log2(e)
+        const unsigned win_eff = window > 0 ? (unsigned)window : 0x7fffffffu;    // key visible: 0 ≤ q_pos − key < win_eff
+        if (n_i > 0) {
+            // the queries, eight entries a piece, in the producers' order
+            for (int idx = threadIdx.x & 255; idx < 128 * (DH / 8); idx += 256) {
+                const int rr = idx / (DH / 8), c = idx % (DH / 8);
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (rr < group_rows) v = *reinterpret_cast<const uint4*>(qkv + (size_t)(row0 + t_first + g * 128 + rr) * ld + q_off + (size_t)h * DH + c * 8);
+                *reinterpret_cast<uint4*>(q_tile + (c >> 3) * ATOM_Q + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) =
+                    make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tbar_arrive(&q_full[g]);
+        }
+        float m_run = -INFINITY, l_run = 0.f;                       // the row's maximum; the sum of this half
+        bool ok = true;
+        auto block = [&](int i, auto masked_c) {
+            constexpr bool MASKED = decltype(masked_c)::value;
+            const int k0 = (my_lo + i) * BK + half * HK;            // the half's first key
+            // chunks of 32 keys of which a row of this warp sees any (those behind lie above the diagonal)
+            const int q_top = group_first + q * 32 + 31;
+            const int n_live = MASKED ? (q_top < k0 ? 0 : min(NC, ((q_top - k0) >> 5) + 1)) : NC;
+            // (a warp that has given up goes on meeting its neighbour, who may not have)
+            if (!ok || !tbar_wait_warp(&s_full[g], (uint32_t)(i & 1), s_abort)) {
+                ok = false;
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+                return;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t s_at = tmem_s + (uint32_t)(half * HK);
+            uint32_t sv[NC][32];
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (!MASKED) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) tmem_ld32(s_at + 32u * c, sv[c]);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tbar_arrive(&s_read[g]);
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(sv[c][x]));
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < n_live; ++c) {
+                    tmem_ld32(s_at + (uint32_t)(c * 32), sv[0]);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    const int d0 = q_pos - (k0 + c * 32);           // q_pos − key for x = 0
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], (unsigned)(d0 - x) < win_eff ? __uint_as_float(sv[0][x]) : -INFINITY);
+                }
+            }
+            const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            sp[((i & 1) * 2 + half) * 128 + r] = m_half;
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+            const float m_new = fmaxf(m_run, fmaxf(m_half, sp[((i & 1) * 2 + (half ^ 1)) * 128 + r]) * sl2);
+            const float corr = m_run == -INFINITY ? 1.f : pp_exp2(m_run - m_new);        // (from −inf on the row's sums are 0 so far)
+            l_run *= corr;
+            m_run = m_new;
+            const float m_use = (m_run == -INFINITY) ? 0.f : m_run; // a row that sees nothing yet: every p is 0
+            if (i > 0) {                                            // O holds the blocks before, and P may be written again
+                if (!tbar_wait_warp(&o_full[g], (uint32_t)((i - 1) & 1), s_abort)) { ok = false; return; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            float sm4[4] = {0.f, 0.f, 0.f, 0.f};
+            auto chunk = [&](int c, const uint32_t (&x)[32]) {
+                uint32_t pk[16];
+                const int d0 = q_pos - (k0 + c * 32);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float p0 = pp_exp2(fmaf(__uint_as_float(x[e]), sl2, -m_use)), p1 = pp_exp2(fmaf(__uint_as_float(x[e + 1]), sl2, -m_use));
+                    if (MASKED) {
+                        p0 = (unsigned)(d0 - e) < win_eff ? p0 : 0.f;
+                        p1 = (unsigned)(d0 - e - 1) < win_eff ? p1 : 0.f;
+                    }
+                    sm4[e & 3] += p0;
+                    sm4[(e + 1) & 3] += p1;
+                    pk[e >> 1] = pack2(p0, p1);
+                }
+                pp_st16(tmem_p + (uint32_t)(half * (HK / 2) + c * 16), pk);
+            };
+            if (!MASKED) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) chunk(c, sv[c]);
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < NC; ++c) {
+                    if (c < n_live) {
+                        tmem_ld32(s_at + (uint32_t)(c * 32), sv[0]);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        chunk(c, sv[0]);
+                    } else {
+                        uint32_t none[16];
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) none[x] = 0u;
+                        pp_st16(tmem_p + (uint32_t)(half * (HK / 2) + c * 16), none);
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tbar_arrive(&s_read[g]);
+            }
+            l_run += (sm4[0] + sm4[1]) + (sm4[2] + sm4[3]);
+            if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {    // a row's maximum grew: its O (a half of the columns here) follows
+#pragma unroll
+                for (int d0 = 0; d0 < HD; d0 += 32) {
+                    uint32_t ov[32];
+                    tmem_ld32(tmem_o + (uint32_t)(half * HD + d0), ov);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) ov[x] = __float_as_uint(__uint_as_float(ov[x]) * corr);
+                    pp_st32(tmem_o + (uint32_t)(half * HD + d0), ov);
+                }
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tbar_arrive(&p_full[g]);
+        };
+        for (int i = 0; i < n_i; ++i) {
+            if (window > 0 || (my_lo + i) * BK + BK - 1 > group_first) block(i, std::true_type{});       // (uniform over the group)
+            else block(i, std::false_type{});
+        }
+        // the row's result of this half's columns, and the sum of both halves of the keys
+        float o_acc[HD];
+#pragma unroll
+        for (int d = 0; d < HD; ++d) o_acc[d] = 0.f;
+        if (n_i > 0) {
+            if (ok && tbar_wait_warp(&o_full[g], (uint32_t)((n_i - 1) & 1), s_abort)) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int d0 = 0; d0 < HD; d0 += 32) {
+                    uint32_t ov[32];
+                    tmem_ld32(tmem_o + (uint32_t)(half * HD + d0), ov);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o_acc[d0 + x] = __uint_as_float(ov[x]);
+                }
+            } else {
+                ok = false;
+                atomicExch(s_abort, 1);
+            }
+        }
+        asm volatile("bar.sync %0, 256;" ::"r"(9 + g) : "memory");  // (also behind the last block's maxima)
+        sp[half * 128 + r] = l_run;
+        asm volatile("bar.sync %0, 256;" ::"r"(9 + g) : "memory");
+        l_run = sp[r] + sp[128 + r];
+        bool writes_out = true;
+        if (tile_parts > 1 && group_rows > 0) {
+            // leave this part's result in scratch ([d][row], so that a warp writes whole lines), then see whether the tile's other
+            // parts are all there
+            const size_t tile_id = (((size_t)seq * H + h) * n_tiles + qt) * GROUPS + g;
+            float* mine = partials + (tile_id * n_parts + part) * pp_part_floats(DH);
+#pragma unroll
+            for (int d = 0; d < HD; ++d) mine[(half * HD + d) * 128 + r] = o_acc[d];
+            if (half == 0) {
+                mine[DH * 128 + r] = m_run;
+                mine[DH * 128 + 128 + r] = l_run;
+            }
+            __threadfence();
+            asm volatile("bar.sync %0, 256;" ::"r"(9 + g) : "memory");
+            if ((threadIdx.x & 255) == 0) {
+                const int before = atomicAdd(&counters[tile_id], 1);
+                s_last[g] = (before == tile_parts - 1) ? 1 : 0;
+                if (before == tile_parts - 1) counters[tile_id] = 0;             // left as it was found
+            }
+            asm volatile("bar.sync %0, 256;" ::"r"(9 + g) : "memory");
+            writes_out = s_last[g] != 0;
+            if (writes_out) {
+                __threadfence();
+                // every part in turn, this CTA's own included: the sum does not depend on who came last
+                m_run = -INFINITY; l_run = 0.f;
+#pragma unroll
+                for (int d = 0; d < HD; ++d) o_acc[d] = 0.f;
+                for (int pt = 0; pt < tile_parts; ++pt) {
+                    const float* theirs = partials + (tile_id * n_parts + pt) * pp_part_floats(DH);
+                    const float m_p = __ldcg(theirs + DH * 128 + r), l_p = __ldcg(theirs + DH * 128 + 128 + r);
+                    const float m_new = fmaxf(m_run, m_p), use = m_new == -INFINITY ? 0.f : m_new;
+                    const float a = (m_run == -INFINITY) ? 0.f : pp_exp2(m_run - use);
+                    const float b = (m_p == -INFINITY) ? (l_p != l_p ? 1.f : 0.f) : pp_exp2(m_p - use);  // (a part whose scores are all NaN keeps its NaN)
+                    l_run = fmaf(l_run, a, l_p * b);
+                    m_run = m_new;
+#pragma unroll
+                    for (int d0 = 0; d0 < HD; d0 += 16) {
+                        float v[16];
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) v[x] = __ldcg(theirs + (half * HD + d0 + x) * 128 + r);
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) o_acc[d0 + x] = fmaf(o_acc[d0 + x], a, v[x] * b);
+                    }
+                }
+            }
+        }
+        if (writes_out && group_rows > 0) {
+            // the row as bfloat16, entries in order again, into shared memory (Q's tile: no MMA reads it any more); then each warp writes
+            // whole rows, so that a store instruction fills whole lines
+            const float inv = (l_run > 0.f || l_run != l_run) ? 1.f / l_run : 0.f;
+            if (ok) {
+#pragma unroll
+                for (int d = 0; d < HD; d += 8) {
+                    uint4 pk;
+                    pk.x = pack2(o_acc[d] * inv, o_acc[d + 2] * inv); pk.y = pack2(o_acc[d + 4] * inv, o_acc[d + 6] * inv);
+                    pk.z = pack2(o_acc[d + 1] * inv, o_acc[d + 3] * inv); pk.w = pack2(o_acc[d + 5] * inv, o_acc[d + 7] * inv);
+                    const int c = (half * HD + d) >> 3;
+                    *reinterpret_cast<uint4*>(q_tile + (c >> 3) * ATOM_Q + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = pk;
+                }
+            }
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+            if (ok) {
+                constexpr int PIECES = DH / 8, AT_ONCE = 32 / PIECES;
+#pragma unroll
+                for (int it = 0; it < 16 / AT_ONCE; ++it) {
+                    const int rr = q * 32 + half * 16 + it * AT_ONCE + lane / PIECES, c = lane % PIECES;
+                    if (rr < group_rows) {
+                        const uint4 pk = *reinterpret_cast<const uint4*>(q_tile + (c >> 3) * ATOM_Q + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+                        *reinterpret_cast<uint4*>(out + (size_t)(row0 + t_first + g * 128 + rr) * ld_out + (size_t)h * DH + c * 8) = pk;
+                    }
+                }
+            }
+        }
+    }
+    // everyone meets here on every path; then the allocating warp gives the tensor memory back
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (*s_abort) {                                                 // MMAs under way read this CTA's shared memory: wait for them (bounded)
+        if (warp == SOFT + NPROD) {
+            if (elect_one()) umma_commit(drained);
+            __syncwarp();
+            tbar_wait_warp(drained, 0, s_never);
+        }
+        __syncthreads();
+    }
+    if (warp == SOFT) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    if (threadIdx.x == 0 && *s_abort) atomicOr(dev_err, VLRF_DEVERR_WAIT_TIMEOUT);
+}
+
+template <int DH, int GROUPS>
+int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
+              int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_seqs, int max_new, int H, int Hkv,
+              float scale, int window, int n_parts, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+    const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_SLOTS * PP_TILE + GROUPS * 512 * 4 + 32 * 8;
+    static DeviceMarks marks;
+    auto kern = attn_packed_prefill_kernel<DH, GROUPS>;
+    cudaError_t e = allow_shared_memory(marks, kern, smem);
+    if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_prefill: %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    const long long tiles = (max_new + GROUPS * 128 - 1) / (GROUPS * 128);
+    VLRF_REQUIRE(tiles * n_parts <= 65535, "attn_packed_prefill: %lld tiles of %d parts are too many for one launch", tiles, n_parts);
+    e = launch_chained(kern, dim3(H, n_seqs, (unsigned)(tiles * n_parts)), dim3(pp_threads(GROUPS)), smem, stream, (const __nv_bfloat16*)qkv, ld, q_off,
+                       (const unsigned char*)Kq, (const uint32_t*)Kp, (const unsigned char*)Vq, (const uint32_t*)Vp, n_blocks, block_table, max_blocks, seq_slot,
+                       seq_start, seq_pos0, (__nv_bfloat16*)out, ld_out, H, Hkv, scale, window, n_parts, partials, counters, (int)tiles, dev_err);
+    if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_prefill: %s", cudaGetErrorString(e));
+    return vlrf_check_launch("attn_packed_prefill");
+}
+}  // namespace
+
+extern "C" int vlrf_attn_packed_prefill_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out) {
+    return H > 0 && Hkv > 0 && H % Hkv == 0 && (dh == 64 || dh == 128) && BT == PP_CB && ld % 8 == 0 && q_off % 8 == 0 && ld_out % 8 == 0;
+}
+extern "C" int vlrf_attn_packed_prefill_max_parts() { return PP_MAX_PARTS; }
+
+// Scratch of a launch with n_parts > 1: float32 numbers of partials, int32 numbers of counters.
+extern "C" int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, int dh, int groups, int n_parts, long long* floats, long long* ints) {
+    VLRF_REQUIRE(n_seqs >= 0 && max_new >= 0 && H > 0 && (dh == 64 || dh == 128) && (groups == 1 || groups == 2) && n_parts >= 1, "attn_packed_prefill: bad sizes");
+    const long long tiles = (long long)((max_new + groups * 128 - 1) / (groups * 128)) * groups * n_seqs * H;
+    *floats = n_parts > 1 ? tiles * n_parts * pp_part_floats(dh) : 0;
+    *ints = n_parts > 1 ? tiles : 0;
+    return VLRF_OK;
+}
+
+extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
+                                        const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out,
+                                        int ld_out, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int groups, int n_parts,
+                                        float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+    VLRF_REQUIRE(vlrf_attn_packed_prefill_takes(H, Hkv, dh, BT, ld, q_off, ld_out),
+                 "attn_packed_prefill: %d heads over %d of %d, blocks of %d, row strides %d and %d are not taken", H, Hkv, dh, BT, ld, ld_out);
+    VLRF_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && max_new >= 0 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && dev_err != nullptr,
+                 "attn_packed_prefill: bad arguments");
+    VLRF_REQUIRE(groups == 1 || groups == 2, "attn_packed_prefill: %d groups of 128 queries a CTA (1 or 2)", groups);
+    VLRF_REQUIRE(n_parts >= 1 && n_parts <= PP_MAX_PARTS && (n_parts == 1 || (partials != nullptr && counters != nullptr)),
+                 "attn_packed_prefill: %d parts (1 to %d; more than one wants scratch)", n_parts, PP_MAX_PARTS);
+    for (const void* p : {qkv, Kq, Kp, Vq, Vp, (const void*)out})
+        VLRF_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "attn_packed_prefill: tensors begin on 16 bytes");
+    if (n_seqs == 0 || max_new == 0) return VLRF_OK;
+#define GO(DH, G) pp_launch<DH, G>(qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, seq_slot, seq_start, seq_pos0, out, ld_out, n_seqs, \
+                                   max_new, H, Hkv, scale, window, n_parts, partials, counters, dev_err, stream)
+    if (dh == 64) return groups == 1 ? GO(64, 1) : GO(64, 2);
+    return groups == 1 ? GO(128, 1) : GO(128, 2);
+#undef GO
+}

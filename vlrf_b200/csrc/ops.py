@@ -903,19 +903,36 @@ def packed_group(head_dim: int) -> int:
 class PackedKV:
     """One layer's paged keys and values in 4 bits a number (see the kernel library's header): codes uint8 [block, kv_head,
     block_tokens, head_dim/2], entry 2c in the low half of byte c; pairs bfloat16 [block, kv_head, block_tokens, groups, 2], the step
-    and the zero of every group of `packed_group(head_dim)` entries.  A number is zero + step · code."""
+    and the zero of every group of `packed_group(head_dim)` entries.  A number is zero + step · code.  The four tensors are checked
+    here, once; the functions below take it as a whole."""
     k: torch.Tensor
     k_pairs: torch.Tensor
     v: torch.Tensor
     v_pairs: torch.Tensor
 
+    def __post_init__(self):
+        shape = tuple(self.k.shape)
+        group = packed_group(2 * shape[3]) if len(shape) == 4 else 0
+        if group == 0:
+            raise KernelError(f"a cache in 4 bits is [block, kv_head, block_tokens, head_dim/2] with head sizes that are multiples of {HEAD_DIM_STEP} up "
+                              f"to {HEAD_DIM_MAX}, not {list(shape)}")
+        pairs = shape[:3] + (2 * shape[3] // group, 2)
+        for name, t, dtype, want in (("k", self.k, torch.uint8, shape), ("k_pairs", self.k_pairs, torch.bfloat16, pairs),
+                                     ("v", self.v, torch.uint8, shape), ("v_pairs", self.v_pairs, torch.bfloat16, pairs)):
+            if t.dtype != dtype or tuple(t.shape) != want or not t.is_contiguous() or t.data_ptr() % 16 != 0 or t.device != self.k.device:
+                raise KernelError(f"a cache in 4 bits: {name} must be {dtype} {list(want)}, contiguous, on 16 bytes and on one device with the others")
+        object.__setattr__(self, "n_blocks", shape[0])
+        object.__setattr__(self, "n_kv_heads", shape[1])
+        object.__setattr__(self, "block_tokens", shape[2])
+        object.__setattr__(self, "head_dim", 2 * shape[3])
+        object.__setattr__(self, "index", self.k.get_device())
+        object.__setattr__(self, "args", (self.k.data_ptr(), self.k_pairs.data_ptr(), self.v.data_ptr(), self.v_pairs.data_ptr(), shape[0]))
+
     @classmethod
     def zeros(cls, n_blocks: int, n_kv_heads: int, block_tokens: int, head_dim: int, device) -> "PackedKV":
         """A cache that reads back as zeros."""
-        group = packed_group(head_dim)
-        if group == 0:
-            raise KernelError(f"a cache in 4 bits takes head sizes that are multiples of {HEAD_DIM_STEP} up to {HEAD_DIM_MAX}, not {head_dim}")
         at = (n_blocks, n_kv_heads, block_tokens)
+        group = packed_group(head_dim) or head_dim or 1
         codes = [torch.zeros(at + (head_dim // 2,), dtype=torch.uint8, device=device) for _ in range(2)]
         pairs = [torch.zeros(at + (head_dim // group, 2), dtype=torch.bfloat16, device=device) for _ in range(2)]
         return cls(codes[0], pairs[0], codes[1], pairs[1])
@@ -924,40 +941,28 @@ class PackedKV:
         return sum(t.numel() * t.element_size() for t in (self.k, self.k_pairs, self.v, self.v_pairs))
 
 
-def _packed_args(what: str, cache: PackedKV, n_kv_heads: int, head_dim: int, *others) -> list:
-    """The cache's pointers and number of blocks, checked; `others`: tensors that must live on its device."""
+def _packed_check(what: str, cache: PackedKV, n_kv_heads: int, head_dim: int, block_table, tables, dev_err, n_tokens: int, rows) -> None:
+    """What every function over a cache of 4 bits asks of its arguments.  tables: int32 vectors of the step; rows: (name, matrix) whose
+    rows are contiguous.  A launch goes to the current device, so everything lives there."""
     if not isinstance(cache, PackedKV):
         raise KernelError(f"{what}: the cache is a PackedKV, not {type(cache).__name__}")
-    group = packed_group(head_dim)
-    if group == 0:
-        raise KernelError(f"{what}: a cache in 4 bits takes head sizes that are multiples of {HEAD_DIM_STEP} up to {HEAD_DIM_MAX}, not {head_dim}")
-    for name, t, dtype in (("k", cache.k, torch.uint8), ("k_pairs", cache.k_pairs, torch.bfloat16), ("v", cache.v, torch.uint8),
-                           ("v_pairs", cache.v_pairs, torch.bfloat16)):
-        _dev(t, f"{what}: {name}", dtype)
-        if t.data_ptr() % 16 != 0:
-            raise KernelError(f"{what}: {name} must begin on 16 bytes")
-    shape = tuple(cache.k.shape)
-    if len(shape) != 4 or shape[1] != n_kv_heads or shape[3] * 2 != head_dim or tuple(cache.v.shape) != shape \
-            or tuple(cache.k_pairs.shape) != shape[:3] + (head_dim // group, 2) or cache.v_pairs.shape != cache.k_pairs.shape:
+    at = cache.index
+    if at < 0 or at != torch.cuda.current_device():
+        raise KernelError(f"{what}: the cache must live on the current CUDA device (there is no CPU path)")
+    if cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim:
         raise KernelError(f"{what}: cache shape does not match the heads")
-    _same_device(what, cache.k, cache.k_pairs, cache.v, cache.v_pairs, *others)
-    return [_ptr(cache.k), _ptr(cache.k_pairs), _ptr(cache.v), _ptr(cache.v_pairs), shape[0]]
-
-
-def _same_device(what: str, *tensors) -> None:
-    """All on one device, and that the current one: a launch goes to the current device's stream."""
-    devices = {t.device for t in tensors}
-    if len(devices) != 1 or next(iter(devices)).index != torch.cuda.current_device():
-        raise KernelError(f"{what}: every tensor must live on the current CUDA device")
-
-
-def _packed_table(what: str, block_table, tok_slot, tok_pos, dev_err, n_tokens: int) -> None:
-    _dev(block_table, f"{what}: block_table", torch.int32); _dev(tok_slot, f"{what}: tok_slot", torch.int32)
-    _dev(tok_pos, f"{what}: tok_pos", torch.int32); _dev(dev_err, f"{what}: dev_err", torch.int32)
+    for t in (block_table, dev_err, *tables):
+        if t.dtype != torch.int32 or t.get_device() != at or not t.is_contiguous():
+            raise KernelError(f"{what}: block table, slots, positions and error word are contiguous int32 tensors on the cache's device")
     if block_table.dim() != 2 or block_table.shape[1] == 0:
         raise KernelError(f"{what}: the block table is [slots, blocks]")
-    if n_tokens < 0 or min(tok_slot.shape[0], tok_pos.shape[0]) < n_tokens:
-        raise KernelError(f"{what}: fewer slots or positions than tokens")
+    if n_tokens < 0:
+        raise KernelError(f"{what}: a negative number of tokens")
+    for name, t in rows:
+        if t.get_device() != at or t.dim() != 2 or t.stride(1) != 1:
+            raise KernelError(f"{what}: {name} must be a matrix on the cache's device whose rows are contiguous")
+        if t.shape[0] < n_tokens:
+            raise KernelError(f"{what}: {name} has fewer rows than tokens")
 
 
 def kv_append_packed(qkv, k_off: int, v_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, n_tokens: int, n_kv_heads: int,
@@ -965,62 +970,56 @@ def kv_append_packed(qkv, k_off: int, v_off: int, cache: PackedKV, block_table, 
     """Quantise the K and V columns of qkv rows (float32 or bfloat16; qkv may be a range of columns of wider rows) into one layer's paged
     cache of 4 bits.  Rows with slot −1 are skipped."""
     what = "kv_append_packed"
-    _rows(qkv, f"{what}: qkv")
-    code = dtype_code(qkv.dtype)
-    _packed_table(what, block_table, tok_slot, tok_pos, dev_err, n_tokens)
-    args = _packed_args(what, cache, n_kv_heads, head_dim, qkv, block_table, tok_slot, tok_pos, dev_err)
-    if qkv.shape[0] < n_tokens:
-        raise KernelError(f"{what}: fewer rows than tokens")
+    _packed_check(what, cache, n_kv_heads, head_dim, block_table, (tok_slot, tok_pos), dev_err, n_tokens, (("qkv", qkv),))
+    if tok_slot.shape[0] < n_tokens or tok_pos.shape[0] < n_tokens:
+        raise KernelError(f"{what}: fewer slots or positions than tokens")
     if min(k_off, v_off) < 0 or max(k_off, v_off) + n_kv_heads * head_dim > qkv.shape[1]:
         raise KernelError(f"{what}: K/V columns lie outside the row")
-    call("vlrf_packed_append", _ptr(qkv), code, qkv.stride(0), int(k_off), int(v_off), *args, _ptr(block_table), block_table.shape[1],
-         _ptr(tok_slot), _ptr(tok_pos), n_tokens, n_kv_heads, head_dim, cache.k.shape[2], _ptr(dev_err), _stream())
+    call("vlrf_packed_append", qkv.data_ptr(), dtype_code(qkv.dtype), qkv.stride(0), k_off, v_off, *cache.args, block_table.data_ptr(),
+         block_table.shape[1], tok_slot.data_ptr(), tok_pos.data_ptr(), n_tokens, n_kv_heads, head_dim, cache.block_tokens, dev_err.data_ptr(), _stream())
 
 
 def kv_read_packed(cache: PackedKV, block_table, tok_slot, tok_pos, out_k, out_v, n_tokens: int, dev_err) -> None:
     """The tokens' keys and values out of a cache of 4 bits as plain rows [T, kv_heads·head_dim], float32 or bfloat16 (out_k and out_v
     may be ranges of columns of wider rows); rows of padding tokens are zeros."""
     what = "kv_read_packed"
-    if not isinstance(cache, PackedKV) or cache.k.dim() != 4:
-        raise KernelError(f"{what}: the cache is a PackedKV")
-    n_kv_heads, head_dim = cache.k.shape[1], 2 * cache.k.shape[3]
-    _rows(out_k, f"{what}: out_k"); _rows(out_v, f"{what}: out_v", out_k.dtype)
-    code = dtype_code(out_k.dtype)
-    _packed_table(what, block_table, tok_slot, tok_pos, dev_err, n_tokens)
-    args = _packed_args(what, cache, n_kv_heads, head_dim, out_k, out_v, block_table, tok_slot, tok_pos, dev_err)
-    if min(out_k.shape[1], out_v.shape[1]) != n_kv_heads * head_dim or max(out_k.shape[1], out_v.shape[1]) != n_kv_heads * head_dim \
-            or min(out_k.shape[0], out_v.shape[0]) < n_tokens:
-        raise KernelError(f"{what}: the output does not match")
-    call("vlrf_packed_read", *args, _ptr(block_table), block_table.shape[1], _ptr(tok_slot), _ptr(tok_pos), _ptr(out_k), out_k.stride(0),
-         _ptr(out_v), out_v.stride(0), code, n_tokens, n_kv_heads, head_dim, cache.k.shape[2], _ptr(dev_err), _stream())
+    if not isinstance(cache, PackedKV):
+        raise KernelError(f"{what}: the cache is a PackedKV, not {type(cache).__name__}")
+    width = cache.n_kv_heads * cache.head_dim
+    _packed_check(what, cache, cache.n_kv_heads, cache.head_dim, block_table, (tok_slot, tok_pos), dev_err, n_tokens, (("out_k", out_k), ("out_v", out_v)))
+    if tok_slot.shape[0] < n_tokens or tok_pos.shape[0] < n_tokens:
+        raise KernelError(f"{what}: fewer slots or positions than tokens")
+    if out_k.shape[1] != width or out_v.shape[1] != width or out_v.dtype != out_k.dtype:
+        raise KernelError(f"{what}: the outputs are [tokens, kv_heads·head_dim] of one dtype")
+    call("vlrf_packed_read", *cache.args, block_table.data_ptr(), block_table.shape[1], tok_slot.data_ptr(), tok_pos.data_ptr(), out_k.data_ptr(),
+         out_k.stride(0), out_v.data_ptr(), out_v.stride(0), dtype_code(out_k.dtype), n_tokens, cache.n_kv_heads, cache.head_dim, cache.block_tokens,
+         dev_err.data_ptr(), _stream())
+
+
+def _attention_packed_check(what: str, qkv, q_off: int, cache, block_table, tables, out, n_tokens: int, n_heads: int, n_kv_heads: int,
+                            head_dim: int, window: int, dev_err) -> None:
+    _packed_check(what, cache, n_kv_heads, head_dim, block_table, tables, dev_err, n_tokens, (("qkv", qkv), ("out", out)))
+    if n_heads <= 0 or n_heads % n_kv_heads != 0:
+        raise KernelError(f"{what}: {n_heads} heads cannot share {n_kv_heads} key/value heads")
+    if out.dtype != qkv.dtype or out.shape[1] < n_heads * head_dim:
+        raise KernelError(f"{what}: output does not match")
+    if q_off < 0 or q_off + n_heads * head_dim > qkv.shape[1]:
+        raise KernelError(f"{what}: Q columns lie outside the row")
+    if window < 0:
+        raise KernelError(f"{what}: a window is positive, or 0 for none")
 
 
 def attention_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, out, n_tokens: int, n_heads: int, n_kv_heads: int,
                      head_dim: int, scale: float, window: int, dev_err) -> None:
     """Each token's query attends the keys 0…position of its slot in a cache of 4 bits (window > 0: the last `window` of them), any mix of
     tokens; rows with slot −1 are left as they are.  qkv and out may be ranges of columns of wider rows."""
-    args = _attention_packed_args("attention_packed", qkv, q_off, cache, block_table, tok_slot, tok_pos, out, n_tokens, n_heads, n_kv_heads,
-                                  head_dim, window, dev_err)
-    call("vlrf_attn_packed", _ptr(qkv), dtype_code(qkv.dtype), qkv.stride(0), int(q_off), *args, _ptr(block_table), block_table.shape[1],
-         _ptr(tok_slot), _ptr(tok_pos), _ptr(out), out.stride(0), n_tokens, n_heads, n_kv_heads, head_dim, cache.k.shape[2], float(scale),
-         int(window), _ptr(dev_err), _stream())
-
-
-def _attention_packed_args(what: str, qkv, q_off: int, cache, block_table, tok_slot, tok_pos, out, n_tokens: int, n_heads: int,
-                           n_kv_heads: int, head_dim: int, window: int, dev_err) -> list:
-    _rows(qkv, f"{what}: qkv"); _rows(out, f"{what}: out", qkv.dtype)
-    dtype_code(qkv.dtype)
-    _packed_table(what, block_table, tok_slot, tok_pos, dev_err, n_tokens)
-    args = _packed_args(what, cache, n_kv_heads, head_dim, qkv, out, block_table, tok_slot, tok_pos, dev_err)
-    if n_heads <= 0 or n_heads % n_kv_heads != 0:
-        raise KernelError(f"{what}: {n_heads} heads cannot share {n_kv_heads} key/value heads")
-    if out.shape[1] < n_heads * head_dim or out.shape[0] < n_tokens or qkv.shape[0] < n_tokens:
-        raise KernelError(f"{what}: output does not match")
-    if q_off < 0 or q_off + n_heads * head_dim > qkv.shape[1]:
-        raise KernelError(f"{what}: Q columns lie outside the row")
-    if window < 0:
-        raise KernelError(f"{what}: a window is positive, or 0 for none")
-    return args
+    what = "attention_packed"
+    _attention_packed_check(what, qkv, q_off, cache, block_table, (tok_slot, tok_pos), out, n_tokens, n_heads, n_kv_heads, head_dim, window, dev_err)
+    if tok_slot.shape[0] < n_tokens or tok_pos.shape[0] < n_tokens:
+        raise KernelError(f"{what}: fewer slots or positions than tokens")
+    call("vlrf_attn_packed", qkv.data_ptr(), dtype_code(qkv.dtype), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1],
+         tok_slot.data_ptr(), tok_pos.data_ptr(), out.data_ptr(), out.stride(0), n_tokens, n_heads, n_kv_heads, head_dim, cache.block_tokens, float(scale),
+         window, dev_err.data_ptr(), _stream())
 
 
 #: cached numbers in 4 bits on the tensor cores where the kernels take the sizes (off: the general kernel takes every step)
@@ -1028,10 +1027,60 @@ PACKED_ATTENTION_MMA = True
 
 
 def _packed_decode_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
-    if qkv.dtype != torch.bfloat16 or not PACKED_ATTENTION_MMA or qkv.data_ptr() % 16 != 0 or out.data_ptr() % 16 != 0:
+    if not isinstance(cache, PackedKV) or qkv.dtype != torch.bfloat16 or not PACKED_ATTENTION_MMA or qkv.data_ptr() % 16 != 0 \
+            or out.data_ptr() % 16 != 0:
         return False
     from . import library
-    return bool(library().vlrf_attn_packed_decode_takes(n_heads, n_kv_heads, head_dim, cache.k.shape[2], qkv.stride(0), q_off, out.stride(0)))
+    return bool(library().vlrf_attn_packed_decode_takes(n_heads, n_kv_heads, head_dim, cache.block_tokens, qkv.stride(0), q_off, out.stride(0)))
+
+
+def _packed_prefill_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
+    if not isinstance(cache, PackedKV) or qkv.dtype != torch.bfloat16 or not PACKED_ATTENTION_MMA or qkv.data_ptr() % 16 != 0 \
+            or out.data_ptr() % 16 != 0:
+        return False
+    from . import library
+    return bool(library().vlrf_attn_packed_prefill_takes(n_heads, n_kv_heads, head_dim, cache.block_tokens, qkv.stride(0), q_off, out.stride(0)))
+
+
+def packed_prefill_shape(n_tokens: int, n_seqs: int, max_new: int, max_context: int, n_heads: int, head_dim: int, window: int = 0) -> tuple:
+    """(groups of 128 queries a CTA of `attention_prefill_packed` takes, parts to which it deals the keys of a long tile)."""
+    tiles = (n_tokens // 128 + n_seqs) * n_heads
+    keys = 128 if head_dim == 64 else 64
+    reach = min(max_context, window + 127) if window > 0 else max_context
+    chain = -(-reach // keys)
+    parts = max(1, min(16, (2 * sm_count()) // max(1, tiles), chain // 3))
+    return 1, parts
+
+
+def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_slot, seq_start, seq_pos0, out, n_tokens: int, n_seqs: int, max_new: int,
+                             n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int, dev_err, groups: int = 1, n_parts: int = 1,
+                             partials=None, counters=None) -> None:
+    """Causal attention of every sequence's new tokens (rows seq_start[i] … seq_start[i+1]−1 of qkv, the first of them at position
+    seq_pos0[i]) over the sequence's cache of 4 bits, which already holds these tokens; bfloat16, head size 64 or 128, on the tcgen05
+    tensor cores.  n_parts > 1 wants float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero."""
+    what = "attention_prefill_packed"
+    _attention_packed_check(what, qkv, q_off, cache, block_table, (seq_slot, seq_start, seq_pos0), out, n_tokens, n_heads, n_kv_heads, head_dim, window,
+                            dev_err)
+    if qkv.dtype != torch.bfloat16 or seq_slot.shape[0] < n_seqs or seq_start.shape[0] < n_seqs + 1 or seq_pos0.shape[0] < n_seqs:
+        raise KernelError(f"{what}: bfloat16 rows, and a slot, a first row and a first position for every sequence")
+    if n_parts > 1:
+        _dev(partials, f"{what}: partials", torch.float32); _dev(counters, f"{what}: counters", torch.int32)
+        want = packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts)
+        if partials.numel() < want[0] or counters.numel() < want[1]:
+            raise KernelError(f"{what}: scratch is too small for {n_parts} parts")
+    call("vlrf_attn_packed_prefill", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], seq_slot.data_ptr(),
+         seq_start.data_ptr(), seq_pos0.data_ptr(), out.data_ptr(), out.stride(0), n_seqs, max_new, n_heads, n_kv_heads, head_dim, cache.block_tokens,
+         float(scale), window, groups, n_parts, _ptr(partials) if n_parts > 1 else 0, _ptr(counters) if n_parts > 1 else 0, dev_err.data_ptr(), _stream())
+
+
+def packed_prefill_scratch(n_seqs: int, max_new: int, n_heads: int, head_dim: int, groups: int, n_parts: int) -> tuple:
+    """(float32 elements of `partials`, int32 elements of `counters`) that `attention_prefill_packed` wants for n_parts > 1."""
+    import ctypes
+
+    from . import call_host
+    floats, ints = ctypes.c_longlong(0), ctypes.c_longlong(0)
+    call_host("vlrf_attn_packed_prefill_scratch", n_seqs, max_new, n_heads, head_dim, groups, n_parts, ctypes.byref(floats), ctypes.byref(ints))
+    return floats.value, ints.value
 
 
 def packed_decode_splits(n_rows: int, n_heads: int, n_kv_heads: int, max_context: int, window: int = 0) -> int:
@@ -1050,12 +1099,12 @@ def attention_decode_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_s
     """One bfloat16 query per row and head attends the keys 0…position of its slot in a cache of 4 bits, on the tensor cores; the context is
     cut into n_split parts.  Rows with slot −1 are left as they are."""
     what = "attention_decode_packed"
-    args = _attention_packed_args(what, qkv, q_off, cache, block_table, tok_slot, tok_pos, out, n_rows, n_heads, n_kv_heads, head_dim, window, dev_err)
-    if qkv.dtype != torch.bfloat16:
-        raise KernelError(f"{what}: bfloat16 only")
-    call("vlrf_attn_packed_decode", _ptr(qkv), qkv.stride(0), int(q_off), *args, _ptr(block_table), block_table.shape[1], _ptr(tok_slot), _ptr(tok_pos),
-         _ptr(out), out.stride(0), n_rows, n_heads, n_kv_heads, head_dim, cache.k.shape[2], float(scale), int(window), int(n_split), _ptr(dev_err),
-         _stream())
+    _attention_packed_check(what, qkv, q_off, cache, block_table, (tok_slot, tok_pos), out, n_rows, n_heads, n_kv_heads, head_dim, window, dev_err)
+    if qkv.dtype != torch.bfloat16 or tok_slot.shape[0] < n_rows or tok_pos.shape[0] < n_rows:
+        raise KernelError(f"{what}: bfloat16 rows, each with a slot and a position")
+    call("vlrf_attn_packed_decode", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], tok_slot.data_ptr(),
+         tok_pos.data_ptr(), out.data_ptr(), out.stride(0), n_rows, n_heads, n_kv_heads, head_dim, cache.block_tokens, float(scale), window, n_split,
+         dev_err.data_ptr(), _stream())
 
 
 def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ctx, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -1065,6 +1114,16 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
     if ctx.max_new == 1 and _packed_decode_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
         attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
                                 window, packed_decode_splits(ctx.n_tokens, n_heads, n_kv_heads, ctx.max_context, window), ctx.dev_err)
+        return
+    if ctx.max_new > 1 and _packed_prefill_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
+        groups, n_parts = packed_prefill_shape(ctx.n_tokens, ctx.n_seqs, ctx.max_new, ctx.max_context, n_heads, head_dim, window)
+        partials = counters = None
+        if n_parts > 1:
+            n_floats, n_counters = packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts)
+            partials = ctx.ws.get("packed_partials", n_floats, 1, torch.float32)
+            counters = ctx.ws.get_zeroed("packed_counters", n_counters, torch.int32)
+        attention_prefill_packed(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_start, ctx.seq_pos0, out, ctx.n_tokens, ctx.n_seqs, ctx.max_new,
+                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, partials, counters)
         return
     attention_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
                      window, ctx.dev_err)

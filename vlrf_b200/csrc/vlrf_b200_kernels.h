@@ -448,7 +448,7 @@ int vlrf_attn_latent_mma(const void* qp, int ld_q, const void* cache, int row_w,
                          int n_seqs, int max_new, int H, int BT, float scale, int window, int n_split, float* partials,
                          const float* sink, float out_scale, int* dev_err, cudaStream_t stream);
 
-// ---- a cache of keys and values in 4 bits (packed_kv.cu, attention_packed.cu, attention_packed_decode.cu) -----
+// ---- a cache of keys and values in 4 bits (packed_kv.cu, attention_packed*.cu) -------------------------------
 // A token's row of dh numbers of a head is cut into groups of vlrf_packed_group(dh) (64, 32 or 16; 0: a head size that is not taken:
 // those taken are the multiples of 16 up to 256).  A group is held as zero = its least number, rounded to bfloat16, step = (its largest −
 // zero) / 15, rounded once to bfloat16, and codes = (number − zero) / step, rounded once to 0 … 15; it reads back as zero + step ·
@@ -474,6 +474,18 @@ int vlrf_attn_packed_decode_takes(int H, int Hkv, int dh, int BT, int ld, int q_
 int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                             const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows,
                             int H, int Hkv, int dh, int BT, float scale, int window, int n_split, int* dev_err, cudaStream_t stream);
+
+// A prompt step of it on the tcgen05 tensor cores, bfloat16, head sizes 64 and 128, blocks of 64: sequences as in vlrf_attn_prefill (slot −1:
+// skipped).  A CTA takes `groups` (1 or 2) times 128 queries of a head; n_parts > 1 deals the keys of long tiles to that many CTAs (up to
+// vlrf_attn_packed_prefill_max_parts()), which meet in scratch: float32 partials and int32 counters, zero before the first call (every
+// call leaves them zero), of the sizes that vlrf_attn_packed_prefill_scratch gives (host pointers).
+int vlrf_attn_packed_prefill_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out);
+int vlrf_attn_packed_prefill_max_parts();
+int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, int dh, int groups, int n_parts, long long* floats, long long* ints);
+int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
+                             const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0,
+                             void* out, int ld_out, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int groups,
+                             int n_parts, float* partials, int* counters, int* dev_err, cudaStream_t stream);
 
 // ---- routed experts (moe.cu) ---------------------------------------------------------------------------------------
 // z: float32 router logits [T][ld_z] (column E: the logit of a shared expert's gate, if shared_gate).  ids, wts, rank
