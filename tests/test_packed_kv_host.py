@@ -103,3 +103,47 @@ def test_no_cpu_path():
         ops.kv_read_packed(cache, t.view(1, 4), t, t, torch.zeros(4, 128), torch.zeros(4, 128), 4, t)
     with pytest.raises(KernelError):
         ops.attention_packed(torch.zeros(4, 384), 0, cache, t.view(1, 4), t, t, torch.zeros(4, 128), 4, 2, 2, 64, 0.125, 0, t)
+
+
+def test_cache_books_in_4_bits():
+    from vlrf_b200.cache import CacheError, KVNeed, LatentNeed, SequenceCache, StateNeed
+    c = SequenceCache([KVNeed(3, 64), KVNeed(3, 64), LatentNeed(48), (KVNeed(2, 32, "window", 100), StateNeed((4,))), None], max_tokens=256, max_seq_len=256,
+                      dtype=torch.bfloat16, device="cpu", kv_bits=4)
+    view = c.view(1)
+    assert view.k is None and view.packed.k.shape == (4, 3, 64, 32) and view.packed.k_pairs.shape == (4, 3, 64, 1, 2)
+    assert c.view(0).packed.k.data_ptr() != view.packed.k.data_ptr() and c.view(2).rows.dtype == torch.bfloat16
+    assert c.view(3).parts[0].packed.head_dim == 32 and c.view(3).parts[1].state.shape == (c.n_slots, 4)
+    slot = c.acquire()
+    c.reserve(slot, 70)
+    c.advance(slot, 70)
+    assert c.live_kv_bytes([slot]) == 70 * (2 * 3 * 2 * 36 + 48 * 2 + 2 * 2 * 20)
+    assert c.bytes() == 256 * (2 * 3 * 2 * 36 + 48 * 2 + 2 * 2 * 20) + c.n_slots * 4 * 4
+    c.release(slot)
+    c.check()
+    for need, bits in ((KVNeed(3, 64), 8), (KVNeed(3, 24), 4), (KVNeed(3, 64, v_dim=32), 4), (KVNeed(1, 512), 4)):
+        with pytest.raises(CacheError):
+            SequenceCache([need], max_tokens=64, max_seq_len=64, dtype=torch.bfloat16, device="cpu", kv_bits=bits)
+
+
+def test_models_say_whether_they_take_4_bits():
+    from vlrf_b200.cache import KVNeed
+    from vlrf_b200.engine.model import DecoderModel
+    from vlrf_b200.parts.mixer import CausalSelfAttention
+
+    class Mixer:
+        takes_packed_kv = True
+
+    class Layer:
+        def __init__(self, need, mixer):
+            self.need, self.mixer = need, mixer
+
+        def cache_need(self):
+            return self.need
+    model = object.__new__(DecoderModel)
+    model.layers = [Layer(KVNeed(1, 64), Mixer()), Layer(None, object())]
+    model.check_packed_kv()
+    for need in (KVNeed(1, 64), (None, KVNeed(1, 64))):
+        model.layers = [Layer(need, object())]
+        with pytest.raises(ValueError, match="4 bits"):
+            model.check_packed_kv()
+    assert CausalSelfAttention.takes_packed_kv

@@ -24,29 +24,30 @@ from .weights.model_dir import write_random_model
 
 
 class Model:
-    def __init__(self, decoder, *, max_tokens: int | None = None, n_slots: int | None = None):
+    def __init__(self, decoder, *, max_tokens: int | None = None, n_slots: int | None = None, kv_cache: str | None = None):
         self.decoder = decoder
         self.config = decoder.config
         if max_tokens is None:
             max_tokens = decoder.max_seq_len
-        self.engine = Engine(decoder, max_tokens=max_tokens, n_slots=n_slots)
+        self.engine = Engine(decoder, max_tokens=max_tokens, n_slots=n_slots, kv_cache=kv_cache)
         self.backend = DeviceBackend(self.engine)
 
     # -- construction -------------------------------------------------------------------------
     @classmethod
     def load(cls, model_dir, dtype="bfloat16", device="cuda:0", max_tokens: int | None = None,
-             n_slots: int | None = None) -> "Model":
-        """A folder with config.json and model.safetensors (vlrf_load_weights, vlrf.h:124)."""
-        return cls(load_model(model_dir, dtype, device), max_tokens=max_tokens, n_slots=n_slots)
+             n_slots: int | None = None, kv_cache: str | None = None) -> "Model":
+        """A folder with config.json and model.safetensors (vlrf_load_weights, vlrf.h:124).  kv_cache "int4": keys and values in 4 bits
+        (vlrf_set_kv_cache_type there), for models whose attention takes it (GPT-2)."""
+        return cls(load_model(model_dir, dtype, device), max_tokens=max_tokens, n_slots=n_slots, kv_cache=kv_cache)
 
     @classmethod
     def init_random(cls, config: dict, seed: int = 1234, dtype="bfloat16", device="cuda:0",
-                    max_tokens: int | None = None, n_slots: int | None = None) -> "Model":
+                    max_tokens: int | None = None, n_slots: int | None = None, kv_cache: str | None = None) -> "Model":
         """Random weights for a configuration (vlrf_init_random, vlrf.h:120): the folder is written to a
         temporary place and loaded like any other."""
         with tempfile.TemporaryDirectory(prefix="vlrf_b200_random_") as tmp:
             write_random_model(config, seed, tmp)
-            return cls.load(tmp, dtype, device, max_tokens, n_slots)
+            return cls.load(tmp, dtype, device, max_tokens, n_slots, kv_cache)
 
     # -- generation ---------------------------------------------------------------------------
     def generate_ids(self, prompts, params: SamplingParams | list | None = None, on_token=None) -> list:

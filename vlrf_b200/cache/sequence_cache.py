@@ -21,9 +21,14 @@ group owns [layer in group, slot, *shape], zeroed when a slot is taken.  `max_to
 key/value pool: it is the most tokens that live sequences hold at one time, each sequence's count
 rounded up to whole blocks.
 
+With `kv_bits=4` key/value groups hold 4 bits a number instead: codes, and a step and a zero for every few neighbouring entries of a head (see
+csrc.ops.PackedKV; 4.5 bits a number in all where 64 divides the head size).  Mixers then get `CacheView.packed` in place of k and v.
+Latent and state groups are as they were.
+
 The reference keeps one sequence: a [max_seq, kv_heads·head_dim] store per layer with one `used`
 counter (include/model/kv_cache.hpp:132-138, :215-251) that is re-laid out per head on every call
-(include/model/attention.hpp:154-156); here the per-head layout is the stored one.
+(include/model/attention.hpp:154-156); here the per-head layout is the stored one.  Its store in fewer bits (Q8_0, :102-121) is taken back to
+float32 rows ahead of every call; here attention reads the codes.
 """
 from __future__ import annotations
 
@@ -32,6 +37,7 @@ import dataclasses
 import numpy as np
 import torch
 
+from ..csrc.ops import PackedKV, packed_group
 from .allocator import CacheError, FreeList
 
 BLOCK_TOKENS = 64
@@ -68,17 +74,22 @@ class CacheView:
     v: torch.Tensor | None = None
     block_table: torch.Tensor | None = None  # device int32 [slot, block index]
     state: torch.Tensor | None = None        # [slot, *shape]
+    packed: object = None                    # a key/value group in 4 bits: csrc.ops.PackedKV in place of k and v
     rows: torch.Tensor | None = None         # a latent group's [block, block_tokens, width]
     parts: list | None = None                # for a tuple of needs: one view per need, in its order
 
 
 class _KVGroup:
-    def __init__(self, need: KVNeed, entries, n_blocks, n_slots, max_blocks, dtype, device):
+    def __init__(self, need: KVNeed, entries, n_blocks, n_slots, max_blocks, dtype, device, kv_bits=None):
         self.need, self.entries = need, list(entries)
         self.pool = FreeList(n_blocks, "cache block")
+        self.packed = None
         if isinstance(need, LatentNeed):
             self.k = self.v = None
             self.rows = torch.zeros((len(self.entries), n_blocks, BLOCK_TOKENS, need.width), dtype=dtype, device=device)
+        elif kv_bits == 4:
+            self.k = self.v = self.rows = None
+            self.packed = [PackedKV.zeros(n_blocks, need.n_kv_heads, BLOCK_TOKENS, need.head_dim, device) for _ in self.entries]
         else:
             shape = (len(self.entries), n_blocks, need.n_kv_heads, BLOCK_TOKENS, need.head_dim)
             self.k = torch.zeros(shape, dtype=dtype, device=device)
@@ -141,8 +152,11 @@ class _StateGroup:
 
 class SequenceCache:
     def __init__(self, needs, *, max_tokens: int, max_seq_len: int, dtype: torch.dtype, device,
-                 n_slots: int | None = None):
-        """needs: for every cache entry (one per layer execution that keeps something) its need, or None."""
+                 n_slots: int | None = None, kv_bits: int | None = None):
+        """needs: for every cache entry (one per layer execution that keeps something) its need, or None.  kv_bits: 4, or None for
+        keys and values in `dtype`."""
+        if kv_bits not in (None, 4):
+            raise CacheError(f"keys and values are held in the engine's dtype or in 4 bits, not in {kv_bits}")
         if max_tokens <= 0 or max_seq_len <= 0:
             raise CacheError("max_tokens and max_seq_len must be positive")
         self.block_tokens = BLOCK_TOKENS
@@ -154,6 +168,7 @@ class SequenceCache:
         self.max_blocks = (max_seq_len + BLOCK_TOKENS - 1) // BLOCK_TOKENS
         self.device = torch.device(device)
         self.dtype = dtype
+        self.kv_bits = kv_bits
         self.slots = FreeList(self.n_slots, "cache slot")
         self.lengths = [0] * self.n_slots
         self.needs = list(needs)
@@ -178,7 +193,10 @@ class SequenceCache:
                     raise CacheError("a window need has a positive window")
                 if getattr(need, "keep_first", 0) < 0 or (getattr(need, "keep_first", 0) and need.kind != "window"):
                     raise CacheError("keep_first belongs to a window need and is not negative")
-                g = _KVGroup(need, entries, self.n_blocks, self.n_slots, self.max_blocks, dtype, self.device)
+                if kv_bits is not None and isinstance(need, KVNeed) and (packed_group(need.head_dim) == 0 or need.v_dim not in (0, need.head_dim)):
+                    raise CacheError(f"keys and values of {need.head_dim} and {need.v_dim or need.head_dim} numbers cannot be held in {kv_bits} bits: "
+                                     "equal head sizes that are multiples of 16 up to 256 can")
+                g = _KVGroup(need, entries, self.n_blocks, self.n_slots, self.max_blocks, dtype, self.device, kv_bits)
             elif isinstance(need, StateNeed):
                 g = _StateGroup(need, entries, self.n_slots, self.device)
             else:
@@ -197,6 +215,8 @@ class SequenceCache:
         if isinstance(g, _KVGroup):
             if g.rows is not None:
                 return CacheView(g.need, rows=g.rows[i], block_table=g.table_dev)
+            if g.packed is not None:
+                return CacheView(g.need, packed=g.packed[i], block_table=g.table_dev)
             return CacheView(g.need, k=g.k[i], v=g.v[i], block_table=g.table_dev)
         return CacheView(g.need, state=g.state[i])
 
@@ -205,6 +225,8 @@ class SequenceCache:
         for g in self._groups:
             if isinstance(g, _KVGroup) and g.rows is not None:
                 total += g.rows.numel() * g.rows.element_size()
+            elif isinstance(g, _KVGroup) and g.packed is not None:
+                total += sum(p.bytes() for p in g.packed)
             elif isinstance(g, _KVGroup):
                 total += (g.k.numel() + g.v.numel()) * g.k.element_size()
             else:
@@ -218,6 +240,8 @@ class SequenceCache:
             if isinstance(g, _KVGroup):
                 if g.rows is not None:
                     per_tok = len(g.entries) * g.need.width * g.rows.element_size()
+                elif g.packed is not None:
+                    per_tok = sum(p.bytes() for p in g.packed) // (self.n_blocks * BLOCK_TOKENS)
                 else:
                     per_tok = len(g.entries) * g.need.n_kv_heads * (g.need.head_dim + (g.need.v_dim or g.need.head_dim)) * g.k.element_size()
                 for s in slots:

@@ -5,7 +5,7 @@ them (tools/vlrf_cli.cpp:93-121, usage :123-170):
                                  [--tokens N] [--ctx N] [--temp F] [--seed N] [--greedy]
                                  [--repeat-penalty F] [--freq-penalty F] [--presence-penalty F]
                                  [--no-repeat-ngram N] [--top-k N] [--top-p F] [--stop-id N ...]
-                                 [--dtype bfloat16|float32]
+                                 [--dtype bfloat16|float32] [--kv-cache model|int4]
     python -m vlrf_b200.cli info --model DIR
     python -m vlrf_b200.cli init --config PRESET|config.json --out DIR [--seed N]
 
@@ -14,8 +14,8 @@ Without a tokenizer, `--prompt "text"` is encoded like the reference does withou
 at the vocabulary (src/api/vlrf_api.cpp:373-381); token ids are printed, since there is nothing to decode
 them with.  `--stop` (stop strings) needs a tokenizer and is not offered; `--stop-id` stops at token ids.
 `--ctx N` sizes the cache in tokens (vlrf_set_ctx there).  `--temp` is applied here (the reference's CLI
-parses it and drops it).  `init` writes a random-weights model folder (disabled there).  `--backend` and
-`--kv-cache` do not exist: there is one backend and the cache has the engine's dtype.
+parses it and drops it).  `init` writes a random-weights model folder (disabled there).  `--kv-cache int4` holds keys and
+values in 4 bits (f16 and q8_0 there); `--backend` does not exist: there is one.
 """
 from __future__ import annotations
 
@@ -44,6 +44,7 @@ def _add_run_options(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--no-repeat-ngram", type=int, default=0)
     ap.add_argument("--stop-id", type=int, action="append", default=None)
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--kv-cache", default="model", choices=["model", "int4"], help="how keys and values are held: in the model's dtype, or in 4 bits")
 
 
 def _prompts(args) -> tuple[list, bool]:
@@ -67,7 +68,8 @@ def cmd_run(args) -> int:
     prompts, from_text = _prompts(args)
     need = sum((len(p) + args.tokens + 63) // 64 * 64 for p in prompts)
     print(f"Loading model from {args.model} ...")
-    model = Model.load(args.model, dtype=args.dtype, max_tokens=args.ctx if args.ctx > 0 else need)
+    model = Model.load(args.model, dtype=args.dtype, max_tokens=args.ctx if args.ctx > 0 else need,
+                       kv_cache=None if args.kv_cache == "model" else args.kv_cache)
     print(model.model_summary())
     if from_text:       # bytes beyond the vocabulary become its last id (src/api/vlrf_api.cpp:373-381)
         prompts = [[min(t, model.decoder.vocab_size - 1) for t in p] for p in prompts]

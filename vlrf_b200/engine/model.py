@@ -83,6 +83,16 @@ class DecoderModel:
                 out.append((i, type(mixer).__name__, mixer.kernels(self.act_dtype, block_tokens)))
         return out
 
+    def check_packed_kv(self) -> None:
+        """Raises ValueError unless every mixer that keeps keys and values reads and writes caches in 4 bits."""
+        from ..cache import KVNeed
+
+        def kv(need):
+            return isinstance(need, KVNeed) or (isinstance(need, tuple) and any(kv(part) for part in need))
+        for i, layer in enumerate(self.layers):
+            if kv(layer.cache_need()) and not getattr(getattr(layer, "mixer", None), "takes_packed_kv", False):
+                raise ValueError(f"layer {i}: {type(getattr(layer, 'mixer', layer)).__name__} does not take keys and values in 4 bits")
+
     def cache_needs(self) -> list:
         """For every schedule entry what it keeps per sequence (None for entries that read another's); behind them, where
         the embedding keeps something per sequence (say, the token before), one more entry with its need."""

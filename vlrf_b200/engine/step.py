@@ -24,6 +24,10 @@ DEVERR_TEXT = {1: "a token id outside the vocabulary", 2: "a position outside th
                4: "a token whose cache block is not mapped", 8: "a bounded wait that gave up"}
 
 
+#: how keys and values may be held -> bits a number (None: the model's dtype)
+KV_CACHES = {None: None, "int4": 4}
+
+
 @dataclasses.dataclass
 class StepEntry:
     slot: int
@@ -36,14 +40,22 @@ class StepError(ValueError):
 
 
 class Engine:
-    def __init__(self, model: DecoderModel, *, max_tokens: int, n_slots: int | None = None):
+    def __init__(self, model: DecoderModel, *, max_tokens: int, n_slots: int | None = None, kv_cache: str | None = None):
+        """kv_cache: None (keys and values in the model's dtype) or "int4" (see cache.SequenceCache's kv_bits)."""
+        if kv_cache not in KV_CACHES:
+            raise StepError(f"unknown kv_cache '{kv_cache}'; choose one of {', '.join(str(k) for k in KV_CACHES)}")
+        if kv_cache is not None:
+            try:
+                model.check_packed_kv()
+            except ValueError as why:
+                raise StepError(str(why)) from None
         if not torch.cuda.is_available():
             raise KernelError("no CUDA device: this framework runs on the GPU only")
         library()  # fail now, loudly, if the kernels cannot be built or loaded
         self.model = model
         self.device = model.device
         self.cache = SequenceCache(model.cache_needs(), max_tokens=max_tokens, max_seq_len=model.max_seq_len,
-                                   dtype=model.act_dtype, device=self.device, n_slots=n_slots)
+                                   dtype=model.act_dtype, device=self.device, n_slots=n_slots, kv_bits=KV_CACHES[kv_cache])
         self.ws = Workspace(self.device)
         self.dev_err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._meta_cap = 0
@@ -70,6 +82,27 @@ class Engine:
 
     def length(self, slot: int) -> int:
         return self.cache.lengths[slot]
+
+    def keys_values(self, slot: int, entry: int = 0, first: int = 0, last: int | None = None, dtype: torch.dtype | None = None) -> tuple:
+        """What cache entry `entry` (see DecoderModel.cache_needs) of a cache in 4 bits holds for the tokens first … last − 1 of a sequence, as two
+        matrices [tokens, kv_heads · head_dim] of `dtype` (the model's where it is not given): for handing a context over, or looking at it."""
+        from ..csrc import ops
+        if not self.cache.slots.is_held(slot):
+            raise StepError(f"slot {slot} is not held by a sequence")
+        view = self.cache.view(entry)
+        if view.packed is None:
+            raise StepError(f"cache entry {entry} does not hold keys and values in 4 bits")
+        last = self.cache.lengths[slot] if last is None else last
+        if not 0 <= first <= last <= self.cache.lengths[slot]:
+            raise StepError(f"slot {slot} holds {self.cache.lengths[slot]} tokens, not {first} to {last}")
+        if view.need.kind == "window" and first < self.cache.lengths[slot] - view.need.window:
+            raise StepError(f"slot {slot} keeps the last {view.need.window} tokens")
+        n, width = last - first, view.packed.n_kv_heads * view.packed.head_dim
+        out = [torch.empty((n, width), dtype=dtype or self.model.act_dtype, device=self.device) for _ in range(2)]
+        self.cache.sync_tables()
+        ops.kv_read_packed(view.packed, view.block_table, torch.full((n,), slot, dtype=torch.int32, device=self.device),
+                           torch.arange(first, last, dtype=torch.int32, device=self.device), out[0], out[1], n, self.dev_err)
+        return out[0], out[1]
 
     # -- the step -----------------------------------------------------------------------------
     def _meta(self, n_ints: int):

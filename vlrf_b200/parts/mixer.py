@@ -35,7 +35,14 @@ class CausalSelfAttention:
 
     n_kv_heads < n_heads shares each key/value head among n_heads/n_kv_heads query heads; window > 0
     limits a query to the last `window` keys.  GPT-2 uses neither.
+
+    Over a cache in 4 bits (`view.packed`) the products write no cache: keys and values are quantised in a kernel behind the
+    projection, and every query, a prompt's too, attends the numbers that the cache then stands for, so a prompt may be
+    brought in any pieces.
     """
+
+    #: this mixer reads and writes caches in 4 bits
+    takes_packed_kv = True
 
     def __init__(self, w_qkv, b_qkv, w_out, b_out, *, n_heads: int, n_kv_heads: int, head_dim: int,
                  scale: float, window: int = 0, position=None):
@@ -78,7 +85,7 @@ class CausalSelfAttention:
                 and ops.can_fuse_layernorm(T, x.shape[1], self.w_qkv.dtype, x, norm.weight, norm.bias, self.w_qkv):
             # few rows: norm, projection and the cache write in one kernel
             scatter = None
-            if writes_cache:
+            if writes_cache and view.packed is None:
                 scatter = (view.k, view.v, view.block_table, ctx.tok_slot, ctx.tok_pos, self.k_off, self.v_off,
                            self.n_kv_heads, self.head_dim)
                 appended = True
@@ -88,11 +95,14 @@ class CausalSelfAttention:
             if h is None:
                 h = norm(x, ctx.ws.get("block_normed", T, x.shape[1], ctx.act_dtype))
             scatter = None
-            if writes_cache:
+            if writes_cache and view.packed is None:
                 scatter = (view.k, view.v, view.block_table, ctx.tok_slot, ctx.tok_pos, self.k_off, self.v_off,
                            self.n_kv_heads, self.head_dim)
             appended = ops.linear(h, self.w_qkv, self.b_qkv, qkv, kv_scatter=scatter)   # the epilogue writes the cache if it can
-        if writes_cache and not appended:
+        if writes_cache and view.packed is not None:
+            ops.kv_append_packed(qkv, self.k_off, self.v_off, view.packed, view.block_table, ctx.tok_slot, ctx.tok_pos, T, self.n_kv_heads,
+                                 self.head_dim, ctx.dev_err)
+        elif writes_cache and not appended:
             ops.kv_append(qkv, self.k_off, self.v_off, view.k, view.v, view.block_table, ctx.tok_slot,
                           ctx.tok_pos, T, self.n_kv_heads, self.head_dim, ctx.dev_err)
         merged = ctx.ws.get("attn_out", T, self.n_heads * self.head_dim, ctx.act_dtype)
@@ -102,7 +112,9 @@ class CausalSelfAttention:
     def emit_decode(self, program, x: torch.Tensor, norm, view, writes_cache: bool = True) -> None:
         """The decode step of this mixer as operations of a decode program: norm + q/k/v projection (+ cache
         write), attention over the cache, output projection + residual."""
-        from .program import norm_terms
+        from .program import NotFusable, norm_terms
+        if view.packed is not None:
+            raise NotFusable("a cache in 4 bits is not read by the decode program's operations")
         rows = program.n_rows
         qkv = program.scratch("attn_qkv", rows, self.qkv_width, program.act_dtype)
         merged = program.scratch("attn_out", rows, self.n_heads * self.head_dim, program.act_dtype, seg=self.head_dim)
@@ -123,6 +135,10 @@ class CausalSelfAttention:
 
     def _attend(self, qkv, view, merged, ctx: StepContext) -> None:
         T = ctx.n_tokens
+        if view.packed is not None:
+            ops.attention_packed_step(qkv, self.q_off, view.packed, view.block_table, merged, ctx, self.n_heads, self.n_kv_heads, self.head_dim,
+                                      self.scale, self.window)
+            return
         if ctx.max_new == 1:
             # a decode step: few queries, long contexts → split every context across CTAs
             n_split = ops.decode_splits(T, self.n_heads, ctx.max_context)
