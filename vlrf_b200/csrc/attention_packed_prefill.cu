@@ -3,7 +3,7 @@
 //
 // A CTA takes GROUPS · 128 consecutive new tokens of one sequence and one head and walks the keys they see in blocks of BK (128 keys of
 // 64 numbers, 64 of 128) up to the diagonal.  Its warps have fixed jobs:
-//   producers      codes and pairs of a block from the cache into registers, a tile ahead; from there zero + step · code as bfloat16 (one rounding)
+//   producers      codes and pairs of a block from the cache into registers, a block ahead; from there zero + step · code as bfloat16 (one rounding)
 //                  into a ring of four shared-memory slots, K and V in turn, in the 128-byte swizzle that the MMA reads.  A code becomes
 //                  a bfloat16 by a mask under the exponent of 128, less 128 (exact), two at a time; pairs of entries i and i + 4 of eight
 //                  stay neighbours, so the numbers of a row lie permuted, those of the queries likewise (the sum does not care), and the
@@ -175,53 +175,71 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         constexpr int PR = BK / NPROD, UNITS = PR * (DH / 32) / 32; // a unit: 32 entries of a row (16 bytes of codes); so many a lane
         const int p = warp - SOFT;
         const int n_exist = pos0 + n_new;                           // tokens that the cache holds
-        uint4 codes[UNITS];
-        uint32_t pairs[UNITS];
-        // tile t of this CTA: block my_first + t / 2, K or V
-        auto fetch = [&](int t) {
-            const int k0 = (my_first + (t >> 1)) * BK;
-            const unsigned char* src = (t & 1) ? Vq : Kq;
-            const uint32_t* psrc = (t & 1) ? Vp : Kp;
-            const int cb = (k0 + p * PR) / PP_CB;                   // (a warp's rows lie in one cache block)
-            const bool wanted = k0 + p * PR < n_exist && (cb + 1) * PP_CB > first_key;
-            const int blk = wanted ? packed_block(table, max_blocks, n_blocks, cb) : -1;
-            if (wanted && blk < 0 && lane == 0) atomicOr(dev_err, VLRF_DEVERR_NO_BLOCK);
-            const size_t at = ((size_t)max(blk, 0) * Hkv + hk) * PP_CB + (k0 + p * PR) % PP_CB;
+        struct Piece { uint4 codes[UNITS]; uint32_t pairs[UNITS]; } piece[2];    // of the next K tile and the next V tile
+        int held = -1;                                              // the cache blocks of 32 blocks at a time lie a lane each
+        auto block_of = [&](int b) {
+            if ((b & 31) == 0) {
+                const int k0 = (my_first + b + lane) * BK + p * PR, cb = k0 / PP_CB;         // (a warp's rows lie in one cache block)
+                const bool wanted = b + lane < my_n && k0 < n_exist && (cb + 1) * PP_CB > first_key;
+                held = wanted ? packed_block(table, max_blocks, n_blocks, cb) : -1;
+                if (wanted && held < 0) atomicOr(dev_err, VLRF_DEVERR_NO_BLOCK);
+            }
+            return __shfl_sync(0xffffffffu, held, b & 31);
+        };
+        auto fetch = [&](int b, int blk, auto value_c, Piece& into) {
+            constexpr bool VALUE = decltype(value_c)::value;
+            const int k0 = (my_first + b) * BK + p * PR;
+            const size_t at = ((size_t)max(blk, 0) * Hkv + hk) * PP_CB + k0 % PP_CB;
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) {
                 const int u = i * 32 + lane, r = u / (DH / 32), c = u % (DH / 32);
-                codes[i] = make_uint4(0u, 0u, 0u, 0u);
-                pairs[i] = 0u;
-                if (blk >= 0 && k0 + p * PR + r < n_exist) {
-                    codes[i] = *reinterpret_cast<const uint4*>(src + (at + r) * (DH / 2) + c * 16);
-                    pairs[i] = psrc[(at + r) * NG + c / 2];
+                into.codes[i] = make_uint4(0u, 0u, 0u, 0u);
+                into.pairs[i] = 0u;
+                if (blk >= 0 && k0 + r < n_exist) {
+                    into.codes[i] = *reinterpret_cast<const uint4*>((VALUE ? Vq : Kq) + (at + r) * (DH / 2) + c * 16);
+                    const uint32_t value_pair = Vp[(at + r) * NG + c / 2];
+                    into.pairs[i] = VALUE ? value_pair : Kp[(at + r) * NG + c / 2];
                     // (NaN in a value's pair, both halves of it: zeros in V, NaN in K)
-                    const uint32_t other = (t & 1) ? pairs[i] : Vp[(at + r) * NG + c / 2];
-                    if ((other & 0x7fffu) > 0x7f80u) pairs[i] = (t & 1) ? 0u : 0x7fff7fffu;
+                    if ((value_pair & 0x7fffu) > 0x7f80u) into.pairs[i] = VALUE ? 0u : 0x7fff7fffu;
                 }
             }
         };
-        bool ok = true;
-        if (my_n > 0) fetch(0);
-        for (int t = 0; t < 2 * my_n; ++t) {
+        auto put = [&](int t, const Piece& from) -> bool {          // tile t of this CTA: block t / 2, K or V
             const int sl = t % PP_SLOTS, use = t / PP_SLOTS;
-            if (use >= 1 && !tbar_wait_warp(&empty[sl], (uint32_t)((use - 1) & 1), s_abort)) { ok = false; break; }
+            if (use >= 1 && !tbar_wait_warp(&empty[sl], (uint32_t)((use - 1) & 1), s_abort)) return false;
             unsigned char* tile = kv_tiles + (size_t)sl * PP_TILE;
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) {
                 const int u = i * 32 + lane, r = p * PR + u / (DH / 32), c = u % (DH / 32);
-                const uint32_t s2 = __byte_perm(pairs[i], 0, 0x1010), z2 = __byte_perm(pairs[i], 0, 0x3232);
+                const uint32_t s2 = __byte_perm(from.pairs[i], 0, 0x1010), z2 = __byte_perm(from.pairs[i], 0, 0x3232);
                 const __nv_bfloat162 step = *reinterpret_cast<const __nv_bfloat162*>(&s2), zero = *reinterpret_cast<const __nv_bfloat162*>(&z2);
                 unsigned char* dst = tile + (c >> 1) * ATOM_KV + r * 128;
-                const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+                const uint32_t w[4] = {from.codes[i].x, from.codes[i].y, from.codes[i].z, from.codes[i].w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     *reinterpret_cast<uint4*>(dst + ((((c & 1) * 4 + j) ^ (r & 7)) << 4)) = pp_numbers(w[j], step, zero);
             }
-            if (t + 1 < 2 * my_n) fetch(t + 1);
+            return true;
+        };
+        auto hand_over = [&](int t) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the MMA reads them
             __syncwarp();
-            if (lane == 0) tbar_arrive(&full[sl]);
+            if (lane == 0) tbar_arrive(&full[t % PP_SLOTS]);
+        };
+        bool ok = true;
+        if (my_n > 0) {
+            const int blk = block_of(0);
+            fetch(0, blk, std::false_type{}, piece[0]);
+            fetch(0, blk, std::true_type{}, piece[1]);
+        }
+        for (int b = 0; b < my_n; ++b) {
+            const int next = b + 1 < my_n ? block_of(b + 1) : -1;
+            if (!(ok = put(2 * b, piece[0]))) break;
+            if (b + 1 < my_n) fetch(b + 1, next, std::false_type{}, piece[0]);
+            hand_over(2 * b);
+            if (!(ok = put(2 * b + 1, piece[1]))) break;
+            if (b + 1 < my_n) fetch(b + 1, next, std::true_type{}, piece[1]);
+            hand_over(2 * b + 1);
         }
         if (!ok) atomicExch(s_abort, 1);
     } else if (warp == SOFT + NPROD) {
@@ -468,7 +486,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                     const float m_p = __ldcg(theirs + DH * 128 + r), l_p = __ldcg(theirs + DH * 128 + 128 + r);
                     const float m_new = fmaxf(m_run, m_p), use = m_new == -INFINITY ? 0.f : m_new;
                     const float a = (m_run == -INFINITY) ? 0.f : pp_exp2(m_run - use);
-                    const float b = (m_p == -INFINITY) ? (l_p != l_p ? 1.f : 0.f) : pp_exp2(m_p - use);  // (a part whose scores are all NaN keeps its NaN)
+                    const float b = (m_p == -INFINITY) ? 0.f : pp_exp2(m_p - use);       // (sums that are not numbers stay so)
                     l_run = fmaf(l_run, a, l_p * b);
                     m_run = m_new;
 #pragma unroll

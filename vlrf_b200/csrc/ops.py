@@ -1063,14 +1063,12 @@ def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_
                             dev_err)
     if qkv.dtype != torch.bfloat16 or seq_slot.shape[0] < n_seqs or seq_start.shape[0] < n_seqs + 1 or seq_pos0.shape[0] < n_seqs:
         raise KernelError(f"{what}: bfloat16 rows, and a slot, a first row and a first position for every sequence")
+    scratch = (0, 0)
     if n_parts > 1:
-        _dev(partials, f"{what}: partials", torch.float32); _dev(counters, f"{what}: counters", torch.int32)
-        want = packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts)
-        if partials.numel() < want[0] or counters.numel() < want[1]:
-            raise KernelError(f"{what}: scratch is too small for {n_parts} parts")
+        scratch = _packed_scratch(what, packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts), partials, counters)
     call("vlrf_attn_packed_prefill", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], seq_slot.data_ptr(),
          seq_start.data_ptr(), seq_pos0.data_ptr(), out.data_ptr(), out.stride(0), n_seqs, max_new, n_heads, n_kv_heads, head_dim, cache.block_tokens,
-         float(scale), window, groups, n_parts, _ptr(partials) if n_parts > 1 else 0, _ptr(counters) if n_parts > 1 else 0, dev_err.data_ptr(), _stream())
+         float(scale), window, groups, n_parts, *scratch, dev_err.data_ptr(), _stream())
 
 
 def packed_prefill_scratch(n_seqs: int, max_new: int, n_heads: int, head_dim: int, groups: int, n_parts: int) -> tuple:
@@ -1089,22 +1087,43 @@ def packed_decode_splits(n_rows: int, n_heads: int, n_kv_heads: int, max_context
     if forced:
         return max(1, min(16, int(forced)))
     reach = min(max_context, window + 63) if window > 0 else max_context
-    share = n_heads // n_kv_heads
-    ctas = max(1, n_rows * n_kv_heads * (-(-share // 16)))
-    return max(1, min(16, (2 * sm_count()) // ctas, -(-reach // 256)))
+    pairs = max(1, n_rows * n_kv_heads * (-(-(n_heads // n_kv_heads) // 8)))
+    return max(1, min(64, sm_count() // pairs, -(-reach // 768)))
+
+
+def packed_decode_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, n_split: int) -> tuple:
+    """(float32 elements of `partials`, int32 elements of `counters`) that `attention_decode_packed` wants for n_split > 1."""
+    import ctypes
+
+    from . import call_host
+    floats, ints = ctypes.c_longlong(0), ctypes.c_longlong(0)
+    call_host("vlrf_attn_packed_decode_scratch", n_rows, n_heads, n_kv_heads, head_dim, n_split, ctypes.byref(floats), ctypes.byref(ints))
+    return floats.value, ints.value
+
+
+def _packed_scratch(what: str, want: tuple, partials, counters) -> tuple:
+    """Pointers to scratch of at least the wanted sizes."""
+    _dev(partials, f"{what}: partials", torch.float32); _dev(counters, f"{what}: counters", torch.int32)
+    if partials.numel() < want[0] or counters.numel() < want[1]:
+        raise KernelError(f"{what}: scratch is too small")
+    return partials.data_ptr(), counters.data_ptr()
 
 
 def attention_decode_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, out, n_rows: int, n_heads: int, n_kv_heads: int,
-                            head_dim: int, scale: float, window: int, n_split: int, dev_err) -> None:
+                            head_dim: int, scale: float, window: int, n_split: int, dev_err, partials=None, counters=None) -> None:
     """One bfloat16 query per row and head attends the keys 0…position of its slot in a cache of 4 bits, on the tensor cores; the context is
-    cut into n_split parts.  Rows with slot −1 are left as they are."""
+    cut into n_split parts, which for more than one meet in float32 `partials` and zeroed int32 `counters` (see packed_decode_scratch; the
+    counters are left zero).  Rows with slot −1 are left as they are."""
     what = "attention_decode_packed"
     _attention_packed_check(what, qkv, q_off, cache, block_table, (tok_slot, tok_pos), out, n_rows, n_heads, n_kv_heads, head_dim, window, dev_err)
     if qkv.dtype != torch.bfloat16 or tok_slot.shape[0] < n_rows or tok_pos.shape[0] < n_rows:
         raise KernelError(f"{what}: bfloat16 rows, each with a slot and a position")
+    scratch = (0, 0)
+    if n_split > 1:
+        scratch = _packed_scratch(what, packed_decode_scratch(n_rows, n_heads, n_kv_heads, head_dim, n_split), partials, counters)
     call("vlrf_attn_packed_decode", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], tok_slot.data_ptr(),
          tok_pos.data_ptr(), out.data_ptr(), out.stride(0), n_rows, n_heads, n_kv_heads, head_dim, cache.block_tokens, float(scale), window, n_split,
-         dev_err.data_ptr(), _stream())
+         *scratch, dev_err.data_ptr(), _stream())
 
 
 def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ctx, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -1112,8 +1131,14 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
     """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
     already holds the step's own keys and values."""
     if ctx.max_new == 1 and _packed_decode_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
+        n_split = packed_decode_splits(ctx.n_tokens, n_heads, n_kv_heads, ctx.max_context, window)
+        partials = counters = None
+        if n_split > 1:
+            n_floats, n_counters = packed_decode_scratch(ctx.n_tokens, n_heads, n_kv_heads, head_dim, n_split)
+            partials = ctx.ws.get("packed_partials", n_floats, 1, torch.float32)
+            counters = ctx.ws.get_zeroed("packed_counters", n_counters, torch.int32)
         attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
-                                window, packed_decode_splits(ctx.n_tokens, n_heads, n_kv_heads, ctx.max_context, window), ctx.dev_err)
+                                window, n_split, ctx.dev_err, partials, counters)
         return
     if ctx.max_new > 1 and _packed_prefill_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
         groups, n_parts = packed_prefill_shape(ctx.n_tokens, ctx.n_seqs, ctx.max_new, ctx.max_context, n_heads, head_dim, window)
