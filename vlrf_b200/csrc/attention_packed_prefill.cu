@@ -28,6 +28,7 @@
 namespace {
 constexpr int PP_CB = 64, PP_SLOTS = 4, PP_TILE = 16384;            // tokens of a cache block; slots of the ring, bytes of each
 constexpr int PP_PART_BLOCKS = 3, PP_MAX_PARTS = 16;
+constexpr float PP_LAZY = 6.f;
 constexpr __host__ __device__ int pp_bk(int DH) { return DH == 64 ? 128 : 64; }
 constexpr __host__ __device__ int pp_producers(int GROUPS) { return 2 * GROUPS; }
 constexpr __host__ __device__ int pp_threads(int GROUPS) { return (GROUPS * 8 + pp_producers(GROUPS) + 1) * 32; }
@@ -99,6 +100,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                            int* __restrict__ counters, int n_tiles, int* __restrict__ dev_err) {
     constexpr int BK = pp_bk(DH), ROWS = GROUPS * 128, NG = DH / 64, NPROD = pp_producers(GROUPS), SOFT = GROUPS * 8;
     constexpr int Q_BYTES = 128 * DH * 2, ATOM_Q = 16384, ATOM_KV = BK * 128;    // a 64-number chunk of 128 queries / of a block
+    constexpr int NP = BK + DH + BK <= 256 ? 2 : 1;                 // buffers of P that a group's 256 columns have room for
     constexpr int HK = BK / 2, NC = HK / 32, HD = DH / 2;           // keys, chunks of 32 keys, and columns of O of a softmax thread
     extern __shared__ unsigned char pp_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pp_raw) + 1023) & ~(uintptr_t)1023);
@@ -110,9 +112,9 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     uint64_t* empty = full + PP_SLOTS;
     uint64_t* s_full = empty + PP_SLOTS;                            // [GROUPS] each from here
     uint64_t* s_read = s_full + GROUPS;
-    uint64_t* p_full = s_read + GROUPS;
-    uint64_t* o_full = p_full + GROUPS;
-    uint64_t* drained = o_full + GROUPS;
+    uint64_t* p_full = s_read + GROUPS;                             // [GROUPS][NP], product i at i % NP: either side may be NP − 1 blocks ahead
+    uint64_t* o_full = p_full + GROUPS * NP;
+    uint64_t* drained = o_full + GROUPS * NP;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
     int* s_never = s_abort + 1;                                     // stays 0: for waits that nothing calls off
@@ -127,19 +129,13 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             tbar_init(&q_full[g], 8);
             tbar_init(&s_full[g], 1);
             tbar_init(&s_read[g], 8);
-            tbar_init(&p_full[g], 8);
-            tbar_init(&o_full[g], 1);
+            for (int i = 0; i < NP; ++i) { tbar_init(&p_full[g * NP + i], 8); tbar_init(&o_full[g * NP + i], 1); }
             s_last[g] = 1;
         }
         tbar_init(drained, 1);
         *s_abort = 0;
         *s_never = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    constexpr uint32_t TMEM_COLS = 256 * GROUPS;                    // a group: S BK columns, O DH, P BK / 2 (two bfloat16 a column)
-    if (warp == SOFT) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tsm(tmem_slot)), "r"(TMEM_COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_wait();
     pdl_launch_dependents();
@@ -152,8 +148,14 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     // the tile's key blocks are dealt to tile_parts CTAs; the others of its n_parts have nothing to do
     const int tile_parts = max(1, min(n_parts, (n_kb + PP_PART_BLOCKS - 1) / PP_PART_BLOCKS));
     const bool active = n_rows > 0 && slot >= 0 && pos0 >= 0 && part < tile_parts;      // uniform over the CTA
+    if (!active) return;                                            // (before it holds anything)
+    constexpr uint32_t TMEM_COLS = 256 * GROUPS;                    // a group: S BK columns, O DH, P NP times BK / 2 (two bfloat16 a column)
+    if (warp == SOFT) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tsm(tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     const int my_first = kb_first + part * n_kb / tile_parts;
-    const int my_n = active ? kb_first + (part + 1) * n_kb / tile_parts - my_first : 0, my_end = my_first + my_n;
+    const int my_n = kb_first + (part + 1) * n_kb / tile_parts - my_first, my_end = my_first + my_n;
     // the blocks of group g: lo … hi − 1 (a group without rows: none)
     int lo[GROUPS], hi[GROUPS];
 #pragma unroll
@@ -279,14 +281,14 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                 for (int g = 0; g < GROUPS; ++g) {
                     if (!ok || j < lo[g] || j >= hi[g]) continue;
                     const int i = j - lo[g];
-                    if (!tbar_wait_warp(&p_full[g], (uint32_t)(i & 1), s_abort)) { ok = false; continue; }
+                    if (!tbar_wait_warp(&p_full[g * NP + i % NP], (uint32_t)((i / NP) & 1), s_abort)) { ok = false; continue; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < BK / 16; ++k)           // 16 keys a step: 8 columns of P, 16 rows of V
-                            pp_mma_ta(tmem + g * 256 + BK, tmem + g * 256 + BK + DH + 8u * k, dv0 + (uint64_t)((sl * PP_TILE + k * 16 * 128) >> 4), idesc_o,
+                            pp_mma_ta(tmem + g * 256 + BK, tmem + g * 256 + BK + DH + (uint32_t)((i % NP) * (BK / 2)) + 8u * k, dv0 + (uint64_t)((sl * PP_TILE + k * 16 * 128) >> 4), idesc_o,
                                       (i > 0 || k > 0) ? 1u : 0u);
-                        umma_commit(&o_full[g]);
+                        umma_commit(&o_full[g * NP + i % NP]);
                     }
                     __syncwarp();
                 }
@@ -295,7 +297,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             }
             if (!ok) atomicExch(s_abort, 1);
         }
-    } else if (active) {
+    } else {
         // ---- softmax warps: a lane of tensor memory is a query row; warps q and q + 4 of a group have a half of a block's keys each
         const int g = warp >> 3, q = warp & 3, half = (warp >> 2) & 1, r = q * 32 + lane;
         const int my_lo = GROUPS == 1 || g == 0 ? lo[0] : lo[GROUPS - 1], my_hi = GROUPS == 1 || g == 0 ? hi[0] : hi[GROUPS - 1], n_i = my_hi - my_lo;
@@ -320,8 +322,9 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             __syncwarp();
             if (lane == 0) tbar_arrive(&q_full[g]);
         }
-        float m_run = -INFINITY, l_run = 0.f;                       // the row's maximum; the sum of this half
+        float m_run = -INFINITY, l_run = 0.f;                       // the row's reference point; the sum of this half
         bool ok = true;
+        auto wait_o = [&](int j) { return tbar_wait_warp(&o_full[g * NP + j % NP], (uint32_t)((j / NP) & 1), s_abort); };       // until O holds block j
         auto block = [&](int i, auto masked_c) {
             constexpr bool MASKED = decltype(masked_c)::value;
             const int k0 = (my_lo + i) * BK + half * HK;            // the half's first key
@@ -362,13 +365,19 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             sp[((i & 1) * 2 + half) * 128 + r] = m_half;
             asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
-            const float m_new = fmaxf(m_run, fmaxf(m_half, sp[((i & 1) * 2 + (half ^ 1)) * 128 + r]) * sl2);
+            // The weights' reference point m_run follows the row's maximum only where that has grown by 2^PP_LAZY: weights up to that are as exact in
+            // bfloat16 and float32 as weights up to 1, and O need not be scaled (for random rows in one block of twenty instead of all).
+            const float m_blk = fmaxf(m_half, sp[((i & 1) * 2 + (half ^ 1)) * 128 + r]) * sl2;
+            const float m_new = m_blk > m_run + PP_LAZY ? m_blk : m_run;
             const float corr = m_run == -INFINITY ? 1.f : pp_exp2(m_run - m_new);        // (from −inf on the row's sums are 0 so far)
             l_run *= corr;
             m_run = m_new;
             const float m_use = (m_run == -INFINITY) ? 0.f : m_run; // a row that sees nothing yet: every p is 0
-            if (i > 0) {                                            // O holds the blocks before, and P may be written again
-                if (!tbar_wait_warp(&o_full[g], (uint32_t)((i - 1) & 1), s_abort)) { ok = false; return; }
+            const bool grew = i > 0 && __any_sync(0xffffffffu, corr != 1.f);
+            // the P that goes where this one does has been multiplied; where O is to be scaled, all blocks before are in it
+            const int before = grew ? i - 1 : i - NP;
+            if (before >= 0) {
+                if (!wait_o(before)) { ok = false; return; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
             float sm4[4] = {0.f, 0.f, 0.f, 0.f};
@@ -386,7 +395,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                     sm4[(e + 1) & 3] += p1;
                     pk[e >> 1] = pack2(p0, p1);
                 }
-                pp_st16(tmem_p + (uint32_t)(half * (HK / 2) + c * 16), pk);
+                pp_st16(tmem_p + (uint32_t)((i % NP) * (BK / 2) + half * (HK / 2) + c * 16), pk);
             };
             if (!MASKED) {
 #pragma unroll
@@ -402,7 +411,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                         uint32_t none[16];
 #pragma unroll
                         for (int x = 0; x < 16; ++x) none[x] = 0u;
-                        pp_st16(tmem_p + (uint32_t)(half * (HK / 2) + c * 16), none);
+                        pp_st16(tmem_p + (uint32_t)((i % NP) * (BK / 2) + half * (HK / 2) + c * 16), none);
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -410,7 +419,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                 if (lane == 0) tbar_arrive(&s_read[g]);
             }
             l_run += (sm4[0] + sm4[1]) + (sm4[2] + sm4[3]);
-            if (i > 0 && __any_sync(0xffffffffu, corr != 1.f)) {    // a row's maximum grew: its O (a half of the columns here) follows
+            if (grew) {                                             // a row's reference point moved: its O (a half of the columns here) follows
 #pragma unroll
                 for (int d0 = 0; d0 < HD; d0 += 32) {
                     uint32_t ov[32];
@@ -424,7 +433,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tbar_arrive(&p_full[g]);
+            if (lane == 0) tbar_arrive(&p_full[g * NP + i % NP]);
         };
         for (int i = 0; i < n_i; ++i) {
             if (window > 0 || (my_lo + i) * BK + BK - 1 > group_first) block(i, std::true_type{});       // (uniform over the group)
@@ -435,7 +444,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
 #pragma unroll
         for (int d = 0; d < HD; ++d) o_acc[d] = 0.f;
         if (n_i > 0) {
-            if (ok && tbar_wait_warp(&o_full[g], (uint32_t)((n_i - 1) & 1), s_abort)) {
+            if (ok && wait_o(n_i - 1)) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                 for (int d0 = 0; d0 < HD; d0 += 32) {
