@@ -9,7 +9,7 @@
 //                  stay neighbours, so the numbers of a row lie permuted, those of the queries likewise (the sum does not care), and the
 //                  result is put in order where it is written.  Rows that no query may see, behind the sequence's last token or in
 //                  blocks wholly before the window, are zeros and are not read;
-//   the MMA warp   S = Q·Kᵀ into tensor memory and, once the probabilities are there, O += P·V (P is the operand in tensor memory, V
+//   MMA warps      (one a group) S = Q·Kᵀ into tensor memory and, once the probabilities are there, O += P·V (P is the operand in tensor memory, V
 //                  is read as it lies, head dimension contiguous);
 //   softmax warps  eight a group of 128 queries: a query is one lane of tensor memory, and two threads have a half of a block's keys each;
 //                  running maximum and sum in float32, O scaled where a maximum grew.
@@ -31,7 +31,7 @@ constexpr int PP_PART_BLOCKS = 3, PP_MAX_PARTS = 16;
 constexpr float PP_LAZY = 6.f;
 constexpr __host__ __device__ int pp_bk(int DH) { return DH == 64 ? 128 : 64; }
 constexpr __host__ __device__ int pp_producers(int GROUPS) { return 2 * GROUPS; }
-constexpr __host__ __device__ int pp_threads(int GROUPS) { return (GROUPS * 8 + pp_producers(GROUPS) + 1) * 32; }
+constexpr __host__ __device__ int pp_threads(int GROUPS) { return (GROUPS * 8 + pp_producers(GROUPS) + GROUPS) * 32; }
 constexpr __host__ __device__ int pp_part_floats(int DH) { return DH * 128 + 256; }
 
 __device__ __forceinline__ float pp_exp2(float x) {
@@ -106,8 +106,8 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pp_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* q_tiles = smem;                                  // [GROUPS][NG][128][128 B]
     unsigned char* kv_tiles = smem + GROUPS * Q_BYTES;              // [PP_SLOTS][NG][BK][128 B]: K_0, V_0, K_1, V_1, …
-    float* s_part = reinterpret_cast<float*>(kv_tiles + PP_SLOTS * PP_TILE);     // [GROUPS][2][2][128]
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(s_part + GROUPS * 512);       // [GROUPS]
+    float* s_part = reinterpret_cast<float*>(kv_tiles + PP_SLOTS * PP_TILE);     // [GROUPS][2][128]
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(s_part + GROUPS * 256);       // [GROUPS]
     uint64_t* full = q_full + GROUPS;
     uint64_t* empty = full + PP_SLOTS;
     uint64_t* s_full = empty + PP_SLOTS;                            // [GROUPS] each from here
@@ -124,7 +124,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     // z is the slowest index of the order in which CTAs are started: first parts first, and within a part long tiles first
     const int part = blockIdx.z / n_tiles, qt = n_tiles - 1 - blockIdx.z % n_tiles, seq = blockIdx.y, h = blockIdx.x;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < PP_SLOTS; ++i) { tbar_init(&full[i], NPROD); tbar_init(&empty[i], 1); }
+        for (int i = 0; i < PP_SLOTS; ++i) { tbar_init(&full[i], NPROD); tbar_init(&empty[i], GROUPS); }
         for (int g = 0; g < GROUPS; ++g) {
             tbar_init(&q_full[g], 8);
             tbar_init(&s_full[g], 1);
@@ -132,7 +132,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             for (int i = 0; i < NP; ++i) { tbar_init(&p_full[g * NP + i], 8); tbar_init(&o_full[g * NP + i], 1); }
             s_last[g] = 1;
         }
-        tbar_init(drained, 1);
+        tbar_init(drained, GROUPS);
         *s_abort = 0;
         *s_never = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -177,7 +177,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         constexpr int PR = BK / NPROD, UNITS = PR * (DH / 32) / 32; // a unit: 32 entries of a row (16 bytes of codes); so many a lane
         const int p = warp - SOFT;
         const int n_exist = pos0 + n_new;                           // tokens that the cache holds
-        struct Piece { uint4 codes[UNITS]; uint32_t pairs[UNITS]; } piece[2];    // of the next K tile and the next V tile
+        struct Piece { uint4 codes[UNITS]; uint32_t pairs[UNITS], value_pairs[UNITS]; } piece[2];   // of the next K tile and the next V tile
         int held = -1;                                              // the cache blocks of 32 blocks at a time lie a lane each
         auto block_of = [&](int b) {
             if ((b & 31) == 0) {
@@ -196,13 +196,11 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             for (int i = 0; i < UNITS; ++i) {
                 const int u = i * 32 + lane, r = u / (DH / 32), c = u % (DH / 32);
                 into.codes[i] = make_uint4(0u, 0u, 0u, 0u);
-                into.pairs[i] = 0u;
+                into.pairs[i] = into.value_pairs[i] = 0u;
                 if (blk >= 0 && k0 + r < n_exist) {
                     into.codes[i] = *reinterpret_cast<const uint4*>((VALUE ? Vq : Kq) + (at + r) * (DH / 2) + c * 16);
-                    const uint32_t value_pair = Vp[(at + r) * NG + c / 2];
-                    into.pairs[i] = VALUE ? value_pair : Kp[(at + r) * NG + c / 2];
-                    // (NaN in a value's pair, both halves of it: zeros in V, NaN in K)
-                    if ((value_pair & 0x7fffu) > 0x7f80u) into.pairs[i] = VALUE ? 0u : 0x7fff7fffu;
+                    into.value_pairs[i] = Vp[(at + r) * NG + c / 2];
+                    if (!VALUE) into.pairs[i] = Kp[(at + r) * NG + c / 2];
                 }
             }
         };
@@ -213,7 +211,10 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) {
                 const int u = i * 32 + lane, r = p * PR + u / (DH / 32), c = u % (DH / 32);
-                const uint32_t s2 = __byte_perm(from.pairs[i], 0, 0x1010), z2 = __byte_perm(from.pairs[i], 0, 0x3232);
+                // (NaN in a value's pair, both halves of it: zeros in V, NaN in K)
+                uint32_t pair = (t & 1) ? from.value_pairs[i] : from.pairs[i];
+                if ((from.value_pairs[i] & 0x7fffu) > 0x7f80u) pair = (t & 1) ? 0u : 0x7fff7fffu;
+                const uint32_t s2 = __byte_perm(pair, 0, 0x1010), z2 = __byte_perm(pair, 0, 0x3232);
                 const __nv_bfloat162 step = *reinterpret_cast<const __nv_bfloat162*>(&s2), zero = *reinterpret_cast<const __nv_bfloat162*>(&z2);
                 unsigned char* dst = tile + (c >> 1) * ATOM_KV + r * 128;
                 const uint32_t w[4] = {from.codes[i].x, from.codes[i].y, from.codes[i].z, from.codes[i].w};
@@ -244,59 +245,62 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             hand_over(2 * b + 1);
         }
         if (!ok) atomicExch(s_abort, 1);
-    } else if (warp == SOFT + NPROD) {
-        // ---- MMAs
-        if (my_n > 0) {
-            constexpr uint32_t idesc_s = umma_idesc_bf16(128, BK), idesc_o = pp_idesc_mn(128, DH);
-            const uint64_t dq0 = umma_desc_k128(q_tiles), dk0 = umma_desc_k128(kv_tiles), dv0 = pp_desc_mn(kv_tiles, ATOM_KV);
-            bool ok = true;
-            auto issue_s = [&](int j) -> bool {                     // S_j = Q · K_jᵀ of every group that sees block j
-                const uint32_t t = 2u * (j - my_first), sl = t % PP_SLOTS;
-                if (!tbar_wait_warp(&full[sl], (t / PP_SLOTS) & 1u, s_abort)) return false;
+    } else if (warp >= SOFT + NPROD) {
+        // ---- MMAs, a warp a group
+        const int g = warp - SOFT - NPROD, my_lo = g == 0 ? lo[0] : lo[GROUPS - 1], my_hi = g == 0 ? hi[0] : hi[GROUPS - 1];
+        constexpr uint32_t idesc_s = umma_idesc_bf16(128, BK), idesc_o = pp_idesc_mn(128, DH);
+        const uint64_t dq = umma_desc_k128(q_tiles + g * Q_BYTES), dk0 = umma_desc_k128(kv_tiles), dv0 = pp_desc_mn(kv_tiles, ATOM_KV);
+        const uint32_t tmem_s = tmem + g * 256, tmem_o = tmem_s + BK, tmem_p = tmem_o + DH;
+        bool ok = true;
+        // S_j = Q · K_jᵀ where the group sees block j; either way the group is done with K_j then
+        auto issue_s = [&](int j) -> bool {
+            const uint32_t t = 2u * (j - my_first), sl = t % PP_SLOTS;
+            const bool mine = j >= my_lo && j < my_hi;
+            const int i = j - my_lo;
+            if (mine && !tbar_wait_warp(i == 0 ? &q_full[g] : &s_read[g], i == 0 ? 0u : (uint32_t)((i - 1) & 1), s_abort)) return false;
+            if (!tbar_wait_warp(&full[sl], (t / PP_SLOTS) & 1u, s_abort)) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
+                if (mine) {
+                    const uint64_t dk = dk0 + (uint64_t)((sl * PP_TILE) >> 4);
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    if (j < lo[g] || j >= hi[g]) continue;
-                    const int i = j - lo[g];
-                    if (!tbar_wait_warp(i == 0 ? &q_full[g] : &s_read[g], i == 0 ? 0u : (uint32_t)((i - 1) & 1), s_abort)) return false;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < DH / 16; ++k)
-                            umma_bf16(tmem + g * 256, dq0 + (uint64_t)((g * Q_BYTES + (k >> 2) * ATOM_Q) >> 4) + 2 * (k & 3),
-                                      dk0 + (uint64_t)((sl * PP_TILE + (k >> 2) * ATOM_KV) >> 4) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
-                        umma_commit(&s_full[g]);
-                    }
-                    __syncwarp();
+                    for (int k = 0; k < DH / 16; ++k)
+                        umma_bf16(tmem_s, dq + (uint64_t)(((k >> 2) * ATOM_Q) >> 4) + 2 * (k & 3), dk + (uint64_t)(((k >> 2) * ATOM_KV) >> 4) + 2 * (k & 3),
+                                  idesc_s, k > 0 ? 1u : 0u);
+                    umma_commit(&s_full[g]);
+                    umma_commit(&empty[sl]);
+                } else {
+                    tbar_arrive(&empty[sl]);
                 }
-                if (elect_one()) umma_commit(&empty[sl]);
-                __syncwarp();
-                return true;
-            };
-            ok = issue_s(my_first);
-            for (int j = my_first; j < my_end && ok; ++j) {
-                if (j + 1 < my_end && !issue_s(j + 1)) { ok = false; break; }
-                const uint32_t t = 2u * (j - my_first) + 1, sl = t % PP_SLOTS;
-                if (!tbar_wait_warp(&full[sl], (t / PP_SLOTS) & 1u, s_abort)) { ok = false; break; }
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    if (!ok || j < lo[g] || j >= hi[g]) continue;
-                    const int i = j - lo[g];
-                    if (!tbar_wait_warp(&p_full[g * NP + i % NP], (uint32_t)((i / NP) & 1), s_abort)) { ok = false; continue; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < BK / 16; ++k)           // 16 keys a step: 8 columns of P, 16 rows of V
-                            pp_mma_ta(tmem + g * 256 + BK, tmem + g * 256 + BK + DH + (uint32_t)((i % NP) * (BK / 2)) + 8u * k, dv0 + (uint64_t)((sl * PP_TILE + k * 16 * 128) >> 4), idesc_o,
-                                      (i > 0 || k > 0) ? 1u : 0u);
-                        umma_commit(&o_full[g * NP + i % NP]);
-                    }
-                    __syncwarp();
-                }
-                if (elect_one()) umma_commit(&empty[sl]);
-                __syncwarp();
             }
-            if (!ok) atomicExch(s_abort, 1);
+            __syncwarp();
+            return true;
+        };
+        ok = issue_s(my_first);
+        for (int j = my_first; j < my_end && ok; ++j) {
+            if (j + 1 < my_end && !issue_s(j + 1)) { ok = false; break; }
+            const uint32_t t = 2u * (j - my_first) + 1, sl = t % PP_SLOTS;
+            const bool mine = j >= my_lo && j < my_hi;
+            const int i = j - my_lo;
+            if (!tbar_wait_warp(&full[sl], (t / PP_SLOTS) & 1u, s_abort)) { ok = false; break; }
+            if (mine && !tbar_wait_warp(&p_full[g * NP + i % NP], (uint32_t)((i / NP) & 1), s_abort)) { ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
+                if (mine) {
+                    const uint64_t dv = dv0 + (uint64_t)((sl * PP_TILE) >> 4);
+                    const uint32_t p_at = tmem_p + (uint32_t)((i % NP) * (BK / 2));
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k)               // 16 keys a step: 8 columns of P, 16 rows of V
+                        pp_mma_ta(tmem_o, p_at + 8u * k, dv + (uint64_t)((k * 16 * 128) >> 4), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
+                    umma_commit(&o_full[g * NP + i % NP]);
+                    umma_commit(&empty[sl]);
+                } else {
+                    tbar_arrive(&empty[sl]);
+                }
+            }
+            __syncwarp();
         }
+        if (!ok) atomicExch(s_abort, 1);
     } else {
         // ---- softmax warps: a lane of tensor memory is a query row; warps q and q + 4 of a group have a half of a block's keys each
         const int g = warp >> 3, q = warp & 3, half = (warp >> 2) & 1, r = q * 32 + lane;
@@ -306,7 +310,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
         const uint32_t tmem_s = tmem + g * 256 + lane_addr, tmem_o = tmem_s + BK, tmem_p = tmem_o + DH;
         unsigned char* q_tile = q_tiles + g * Q_BYTES;
-        float* sp = s_part + g * 512;
+        float* sp = s_part + g * 256;
         const float sl2 = scale * 1.4426950408889634f;              // scores in units of log2(e)
         const unsigned win_eff = window > 0 ? (unsigned)window : 0x7fffffffu;    // key visible: 0 ≤ q_pos − key < win_eff
         if (n_i > 0) {
@@ -331,10 +335,17 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             // chunks of 32 keys of which a row of this warp sees any (those behind lie above the diagonal)
             const int q_top = group_first + q * 32 + 31;
             const int n_live = MASKED ? (q_top < k0 ? 0 : min(NC, ((q_top - k0) >> 5) + 1)) : NC;
-            // (a warp that has given up goes on meeting its neighbour, who may not have)
-            if (!ok || !tbar_wait_warp(&s_full[g], (uint32_t)(i & 1), s_abort)) {
+            // (a warp that has given up goes on meeting its neighbour, who may not have, until both have: with nothing to tell)
+            const bool there = ok && tbar_wait_warp(&s_full[g], (uint32_t)(i & 1), s_abort);
+            if (!there) {
                 ok = false;
-                asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+                uint32_t any;
+                asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, 64, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+                             : "=r"(any) : "r"(0u), "r"(1 + g * 4 + q) : "memory");
+                if (any) {
+                    asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+                    asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+                }
                 return;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -362,18 +373,26 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                     for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], (unsigned)(d0 - x) < win_eff ? __uint_as_float(sv[0][x]) : -INFINITY);
                 }
             }
-            const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            sp[((i & 1) * 2 + half) * 128 + r] = m_half;
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+            const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
             // The weights' reference point m_run follows the row's maximum only where that has grown by 2^PP_LAZY: weights up to that are as exact in
-            // bfloat16 and float32 as weights up to 1, and O need not be scaled (for random rows in one block of twenty instead of all).
-            const float m_blk = fmaxf(m_half, sp[((i & 1) * 2 + (half ^ 1)) * 128 + r]) * sl2;
-            const float m_new = m_blk > m_run + PP_LAZY ? m_blk : m_run;
-            const float corr = m_run == -INFINITY ? 1.f : pp_exp2(m_run - m_new);        // (from −inf on the row's sums are 0 so far)
-            l_run *= corr;
-            m_run = m_new;
+            // bfloat16 and float32 as weights up to 1, O need not be scaled, and the halves of a row have nothing to tell one another (for random
+            // rows in all but one block of twenty): whether any row of the two warps grew is the barrier's own answer.
+            uint32_t any;
+            asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, 64, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+                         : "=r"(any) : "r"((uint32_t)(m_half > m_run + PP_LAZY)), "r"(1 + g * 4 + q) : "memory");
+            float corr = 1.f;
+            if (any) {                                              // (both warps)
+                sp[half * 128 + r] = m_half;
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+                const float m_blk = fmaxf(m_half, sp[(half ^ 1) * 128 + r]);
+                const float m_new = m_blk > m_run + PP_LAZY ? m_blk : m_run;
+                corr = m_run == -INFINITY ? 1.f : pp_exp2(m_run - m_new);          // (from −inf on the row's sums are 0 so far)
+                l_run *= corr;
+                m_run = m_new;
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");  // (read, before the next is written)
+            }
             const float m_use = (m_run == -INFINITY) ? 0.f : m_run; // a row that sees nothing yet: every p is 0
-            const bool grew = i > 0 && __any_sync(0xffffffffu, corr != 1.f);
+            const bool grew = i > 0 && any;
             // the P that goes where this one does has been multiplied; where O is to be scaled, all blocks before are in it
             const int before = grew ? i - 1 : i - NP;
             if (before >= 0) {
@@ -542,7 +561,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (*s_abort) {                                                 // MMAs under way read this CTA's shared memory: wait for them (bounded)
-        if (warp == SOFT + NPROD) {
+        if (warp >= SOFT + NPROD) {
             if (elect_one()) umma_commit(drained);
             __syncwarp();
             tbar_wait_warp(drained, 0, s_never);
@@ -557,7 +576,7 @@ template <int DH, int GROUPS>
 int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
               int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_seqs, int max_new, int H, int Hkv,
               float scale, int window, int n_parts, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
-    const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_SLOTS * PP_TILE + GROUPS * 512 * 4 + 32 * 8;
+    const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_SLOTS * PP_TILE + GROUPS * 256 * 4 + 32 * 8;
     static DeviceMarks marks;
     auto kern = attn_packed_prefill_kernel<DH, GROUPS>;
     cudaError_t e = allow_shared_memory(marks, kern, smem);
@@ -594,6 +613,7 @@ extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, cons
                  "attn_packed_prefill: %d heads over %d of %d, blocks of %d, row strides %d and %d are not taken", H, Hkv, dh, BT, ld, ld_out);
     VLRF_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && max_new >= 0 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && dev_err != nullptr,
                  "attn_packed_prefill: bad arguments");
+    VLRF_REQUIRE(scale >= 0.f, "attn_packed_prefill: a scale of %g is negative", (double)scale);       // (a row's maximum is taken of the raw scores)
     VLRF_REQUIRE(groups == 1 || groups == 2, "attn_packed_prefill: %d groups of 128 queries a CTA (1 or 2)", groups);
     VLRF_REQUIRE(n_parts >= 1 && n_parts <= PP_MAX_PARTS && (n_parts == 1 || (partials != nullptr && counters != nullptr)),
                  "attn_packed_prefill: %d parts (1 to %d; more than one wants scratch)", n_parts, PP_MAX_PARTS);

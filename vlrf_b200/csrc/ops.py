@@ -1139,7 +1139,7 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
         attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
                                 window, n_split, ctx.dev_err, partials, counters)
         return
-    if ctx.max_new > 1 and _packed_prefill_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
+    if ctx.max_new > 1 and scale >= 0.0 and _packed_prefill_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
         groups, n_parts = packed_prefill_shape(ctx.n_tokens, ctx.n_seqs, ctx.max_new, ctx.max_context, n_heads, head_dim, window)
         partials = counters = None
         if n_parts > 1:
