@@ -1,10 +1,10 @@
 // Prompt attention over a cache of keys and values in 4 bits (packed_kv.cuh) on the tcgen05 tensor cores: ragged, causal, with or without a
 // window, bfloat16, head sizes 64 and 128.
 //
-// A CTA takes GROUPS · 128 consecutive new tokens of one sequence and one head and walks the keys they see in blocks of BK (128 keys of
-// 64 numbers, 64 of 128) up to the diagonal.  Its warps have fixed jobs:
+// A CTA takes GROUPS · 128 consecutive new tokens of one sequence and one head and walks the keys they see in blocks of 64 up to the
+// diagonal.  Its warps have fixed jobs:
 //   producers      codes and pairs of a block from the cache into registers, a block ahead; from there zero + step · code as bfloat16 (one rounding)
-//                  into a ring of four shared-memory slots, K and V in turn, in the 128-byte swizzle that the MMA reads.  A code becomes
+//                  into a ring of 64 KB of shared memory, K and V in turn, in the 128-byte swizzle that the MMA reads.  A code becomes
 //                  a bfloat16 by a mask under the exponent of 128, less 128 (exact), two at a time; pairs of entries i and i + 4 of eight
 //                  stay neighbours, so the numbers of a row lie permuted, those of the queries likewise (the sum does not care), and the
 //                  result is put in order where it is written.  Rows that no query may see, behind the sequence's last token or in
@@ -26,10 +26,9 @@
 #include "tcgen05.cuh"
 
 namespace {
-constexpr int PP_CB = 64, PP_SLOTS = 4, PP_TILE = 16384;            // tokens of a cache block; slots of the ring, bytes of each
+constexpr int PP_CB = 64, PP_BK = 64, PP_RING = 65536;              // tokens of a cache block; keys of a block; bytes of the ring
 constexpr int PP_PART_BLOCKS = 3, PP_MAX_PARTS = 16;
-constexpr float PP_LAZY = 6.f;
-constexpr __host__ __device__ int pp_bk(int DH) { return DH == 64 ? 128 : 64; }
+constexpr float PP_MOST = 2048.f, PP_LEAST = 4.f;                   // (64 weights that add up to 2^11: one is 2^5 at least)
 constexpr __host__ __device__ int pp_producers(int GROUPS) { return 2 * GROUPS; }
 constexpr __host__ __device__ int pp_threads(int GROUPS) { return (GROUPS * 8 + pp_producers(GROUPS) + GROUPS) * 32; }
 constexpr __host__ __device__ int pp_part_floats(int DH) { return DH * 128 + 256; }
@@ -38,6 +37,23 @@ __device__ __forceinline__ float pp_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// two float32 numbers that go through one instruction (sm_100)
+__device__ __forceinline__ uint64_t pp_two(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void pp_apart(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t pp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pp_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 // MN-major tile: rows of 64 elements (128 bytes, swizzled) are the operand's N, a row a step of its K; groups of 8 rows 1024 bytes apart, chunks of
 // 64 along N `chunk` bytes apart
@@ -98,7 +114,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                            int max_blocks, const int* __restrict__ seq_slot, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
                            __nv_bfloat16* __restrict__ out, int ld_out, int H, int Hkv, float scale, int window, int n_parts, float* __restrict__ partials,
                            int* __restrict__ counters, int n_tiles, int* __restrict__ dev_err) {
-    constexpr int BK = pp_bk(DH), ROWS = GROUPS * 128, NG = DH / 64, NPROD = pp_producers(GROUPS), SOFT = GROUPS * 8;
+    constexpr int BK = PP_BK, PP_TILE = BK * DH * 2, PP_SLOTS = PP_RING / PP_TILE, ROWS = GROUPS * 128, NG = DH / 64, NPROD = pp_producers(GROUPS), SOFT = GROUPS * 8;
     constexpr int Q_BYTES = 128 * DH * 2, ATOM_Q = 16384, ATOM_KV = BK * 128;    // a 64-number chunk of 128 queries / of a block
     constexpr int NP = BK + DH + BK <= 256 ? 2 : 1;                 // buffers of P that a group's 256 columns have room for
     constexpr int HK = BK / 2, NC = HK / 32, HD = DH / 2;           // keys, chunks of 32 keys, and columns of O of a softmax thread
@@ -106,7 +122,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(pp_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* q_tiles = smem;                                  // [GROUPS][NG][128][128 B]
     unsigned char* kv_tiles = smem + GROUPS * Q_BYTES;              // [PP_SLOTS][NG][BK][128 B]: K_0, V_0, K_1, V_1, …
-    float* s_part = reinterpret_cast<float*>(kv_tiles + PP_SLOTS * PP_TILE);     // [GROUPS][2][128]
+    float* s_part = reinterpret_cast<float*>(kv_tiles + PP_RING);     // [GROUPS][2][128]
     uint64_t* q_full = reinterpret_cast<uint64_t*>(s_part + GROUPS * 256);       // [GROUPS]
     uint64_t* full = q_full + GROUPS;
     uint64_t* empty = full + PP_SLOTS;
@@ -349,9 +365,58 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                 return;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t s_at = tmem_s + (uint32_t)(half * HK);
+            const uint32_t s_at = tmem_s + (uint32_t)(half * HK), p_at = tmem_p + (uint32_t)((i % NP) * (BK / 2) + half * (HK / 2));
             uint32_t sv[NC][32];
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // Exponentials of a chunk against m_use, P as bfloat16 into tensor memory; their sum onto `sum`.
+            auto chunk = [&](int c, const uint32_t (&x)[32], float m_use, uint64_t (&sum)[2]) {
+                uint32_t pk[16];
+                const int d0 = q_pos - (k0 + c * 32);               // q_pos − key for e = 0
+                const uint64_t by = pp_two(sl2, sl2), from = pp_two(-m_use, -m_use);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float p0, p1;
+                    pp_apart(pp_fma2(pp_two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), by, from), p0, p1);
+                    p0 = pp_exp2(p0);
+                    p1 = pp_exp2(p1);
+                    if (MASKED) {
+                        p0 = (unsigned)(d0 - e) < win_eff ? p0 : 0.f;
+                        p1 = (unsigned)(d0 - e - 1) < win_eff ? p1 : 0.f;
+                    }
+                    sum[(e >> 1) & 1] = pp_add2(sum[(e >> 1) & 1], pp_two(p0, p1));
+                    pk[e >> 1] = pack2(p0, p1);
+                }
+                pp_st16(p_at + (uint32_t)(c * 16), pk);
+            };
+            auto total = [](const uint64_t (&sum)[2]) {
+                float a0, a1, b0, b1;
+                pp_apart(sum[0], a0, a1);
+                pp_apart(sum[1], b0, b1);
+                return (a0 + a1) + (b0 + b1);
+            };
+            // whether any row of the two warps asks for it
+            auto either = [&](bool mine) {
+                uint32_t any;
+                asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, 64, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+                             : "=r"(any) : "r"((uint32_t)mine), "r"(1 + g * 4 + q) : "memory");
+                return any != 0;
+            };
+            // The weights' reference point m_run moves to the row's maximum where that lies 2^least above it (both halves' maxima meet in shared memory);
+            // returns what the sums so far are to be multiplied by.
+            auto move_reference = [&](float m_half, float least) {
+                sp[half * 128 + r] = m_half;
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
+                const float m_blk = fmaxf(m_half, sp[(half ^ 1) * 128 + r]);
+                const float m_new = m_blk > m_run + least ? m_blk : m_run;
+                const float corr = m_run == -INFINITY ? 1.f : pp_exp2(m_run - m_new);    // (from −inf on the row's sums are 0 so far)
+                l_run *= corr;
+                m_run = m_new;
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");        // (read, before the next is written)
+                return corr;
+            };
+            auto reference = [&]() { return m_run == -INFINITY ? 0.f : m_run; };         // (a row that sees nothing yet: every weight is 0)
+            float corr = 1.f, sum = 0.f;
+            bool moved;
+            // (P goes where the product of NP blocks before has read it; where O is to be scaled, all blocks before are in it)
             if (!MASKED) {
 #pragma unroll
                 for (int c = 0; c < NC; ++c) tmem_ld32(s_at + 32u * c, sv[c]);
@@ -359,86 +424,72 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) tbar_arrive(&s_read[g]);
+                // No maximum is looked for while the weights against the reference point stay small: they are as exact in bfloat16 and float32 up to 2^11 as
+                // up to 1.  A row whose weights of this block add up to more (for random rows hardly any behind the first block) moves its reference
+                // point, and the two warps begin the block anew.
+                if (i > 0) {
+                    if (i >= NP && !wait_o(i - NP)) ok = false;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    uint64_t s2[2] = {0ull, 0ull};
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
+                    for (int c = 0; c < NC; ++c) chunk(c, sv[c], reference(), s2);
+                    sum = total(s2);
+                }
+                moved = either(i == 0 || m_run == -INFINITY || sum > PP_MOST);
+                if (moved) {
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(sv[c][x]));
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(sv[c][x]));
+                    corr = move_reference(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2, PP_LEAST);
+                    if (i > 0 && !wait_o(i - 1)) ok = false;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    uint64_t s2[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) chunk(c, sv[c], reference(), s2);
+                    sum = total(s2);
+                }
+                if (!ok) return;
             } else {
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
                 for (int c = 0; c < n_live; ++c) {
                     tmem_ld32(s_at + (uint32_t)(c * 32), sv[0]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    const int d0 = q_pos - (k0 + c * 32);           // q_pos − key for x = 0
+                    const int d0 = q_pos - (k0 + c * 32);
 #pragma unroll
                     for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], (unsigned)(d0 - x) < win_eff ? __uint_as_float(sv[0][x]) : -INFINITY);
                 }
-            }
-            const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-            // The weights' reference point m_run follows the row's maximum only where that has grown by 2^PP_LAZY: weights up to that are as exact in
-            // bfloat16 and float32 as weights up to 1, O need not be scaled, and the halves of a row have nothing to tell one another (for random
-            // rows in all but one block of twenty): whether any row of the two warps grew is the barrier's own answer.
-            uint32_t any;
-            asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, 64, p;\nselp.u32 %0, 1, 0, q;\n}\n"
-                         : "=r"(any) : "r"((uint32_t)(m_half > m_run + PP_LAZY)), "r"(1 + g * 4 + q) : "memory");
-            float corr = 1.f;
-            if (any) {                                              // (both warps)
-                sp[half * 128 + r] = m_half;
-                asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
-                const float m_blk = fmaxf(m_half, sp[(half ^ 1) * 128 + r]);
-                const float m_new = m_blk > m_run + PP_LAZY ? m_blk : m_run;
-                corr = m_run == -INFINITY ? 1.f : pp_exp2(m_run - m_new);          // (from −inf on the row's sums are 0 so far)
-                l_run *= corr;
-                m_run = m_new;
-                asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");  // (read, before the next is written)
-            }
-            const float m_use = (m_run == -INFINITY) ? 0.f : m_run; // a row that sees nothing yet: every p is 0
-            const bool grew = i > 0 && any;
-            // the P that goes where this one does has been multiplied; where O is to be scaled, all blocks before are in it
-            const int before = grew ? i - 1 : i - NP;
-            if (before >= 0) {
-                if (!wait_o(before)) { ok = false; return; }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            }
-            float sm4[4] = {0.f, 0.f, 0.f, 0.f};
-            auto chunk = [&](int c, const uint32_t (&x)[32]) {
-                uint32_t pk[16];
-                const int d0 = q_pos - (k0 + c * 32);
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float p0 = pp_exp2(fmaf(__uint_as_float(x[e]), sl2, -m_use)), p1 = pp_exp2(fmaf(__uint_as_float(x[e + 1]), sl2, -m_use));
-                    if (MASKED) {
-                        p0 = (unsigned)(d0 - e) < win_eff ? p0 : 0.f;
-                        p1 = (unsigned)(d0 - e - 1) < win_eff ? p1 : 0.f;
-                    }
-                    sm4[e & 3] += p0;
-                    sm4[(e + 1) & 3] += p1;
-                    pk[e >> 1] = pack2(p0, p1);
+                const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+                moved = either(m_half > m_run + PP_LEAST);
+                if (moved) corr = move_reference(m_half, PP_LEAST);
+                const int before = moved ? i - 1 : i - NP;
+                if (before >= 0) {
+                    if (!wait_o(before)) { ok = false; return; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
-                pp_st16(tmem_p + (uint32_t)((i % NP) * (BK / 2) + half * (HK / 2) + c * 16), pk);
-            };
-            if (!MASKED) {
-#pragma unroll
-                for (int c = 0; c < NC; ++c) chunk(c, sv[c]);
-            } else {
+                uint64_t s2[2] = {0ull, 0ull};
 #pragma unroll 1
                 for (int c = 0; c < NC; ++c) {
                     if (c < n_live) {
                         tmem_ld32(s_at + (uint32_t)(c * 32), sv[0]);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        chunk(c, sv[0]);
+                        chunk(c, sv[0], reference(), s2);
                     } else {
                         uint32_t none[16];
 #pragma unroll
                         for (int x = 0; x < 16; ++x) none[x] = 0u;
-                        pp_st16(tmem_p + (uint32_t)((i % NP) * (BK / 2) + half * (HK / 2) + c * 16), none);
+                        pp_st16(p_at + (uint32_t)(c * 16), none);
                     }
                 }
+                sum = total(s2);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) tbar_arrive(&s_read[g]);
             }
-            l_run += (sm4[0] + sm4[1]) + (sm4[2] + sm4[3]);
-            if (grew) {                                             // a row's reference point moved: its O (a half of the columns here) follows
+            l_run += sum;
+            if (i > 0 && moved) {                                           // a row's reference point moved: its O (a half of the columns here) follows
 #pragma unroll
                 for (int d0 = 0; d0 < HD; d0 += 32) {
                     uint32_t ov[32];
@@ -576,7 +627,7 @@ template <int DH, int GROUPS>
 int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
               int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_seqs, int max_new, int H, int Hkv,
               float scale, int window, int n_parts, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
-    const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_SLOTS * PP_TILE + GROUPS * 256 * 4 + 32 * 8;
+    const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_RING + GROUPS * 256 * 4 + 40 * 8;
     static DeviceMarks marks;
     auto kern = attn_packed_prefill_kernel<DH, GROUPS>;
     cudaError_t e = allow_shared_memory(marks, kern, smem);

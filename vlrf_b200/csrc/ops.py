@@ -1044,9 +1044,8 @@ def _packed_prefill_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n
 
 def packed_prefill_shape(n_tokens: int, n_seqs: int, max_new: int, max_context: int, n_heads: int, head_dim: int, window: int = 0) -> tuple:
     """(groups of 128 queries a CTA of `attention_prefill_packed` takes, parts to which it deals the keys of a long tile)."""
-    keys = 128 if head_dim == 64 else 64
-    reach = min(max_context, window + 127) if window > 0 else max_context
-    chain = -(-reach // keys)
+    reach = min(max_context, window + 255) if window > 0 else max_context
+    chain = -(-reach // 64)
     tiles = (n_tokens // 256 + n_seqs) * n_heads
     return 2, max(1, min(16, (2 * sm_count()) // max(1, tiles), chain // 6))
 
