@@ -347,7 +347,7 @@ def prefill(pages, new, heads, kv_heads, dim, window, groups, n_parts, scratch=N
 
     def fn(qkv, q_off, table, slot, pos, out, scale, e):
         ops.attention_prefill_packed(qkv, q_off, pages.cache, table, ints(list(range(len(new)))), ints(start), ints([n - a for a, n in zip(new, pages.lengths)]),
-                                     out, sum(new), len(new), max(new), heads, kv_heads, dim, scale, window, e, groups, n_parts, partials, counters)
+                                     out, sum(new), len(new), max(new), heads, kv_heads, dim, scale, window, e, groups, n_parts, 2, partials, counters)
         assert int(counters.abs().sum()) == 0
     return fn
 

@@ -358,16 +358,16 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
     }
     if (n_split == 1) return;
     // the CTA that finds all parts there merges them, each in its turn, so the sum does not depend on who came last
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();                                            // (of everything that the barrier has shown this thread)
         const int before = atomicAdd(&counters[place], 1);
         s_last = before == n_split - 1;
         if (s_last) counters[place] = 0;                            // left as it was found
+        __threadfence();
     }
     __syncthreads();
     if (!s_last) return;
-    __threadfence();
     // lanes of threads: SHARES of them take every SHARES-th part of a piece of four numbers, and meet in shared memory
     constexpr int N4 = RC * (DH / 4), SHARES = WARPS * 32 / N4 > 0 ? WARPS * 32 / N4 : 1;
     float* meet = reinterpret_cast<float*>(pd_raw);                 // [SHARES][N4][8]
@@ -376,7 +376,7 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
         float M = -INFINITY, L = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (qi < n_q) {
-#pragma unroll 4
+#pragma unroll 8
             for (int p = share; p < n_split; p += SHARES) {
                 const float* theirs = my_parts + (size_t)(p * RC + qi) * (DH + 4);
                 const float2 ml = __ldcg(reinterpret_cast<const float2*>(theirs + DH));

@@ -27,7 +27,7 @@
 
 namespace {
 constexpr int PP_CB = 64, PP_BK = 64, PP_RING = 65536;              // tokens of a cache block; keys of a block; bytes of the ring
-constexpr int PP_PART_BLOCKS = 3, PP_MAX_PARTS = 16;
+constexpr int PP_MAX_PARTS = 16;
 constexpr float PP_MOST = 2048.f, PP_LEAST = 4.f;                   // (64 weights that add up to 2^11: one is 2^5 at least)
 constexpr __host__ __device__ int pp_producers(int GROUPS) { return 2 * GROUPS; }
 constexpr __host__ __device__ int pp_threads(int GROUPS) { return (GROUPS * 8 + pp_producers(GROUPS) + GROUPS) * 32; }
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(pp_threads(GROUPS), GROUPS == 1 ? 2 : 1)
 attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_off, const unsigned char* __restrict__ Kq, const uint32_t* __restrict__ Kp,
                            const unsigned char* __restrict__ Vq, const uint32_t* __restrict__ Vp, int n_blocks, const int* __restrict__ block_table,
                            int max_blocks, const int* __restrict__ seq_slot, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
-                           __nv_bfloat16* __restrict__ out, int ld_out, int H, int Hkv, float scale, int window, int n_parts, float* __restrict__ partials,
+                           __nv_bfloat16* __restrict__ out, int ld_out, int H, int Hkv, float scale, int window, int n_parts, int part_blocks, float* __restrict__ partials,
                            int* __restrict__ counters, int n_tiles, int* __restrict__ dev_err) {
     constexpr int BK = PP_BK, PP_TILE = BK * DH * 2, PP_SLOTS = PP_RING / PP_TILE, ROWS = GROUPS * 128, NG = DH / 64, NPROD = pp_producers(GROUPS), SOFT = GROUPS * 8;
     constexpr int Q_BYTES = 128 * DH * 2, ATOM_Q = 16384, ATOM_KV = BK * 128;    // a 64-number chunk of 128 queries / of a block
@@ -161,8 +161,8 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     const int n_rows = min(n_new - t_first, ROWS), q_last = q_first + n_rows - 1;
     const int first_key = window > 0 ? max(0, q_first - window + 1) : 0;
     const int kb_first = first_key / BK, n_kb = q_last / BK - kb_first + 1;
-    // the tile's key blocks are dealt to tile_parts CTAs; the others of its n_parts have nothing to do
-    const int tile_parts = max(1, min(n_parts, (n_kb + PP_PART_BLOCKS - 1) / PP_PART_BLOCKS));
+    // the tile's key blocks are dealt to tile_parts CTAs, of part_blocks each or more; the others of its n_parts have nothing to do
+    const int tile_parts = max(1, min(n_parts, (n_kb + part_blocks - 1) / part_blocks));
     const bool active = n_rows > 0 && slot >= 0 && pos0 >= 0 && part < tile_parts;      // uniform over the CTA
     if (!active) return;                                            // (before it holds anything)
     constexpr uint32_t TMEM_COLS = 256 * GROUPS;                    // a group: S BK columns, O DH, P NP times BK / 2 (two bfloat16 a column)
@@ -626,7 +626,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
 template <int DH, int GROUPS>
 int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
               int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_seqs, int max_new, int H, int Hkv,
-              float scale, int window, int n_parts, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+              float scale, int window, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
     const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_RING + GROUPS * 256 * 4 + 40 * 8;
     static DeviceMarks marks;
     auto kern = attn_packed_prefill_kernel<DH, GROUPS>;
@@ -636,7 +636,7 @@ int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp
     VLRF_REQUIRE(tiles * n_parts <= 65535, "attn_packed_prefill: %lld tiles of %d parts are too many for one launch", tiles, n_parts);
     e = launch_chained(kern, dim3(H, n_seqs, (unsigned)(tiles * n_parts)), dim3(pp_threads(GROUPS)), smem, stream, (const __nv_bfloat16*)qkv, ld, q_off,
                        (const unsigned char*)Kq, (const uint32_t*)Kp, (const unsigned char*)Vq, (const uint32_t*)Vp, n_blocks, block_table, max_blocks, seq_slot,
-                       seq_start, seq_pos0, (__nv_bfloat16*)out, ld_out, H, Hkv, scale, window, n_parts, partials, counters, (int)tiles, dev_err);
+                       seq_start, seq_pos0, (__nv_bfloat16*)out, ld_out, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, (int)tiles, dev_err);
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_prefill: %s", cudaGetErrorString(e));
     return vlrf_check_launch("attn_packed_prefill");
 }
@@ -659,20 +659,20 @@ extern "C" int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, 
 extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                                         const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out,
                                         int ld_out, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int groups, int n_parts,
-                                        float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+                                        int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
     VLRF_REQUIRE(vlrf_attn_packed_prefill_takes(H, Hkv, dh, BT, ld, q_off, ld_out),
                  "attn_packed_prefill: %d heads over %d of %d, blocks of %d, row strides %d and %d are not taken", H, Hkv, dh, BT, ld, ld_out);
     VLRF_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && max_new >= 0 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && dev_err != nullptr,
                  "attn_packed_prefill: bad arguments");
     VLRF_REQUIRE(scale >= 0.f, "attn_packed_prefill: a scale of %g is negative", (double)scale);       // (a row's maximum is taken of the raw scores)
     VLRF_REQUIRE(groups == 1 || groups == 2, "attn_packed_prefill: %d groups of 128 queries a CTA (1 or 2)", groups);
-    VLRF_REQUIRE(n_parts >= 1 && n_parts <= PP_MAX_PARTS && (n_parts == 1 || (partials != nullptr && counters != nullptr)),
+    VLRF_REQUIRE(n_parts >= 1 && n_parts <= PP_MAX_PARTS && part_blocks >= 1 && (n_parts == 1 || (partials != nullptr && counters != nullptr)),
                  "attn_packed_prefill: %d parts (1 to %d; more than one wants scratch)", n_parts, PP_MAX_PARTS);
     for (const void* p : {qkv, Kq, Kp, Vq, Vp, (const void*)out})
         VLRF_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "attn_packed_prefill: tensors begin on 16 bytes");
     if (n_seqs == 0 || max_new == 0) return VLRF_OK;
 #define GO(DH, G) pp_launch<DH, G>(qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, seq_slot, seq_start, seq_pos0, out, ld_out, n_seqs, \
-                                   max_new, H, Hkv, scale, window, n_parts, partials, counters, dev_err, stream)
+                                   max_new, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, dev_err, stream)
     if (dh == 64) return groups == 1 ? GO(64, 1) : GO(64, 2);
     return groups == 1 ? GO(128, 1) : GO(128, 2);
 #undef GO

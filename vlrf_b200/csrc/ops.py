@@ -7,6 +7,7 @@ no function has a CPU or library fallback.
 from __future__ import annotations
 
 import dataclasses
+import functools
 import os
 
 import torch
@@ -1042,20 +1043,58 @@ def _packed_prefill_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n
     return bool(library().vlrf_attn_packed_prefill_takes(n_heads, n_kv_heads, head_dim, cache.block_tokens, qkv.stride(0), q_off, out.stride(0)))
 
 
-def packed_prefill_shape(n_tokens: int, n_seqs: int, max_new: int, max_context: int, n_heads: int, head_dim: int, window: int = 0) -> tuple:
-    """(groups of 128 queries a CTA of `attention_prefill_packed` takes, parts to which it deals the keys of a long tile)."""
-    reach = min(max_context, window + 255) if window > 0 else max_context
-    chain = -(-reach // 64)
-    tiles = (n_tokens // 256 + n_seqs) * n_heads
-    return 2, max(1, min(16, (2 * sm_count()) // max(1, tiles), chain // 6))
+#: Microseconds of a CTA of `attention_prefill_packed`, measured: its start, queries and result (with one and with two groups of queries), a block of 64 keys
+#: (head sizes 64 and 128), and meeting the other parts of a tile in scratch.
+PACKED_PROMPT_US = dict(cta=(4.5, 5.5), block={64: 1.05, 128: 1.45}, meet=5.0)
+
+
+def packed_prefill_shape(lens, pos0, n_heads: int, head_dim: int, window: int = 0) -> tuple:
+    """(groups of 128 queries a CTA of `attention_prefill_packed` takes, most CTAs to which it deals the keys of a tile, blocks of 64 that each of those
+    holds at least) for sequences that bring lens[i] tokens behind pos0[i].  Two groups share the keys that a CTA takes apart; one makes twice the CTAs,
+    two an SM, which pays for small heads and few tokens (one prompt of 200 tokens of 12 heads of 64: 8.1 us against 9.5; four of 1,000 behind 4,000: 176
+    against 163).  A tile's blocks are a chain: parts shorten it where the tiles leave SMs idle (512 tokens of 32 heads of 128 behind 7,500: 172 us whole, 102
+    in two parts, 140 in three, which come in two waves)."""
+    return _packed_prefill_shape(tuple(lens), tuple(pos0), n_heads, head_dim, window)
+
+
+@functools.lru_cache(maxsize=1024)                # (a rule of sizes alone; worked out anew it takes longer than a launch)
+def _packed_prefill_shape(lens: tuple, pos0: tuple, n_heads: int, head_dim: int, window: int) -> tuple:
+    best = None
+    for groups in (1, 2) if head_dim == 64 else (2,):
+        places, rows = sm_count() * (3 - groups), 128 * groups
+        cta, block, meet = PACKED_PROMPT_US["cta"][groups - 1], PACKED_PROMPT_US["block"][head_dim], PACKED_PROMPT_US["meet"]
+        lengths: dict = {}                         # blocks of a tile -> tiles of a head that have so many
+        for a, b in zip(lens, pos0):
+            for t in range(0, a, rows):
+                n = (b + min(t + rows, a) - 1) // 64 - (max(0, b + t - window + 1) // 64 if window > 0 else 0) + 1
+                lengths[n] = lengths.get(n, 0) + 1
+        chain, work = max(lengths), sum(n * k for n, k in lengths.items())
+        even = 4 * work > 3 * chain * sum(lengths.values())
+        for each in sorted({-(-chain // k) for k in ((1,) if groups == 1 else (1, 2, 3, 4, 6, 8, 12, 16))} | ({-(-3 * chain // 4)} if groups == 2 else set()),
+                           reverse=True):
+            if each < min(chain, 6):
+                break
+            parts = {n: min(16, -(-n // each)) for n in lengths}
+            ctas = n_heads * sum(k * parts[n] for n, k in lengths.items())
+            longest = max(cta + -(-n // p) * block + (meet if p > 1 else 0.0) for n, p in parts.items())
+            if ctas <= places:
+                time = longest
+            elif even:
+                time = -(-ctas // places) * longest
+            else:
+                busy = sum(k * (n * block + parts[n] * (0.6 * cta + (meet if parts[n] > 1 else 0.0))) for n, k in lengths.items())
+                time = max(longest, n_heads * busy / places + longest / 2)
+            if best is None or time < 0.97 * best[0]:
+                best = (time, groups, max(parts.values()), each)
+    return best[1:]
 
 
 def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_slot, seq_start, seq_pos0, out, n_tokens: int, n_seqs: int, max_new: int,
                              n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int, dev_err, groups: int = 1, n_parts: int = 1,
-                             partials=None, counters=None) -> None:
+                             part_blocks: int = 6, partials=None, counters=None) -> None:
     """Causal attention of every sequence's new tokens (rows seq_start[i] … seq_start[i+1]−1 of qkv, the first of them at position
     seq_pos0[i]) over the sequence's cache of 4 bits, which already holds these tokens; bfloat16, head size 64 or 128, on the tcgen05
-    tensor cores.  n_parts > 1 wants float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero."""
+    tensor cores.  n_parts > 1 deals the keys of long tiles to that many CTAs (see packed_prefill_shape) and wants float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero."""
     what = "attention_prefill_packed"
     _attention_packed_check(what, qkv, q_off, cache, block_table, (seq_slot, seq_start, seq_pos0), out, n_tokens, n_heads, n_kv_heads, head_dim, window,
                             dev_err)
@@ -1066,7 +1105,7 @@ def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_
         scratch = _packed_scratch(what, packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts), partials, counters)
     call("vlrf_attn_packed_prefill", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], seq_slot.data_ptr(),
          seq_start.data_ptr(), seq_pos0.data_ptr(), out.data_ptr(), out.stride(0), n_seqs, max_new, n_heads, n_kv_heads, head_dim, cache.block_tokens,
-         float(scale), window, groups, n_parts, *scratch, dev_err.data_ptr(), _stream())
+         float(scale), window, groups, n_parts, part_blocks, *scratch, dev_err.data_ptr(), _stream())
 
 
 def packed_prefill_scratch(n_seqs: int, max_new: int, n_heads: int, head_dim: int, groups: int, n_parts: int) -> tuple:
@@ -1139,14 +1178,14 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
                                 window, n_split, ctx.dev_err, partials, counters)
         return
     if ctx.max_new > 1 and scale >= 0.0 and _packed_prefill_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
-        groups, n_parts = packed_prefill_shape(ctx.n_tokens, ctx.n_seqs, ctx.max_new, ctx.max_context, n_heads, head_dim, window)
+        groups, n_parts, part_blocks = packed_prefill_shape(ctx.host_seq_lens, ctx.host_seq_pos0, n_heads, head_dim, window)
         partials = counters = None
         if n_parts > 1:
             n_floats, n_counters = packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts)
             partials = ctx.ws.get("packed_partials", n_floats, 1, torch.float32)
             counters = ctx.ws.get_zeroed("packed_counters", n_counters, torch.int32)
         attention_prefill_packed(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_start, ctx.seq_pos0, out, ctx.n_tokens, ctx.n_seqs, ctx.max_new,
-                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, partials, counters)
+                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, part_blocks, partials, counters)
         return
     attention_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
                      window, ctx.dev_err)

@@ -479,8 +479,8 @@ int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const void* Kq, 
                             cudaStream_t stream);
 int vlrf_attn_packed_decode_force(int few);    // for measurements and tests: a CTA an SM (1), several (0), chosen by size again (−1)
 // A prompt step of it on the tcgen05 tensor cores, bfloat16, head sizes 64 and 128, blocks of 64: sequences as in vlrf_attn_prefill (slot −1:
-// skipped).  A CTA takes `groups` (1 or 2) times 128 queries of a head; n_parts > 1 deals the keys of long tiles to that many CTAs (up to
-// vlrf_attn_packed_prefill_max_parts()), which meet in scratch: float32 partials and int32 counters, zero before the first call (every
+// skipped).  A CTA takes `groups` (1 or 2) times 128 queries of a head; n_parts > 1 deals the keys of long tiles, part_blocks blocks of 64 to each or
+// more, to that many CTAs (up to vlrf_attn_packed_prefill_max_parts()), which meet in scratch: float32 partials and int32 counters, zero before the first call (every
 // call leaves them zero), of the sizes that vlrf_attn_packed_prefill_scratch gives (host pointers).
 int vlrf_attn_packed_prefill_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out);
 int vlrf_attn_packed_prefill_max_parts();
@@ -488,7 +488,7 @@ int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, int dh, int
 int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                              const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0,
                              void* out, int ld_out, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int groups,
-                             int n_parts, float* partials, int* counters, int* dev_err, cudaStream_t stream);
+                             int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream);
 
 // ---- routed experts (moe.cu) ---------------------------------------------------------------------------------------
 // z: float32 router logits [T][ld_z] (column E: the logit of a shared expert's gate, if shared_gate).  ids, wts, rank
