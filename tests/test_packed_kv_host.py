@@ -66,14 +66,14 @@ def test_attention_refuses(change):
 
 
 @pytest.mark.parametrize("change", [dict(dh=32), dict(dh=320), dict(rows=-1), dict(rows=70000), dict(H=3), dict(BT=32), dict(max_blocks=0), dict(window=-1),
-                                    dict(dev_err=None), dict(n_split=0), dict(n_split=65), dict(n_split=2), dict(ld=385), dict(q_off=4), dict(ld_out=130), dict(qkv=4100)])
+                                    dict(dev_err=None), dict(n_split=0), dict(n_split=65), dict(n_split=2), dict(part_tiles=0), dict(ld=385), dict(q_off=4), dict(ld_out=130), dict(qkv=4100)])
 def test_decode_attention_refuses(change):
     from vlrf_b200.csrc import library
     lib = library()
-    a = dict(dict(rows=3, H=4, Hkv=2, dh=64, BT=64, max_blocks=4, window=0, n_split=1, ld=512, q_off=0, ld_out=256, qkv=4096,
+    a = dict(dict(rows=3, H=4, Hkv=2, dh=64, BT=64, max_blocks=4, window=0, n_split=1, part_tiles=1, ld=512, q_off=0, ld_out=256, qkv=4096,
                   dev_err=ctypes.c_void_p(4096)), **change)
     assert lib.vlrf_attn_packed_decode(ctypes.c_void_p(a["qkv"]), a["ld"], a["q_off"], *pointers(4), 10, *pointers(1), a["max_blocks"], *pointers(3),
-                                       a["ld_out"], a["rows"], a["H"], a["Hkv"], a["dh"], a["BT"], 0.125, a["window"], a["n_split"], None, None, a["dev_err"],
+                                       a["ld_out"], a["rows"], a["H"], a["Hkv"], a["dh"], a["BT"], 0.125, a["window"], 0, a["n_split"], a["part_tiles"], None, None, a["dev_err"],
                                        None) != 0
     assert b"attn_packed_decode" in lib.vlrf_last_error()
 

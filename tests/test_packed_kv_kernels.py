@@ -278,10 +278,7 @@ def scratch(rows, heads, kv_heads, dim, n_split):
 
 @pytest.fixture(params=[1, 0], ids=["a CTA an SM", "several"])
 def few(request):
-    from vlrf_b200.csrc import call_host
-    call_host("vlrf_attn_packed_decode_force", request.param)
-    yield request.param
-    call_host("vlrf_attn_packed_decode_force", -1)
+    return request.param
 
 
 DECODE_SHAPES = [(3, 3, 64), (8, 2, 128), (6, 2, 64), (4, 2, 128), (4, 4, 128), (2, 1, 256), (2, 2, 192), (12, 1, 64), (24, 1, 128), (40, 2, 64), (10, 1, 256)]
@@ -289,13 +286,13 @@ DECODE_SHAPES = [(3, 3, 64), (8, 2, 128), (6, 2, 64), (4, 2, 128), (4, 4, 128), 
 
 @pytest.mark.parametrize("heads,kv_heads,dim", DECODE_SHAPES)
 @pytest.mark.parametrize("window", [0, 1, 70])
-@pytest.mark.parametrize("n_split", [1, 3, 37])
-def test_decode_attention_on_the_tensor_cores(heads, kv_heads, dim, window, n_split, few):
+@pytest.mark.parametrize("n_split,part_tiles", [(1, 32), (3, 11), (37, 1), (2, 1)])
+def test_decode_attention_on_the_tensor_cores(heads, kv_heads, dim, window, n_split, part_tiles, few):
     """Contexts of one token, of whole blocks, of a token more, longer than all stages of a warp's ring; more parts than tiles."""
     from vlrf_b200.csrc import ops
     pages = Pages([1, 64, 65, 130, 2000, 7], kv_heads, dim, seed=heads)
     run_tokens(lambda qkv, q_off, table, slot, pos, out, scale, e: ops.attention_decode_packed(
-        qkv, q_off, pages.cache, table, slot, pos, out, slot.numel(), heads, kv_heads, dim, scale, window, n_split, e,
+        qkv, q_off, pages.cache, table, slot, pos, out, slot.numel(), heads, kv_heads, dim, scale, window, (few, n_split, part_tiles), e,
         *scratch(6, heads, kv_heads, dim, n_split)),
         pages, [1] * 6, heads, kv_heads, dim, torch.bfloat16, window, tensor_cores=True)
 
@@ -306,7 +303,7 @@ def test_decode_attention_with_sharp_and_flat_scores(scale, sharp, few):
     from vlrf_b200.csrc import ops
     pages = Pages([300, 900], 2, 64, seed=4)
     run_tokens(lambda qkv, q_off, table, slot, pos, out, scale, e: ops.attention_decode_packed(
-        qkv, q_off, pages.cache, table, slot, pos, out, 2, 4, 2, 64, scale, 0, 2, e, *scratch(2, 4, 2, 64, 2)),
+        qkv, q_off, pages.cache, table, slot, pos, out, 2, 4, 2, 64, scale, 0, (few, 2, 8), e, *scratch(2, 4, 2, 64, 2)),
         pages, [1, 1], 4, 2, 64, torch.bfloat16, 0, scale=scale, sharp=sharp, tensor_cores=True)
 
 
@@ -320,18 +317,18 @@ def test_decode_attention_skips_padding_reports_missing_blocks_and_repeats_itsel
     outs, room = [], scratch(5, 3, 3, 64, 4)
     for n_split in (1, 4, 4):
         out = torch.full((5, 192), 8.0, device=DEV, dtype=torch.bfloat16)
-        ops.attention_decode_packed(qkv, 0, pages.cache, table, slot, pos, out, 5, 3, 3, 64, 0.125, 0, n_split, e, *room)
+        ops.attention_decode_packed(qkv, 0, pages.cache, table, slot, pos, out, 5, 3, 3, 64, 0.125, 0, (few, n_split, 6), e, *room)
         assert int(room[1].abs().sum()) == 0
         assert bool((out[0] == 8).all()) and bool((out[3] == 8).all()) and int(e.item()) == 0
         outs.append(out)
     assert torch.equal(outs[1], outs[2])
     bad = table.clone()
     bad[2, 7], bad[0, 1] = -1, pages.n_blocks        # a page in the middle that is not mapped, one outside the cache
-    ops.attention_decode_packed(qkv, 0, pages.cache, bad, slot, pos, outs[1], 5, 3, 3, 64, 0.125, 0, 4, e, *room)
+    ops.attention_decode_packed(qkv, 0, pages.cache, bad, slot, pos, outs[1], 5, 3, 3, 64, 0.125, 0, (few, 4, 6), e, *room)
     assert int(e.item()) == 4 and torch.equal(outs[1][4], outs[2][4])
     pos[1] = 100_000
     e.zero_()
-    ops.attention_decode_packed(qkv, 0, pages.cache, table, slot, pos, outs[1], 5, 3, 3, 64, 0.125, 0, 4, e, *room)
+    ops.attention_decode_packed(qkv, 0, pages.cache, table, slot, pos, outs[1], 5, 3, 3, 64, 0.125, 0, (few, 4, 6), e, *room)
     assert int(e.item()) == 4
 
 
@@ -478,7 +475,7 @@ def test_numbers_that_are_not_finite_show_in_their_rows_only(few):
     slot, pos = torch.arange(2, dtype=torch.int32, device=DEV), torch.full((2,), 199, dtype=torch.int32, device=DEV)
     for n_split, window in ((1, 0), (3, 0), (1, 50), (2, 140)):
         out, general = [torch.zeros(2, 128, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
-        ops.attention_decode_packed(qkv, 0, pages.cache, pages.table.to(DEV), slot, pos, out, 2, 2, 2, 64, 0.125, window, n_split, err_word(),
+        ops.attention_decode_packed(qkv, 0, pages.cache, pages.table.to(DEV), slot, pos, out, 2, 2, 2, 64, 0.125, window, (few, n_split, 2), err_word(),
                                     *scratch(2, 2, 2, 64, n_split))
         ops.attention_packed(qkv, 0, pages.cache, pages.table.to(DEV), slot, pos, general, 2, 2, 2, 64, 0.125, window, err_word())
         nan = torch.zeros(2, 128, dtype=torch.bool)

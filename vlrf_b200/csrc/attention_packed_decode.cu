@@ -62,7 +62,7 @@ __device__ __forceinline__ float pd_exp2(float x) {
 constexpr __host__ __device__ int pd_tile_codes(int NG) { return PD_TOKENS * NG * 32; }    // bytes of a tile's keys (or values)
 constexpr __host__ __device__ int pd_tile_pairs(int NG) { return PD_TOKENS * NG * 4; }
 constexpr __host__ __device__ int pd_tile_bytes(int NG) { return 2 * (pd_tile_codes(NG) + pd_tile_pairs(NG)); }
-// FEW: few (row, key/value head) pairs, a CTA an SM with as many warps as shared memory has rings for; else CTAs of four warps, several an SM.
+// FEW: a CTA an SM with as many warps as shared memory has rings for; else CTAs of four warps, several an SM.
 constexpr int PD_STAGES = 2;
 constexpr __host__ __device__ int pd_warps(int NG, bool FEW) { return !FEW ? 4 : NG == 1 ? 24 : NG == 2 ? 12 : NG == 3 ? 8 : 6; }
 constexpr __host__ __device__ int pd_smem(int NG, bool FEW) { return pd_warps(NG, FEW) * PD_STAGES * pd_tile_bytes(NG); }
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(pd_warps(NG, FEW) * 32, pd_ctas(NG, FEW))
 attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_off, const unsigned char* __restrict__ Kq, const unsigned char* __restrict__ Kp,
                           const unsigned char* __restrict__ Vq, const unsigned char* __restrict__ Vp, int n_blocks, const int* __restrict__ block_table,
                           int max_blocks, const int* __restrict__ tok_slot, const int* __restrict__ tok_pos, __nv_bfloat16* __restrict__ out, int ld_out, int R,
-                          int Hkv, int q_tiles, float scale, int window, int n_split, float* __restrict__ partials, int* __restrict__ counters, int* __restrict__ dev_err) {
+                          int Hkv, int q_tiles, float scale, int window, int part_tiles, float* __restrict__ partials, int* __restrict__ counters, int* __restrict__ dev_err) {
     constexpr int DH = NG * 64, WARPS = pd_warps(NG, FEW), ST = PD_STAGES, CODES = pd_tile_codes(NG), PAIRS = pd_tile_pairs(NG), BYTES = pd_tile_bytes(NG);
     constexpr int CP = 8 / RC, NP = 4 / CP;                         // sub-steps side by side; products one after another for a tile's four sub-steps
     extern __shared__ __align__(128) unsigned char pd_raw[];
@@ -99,8 +99,12 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
     if (slot < 0) return;                                           // padding
     const int first = window > 0 ? max(0, pos - window + 1) : 0;
     const int tile0 = first / PD_TOKENS, n_tiles = pos >= 0 ? pos / PD_TOKENS - tile0 + 1 : 0;
-    const int step_tiles = WARPS * n_split, mine0 = part * WARPS + warp;
-    const int n_mine = n_tiles > mine0 ? (n_tiles - mine0 + step_tiles - 1) / step_tiles : 0;
+    // a context takes as many parts as it needs for at most part_tiles tiles each (a longer one than was said: all there are), about equally long
+    const int parts = max(1, min((int)gridDim.z, (n_tiles + part_tiles - 1) / part_tiles));
+    if (part >= parts) return;
+    const int part_first = (int)((long long)part * n_tiles / parts), part_n = (int)((long long)(part + 1) * n_tiles / parts) - part_first;
+    constexpr int step_tiles = WARPS;
+    const int mine0 = part_first + warp, n_mine = (part_n - warp + WARPS - 1) / WARPS;     // (none or less where the part has fewer tiles than warps)
     const int* table = block_table + (size_t)slot * max_blocks;
 
     // tile number i of this warp into stage i % ST; the blocks of 32 tiles at a time lie a lane each
@@ -326,9 +330,9 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
     }
     __syncthreads();
     // the CTA's sums of a query, over its columns of all warps with any token, into the place of warp 0's first
-    const int n_warps = min(WARPS, max(1, n_tiles - part * WARPS)); // (warps behind have none)
+    const int n_warps = min(WARPS, max(1, part_n));                 // (warps behind have none)
     const int place = row * gridDim.x + blockIdx.x;
-    float* my_parts = partials + (size_t)place * n_split * RC * (DH + 4);
+    float* my_parts = partials + (size_t)place * gridDim.z * RC * (DH + 4);
     for (int idx = threadIdx.x; idx < n_q * (DH / 4); idx += WARPS * 32) {
         const int qi = idx / (DH / 4), c4 = idx % (DH / 4);
         float M = -INFINITY;
@@ -346,7 +350,7 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
                 L = fmaf(w_sum[w][c * RC + qi], f, L);
                 acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
             }
-        if (n_split == 1) {
+        if (parts == 1) {
             const float inv = (L > 0.f || L != L) ? 1.f / L : 0.f;
             *reinterpret_cast<uint2*>(out + (size_t)row * ld_out + (size_t)(hk * R + q0 + qi) * DH + c4 * 4) =
                 make_uint2(pd_pack(acc.x * inv, acc.y * inv), pd_pack(acc.z * inv, acc.w * inv));
@@ -356,13 +360,13 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
             if (c4 == 0) *reinterpret_cast<float2*>(mine + DH) = make_float2(M, L);
         }
     }
-    if (n_split == 1) return;
+    if (parts == 1) return;
     // the CTA that finds all parts there merges them, each in its turn, so the sum does not depend on who came last
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();                                            // (of everything that the barrier has shown this thread)
         const int before = atomicAdd(&counters[place], 1);
-        s_last = before == n_split - 1;
+        s_last = before == parts - 1;
         if (s_last) counters[place] = 0;                            // left as it was found
         __threadfence();
     }
@@ -377,7 +381,7 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (qi < n_q) {
 #pragma unroll 8
-            for (int p = share; p < n_split; p += SHARES) {
+            for (int p = share; p < parts; p += SHARES) {
                 const float* theirs = my_parts + (size_t)(p * RC + qi) * (DH + 4);
                 const float2 ml = __ldcg(reinterpret_cast<const float2*>(theirs + DH));
                 const float4 v = __ldcg(reinterpret_cast<const float4*>(theirs + c4 * 4));
@@ -414,7 +418,7 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
 
 template <int NG, int RC, bool FEW>
 int pd_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
-              int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows, int H, int Hkv, float scale, int window, int n_split,
+              int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows, int H, int Hkv, float scale, int window, int n_split, int part_tiles,
               float* partials, int* counters, int* dev_err, cudaStream_t stream) {
     const int R = H / Hkv, q_tiles = (R + RC - 1) / RC;
     constexpr size_t smem = pd_smem(NG, FEW);
@@ -426,17 +430,13 @@ int pd_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_decode: %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     e = launch_chained(kern, dim3(Hkv * q_tiles, rows, n_split), dim3(pd_warps(NG, FEW) * 32), smem, stream, (const __nv_bfloat16*)qkv, ld, q_off,
                        (const unsigned char*)Kq, (const unsigned char*)Kp, (const unsigned char*)Vq, (const unsigned char*)Vp, n_blocks, block_table, max_blocks,
-                       tok_slot, tok_pos, (__nv_bfloat16*)out, ld_out, R, Hkv, q_tiles, scale, window, n_split, partials, counters, dev_err);
+                       tok_slot, tok_pos, (__nv_bfloat16*)out, ld_out, R, Hkv, q_tiles, scale, window, part_tiles, partials, counters, dev_err);
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_decode: %s", cudaGetErrorString(e));
     return vlrf_check_launch("attn_packed_decode");
 }
 
 constexpr int pd_columns(int dh, int R) { return dh > 128 || R > 4 ? 8 : R > 2 ? 4 : 2; }
-thread_local int g_few = -1;
 }  // namespace
-
-// For measurements and tests: the calling thread's next launches with a CTA an SM (1), with several (0), or as their sizes say (−1).
-extern "C" int vlrf_attn_packed_decode_force(int few) { g_few = few; return VLRF_OK; }
 
 extern "C" int vlrf_attn_packed_decode_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out) {
     return H > 0 && Hkv > 0 && H % Hkv == 0 && dh > 0 && dh % 64 == 0 && dh <= 256 && BT == PD_TOKENS && ld % 8 == 0 && q_off % 8 == 0 && ld_out % 8 == 0;
@@ -454,21 +454,20 @@ extern "C" int vlrf_attn_packed_decode_scratch(int rows, int H, int Hkv, int dh,
 
 extern "C" int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                                        const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows,
-                                       int H, int Hkv, int dh, int BT, float scale, int window, int n_split, float* partials, int* counters, int* dev_err,
-                                       cudaStream_t stream) {
+                                       int H, int Hkv, int dh, int BT, float scale, int window, int few, int n_split, int part_tiles, float* partials,
+                                       int* counters, int* dev_err, cudaStream_t stream) {
     VLRF_REQUIRE(vlrf_attn_packed_decode_takes(H, Hkv, dh, BT, ld, q_off, ld_out),
                  "attn_packed_decode: %d heads over %d of %d, blocks of %d, row strides %d and %d are not taken", H, Hkv, dh, BT, ld, ld_out);
     VLRF_REQUIRE(rows >= 0 && rows <= 65535 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && dev_err != nullptr, "attn_packed_decode: bad arguments");
-    VLRF_REQUIRE(n_split >= 1 && n_split <= PD_MAX_SPLIT && (n_split == 1 || (partials != nullptr && counters != nullptr)),
+    VLRF_REQUIRE(n_split >= 1 && n_split <= PD_MAX_SPLIT && part_tiles >= 1 && (n_split == 1 || (partials != nullptr && counters != nullptr)),
                  "attn_packed_decode: %d parts (1 to %d; more than one wants scratch)", n_split, PD_MAX_SPLIT);
     for (const void* p : {qkv, Kq, Kp, Vq, Vp, (const void*)out, (const void*)partials})
         VLRF_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "attn_packed_decode: tensors begin on 16 bytes");
     if (rows == 0) return VLRF_OK;
     const int R = H / Hkv, RC = pd_columns(dh, R);
-    const bool few = g_few >= 0 ? g_few != 0 : (long long)rows * Hkv * ((R + RC - 1) / RC) * n_split <= vlrf_sm_count();
 #define GO(NG, C) (few ? pd_launch<NG, C, true>(ARGS) : pd_launch<NG, C, false>(ARGS))
-#define ARGS qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, tok_slot, tok_pos, out, ld_out, rows, H, Hkv, scale, window, n_split, partials, \
-             counters, dev_err, stream
+#define ARGS qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, tok_slot, tok_pos, out, ld_out, rows, H, Hkv, scale, window, n_split, part_tiles, \
+             partials, counters, dev_err, stream
     if (dh == 64) return RC == 2 ? GO(1, 2) : RC == 4 ? GO(1, 4) : GO(1, 8);
     if (dh == 128) return RC == 2 ? GO(2, 2) : RC == 4 ? GO(2, 4) : GO(2, 8);
     return dh == 192 ? GO(3, 8) : GO(4, 8);

@@ -170,8 +170,8 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tsm(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const int my_first = kb_first + part * n_kb / tile_parts;
-    const int my_n = kb_first + (part + 1) * n_kb / tile_parts - my_first, my_end = my_first + my_n;
+    const int my_first = kb_first + (int)((long long)part * n_kb / tile_parts);
+    const int my_n = kb_first + (int)((long long)(part + 1) * n_kb / tile_parts) - my_first, my_end = my_first + my_n;
     // the blocks of group g: lo … hi − 1 (a group without rows: none)
     int lo[GROUPS], hi[GROUPS];
 #pragma unroll

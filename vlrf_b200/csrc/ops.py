@@ -1118,14 +1118,39 @@ def packed_prefill_scratch(n_seqs: int, max_new: int, n_heads: int, head_dim: in
     return floats.value, ints.value
 
 
-def packed_decode_splits(n_rows: int, n_heads: int, n_kv_heads: int, max_context: int, window: int = 0) -> int:
-    """Into how many parts a decode step over a cache of 4 bits cuts each context."""
-    forced = os.environ.get("VLRF_B200_DECODE_SPLITS")
-    if forced:
-        return max(1, min(16, int(forced)))
+#: What `attention_decode_packed` takes, in microseconds, measured: a launch, meeting other parts in scratch, and a round of its warps (a tile of 64 tokens
+#: each): the latency of one, or the time a tile takes of an SM's quarter times the warps there, by head size up to 64, 128 and above.
+PACKED_DECODE_US = dict(launch=3.5, wave=1.5, meet=4.0, tile={64: (1.0, 0.42), 128: (1.3, 0.8), 256: (2.0, 1.5)})
+#: … and its CTAs: (warps, CTAs an SM) of several an SM, and of one
+PACKED_DECODE_CTAS = {64: ((4, 6), (24, 1)), 128: ((4, 3), (12, 1)), 256: ((4, 2), (6, 1))}
+
+
+@functools.lru_cache(maxsize=1024)                # (a rule of sizes alone)
+def packed_decode_shape(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, window: int = 0) -> tuple:
+    """(whether a CTA has an SM to itself, into how many parts the longest context is cut, blocks of 64 tokens a part at most) for a decode step over a
+    cache of 4 bits: the shape that the measured costs of its rounds say is fastest, with contexts of a step taken as two thirds of the longest."""
     reach = min(max_context, window + 63) if window > 0 else max_context
-    pairs = max(1, n_rows * n_kv_heads * (-(-(n_heads // n_kv_heads) // 8)))
-    return max(1, min(64, sm_count() // pairs, -(-reach // 768)))
+    tiles = -(-max(1, reach) // 64)
+    size = 64 if head_dim == 64 else 128 if head_dim == 128 else 256
+    pairs = max(1, n_rows * n_kv_heads * -(-(n_heads // n_kv_heads) // 8))
+    sms, cost = sm_count(), PACKED_DECODE_US
+    forced = os.environ.get("VLRF_B200_DECODE_SPLITS")
+    best = None
+    for few in (0, 1):
+        warps, at_once = PACKED_DECODE_CTAS[size][few]
+        for parts in ((max(1, min(64, int(forced))),) if forced else (1, 2, 3, 4, 6, 8, 12, 18, 24, 37, 64)):
+            each = -(-tiles // parts)
+            if parts > 1 and (each < 2 or pairs * parts > 8 * sms * at_once):
+                break
+            ctas = pairs * (parts if pairs == 1 else max(1.0, 0.67 * parts))
+            waves = -(-ctas // (sms * at_once))
+            side = min(at_once, -(-ctas // sms))
+            low, high = cost["tile"][size]
+            rounds = -(-each // warps)
+            time = cost["launch"] + waves * (rounds * max(low, high * min(warps, each) * side / 4.0) + cost["wave"]) + (cost["meet"] if parts > 1 else 0.0)
+            if best is None or time < 0.97 * best[0]:
+                best = (time, few, parts, each)
+    return best[1:]
 
 
 def packed_decode_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, n_split: int) -> tuple:
@@ -1147,20 +1172,22 @@ def _packed_scratch(what: str, want: tuple, partials, counters) -> tuple:
 
 
 def attention_decode_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, out, n_rows: int, n_heads: int, n_kv_heads: int,
-                            head_dim: int, scale: float, window: int, n_split: int, dev_err, partials=None, counters=None) -> None:
-    """One bfloat16 query per row and head attends the keys 0…position of its slot in a cache of 4 bits, on the tensor cores; the context is
-    cut into n_split parts, which for more than one meet in float32 `partials` and zeroed int32 `counters` (see packed_decode_scratch; the
-    counters are left zero).  Rows with slot −1 are left as they are."""
+                            head_dim: int, scale: float, window: int, shape: tuple, dev_err, partials=None, counters=None) -> None:
+    """One bfloat16 query per row and head attends the keys 0…position of its slot in a cache of 4 bits, on the tensor cores.  shape = (a CTA an SM
+    or not, n_split, blocks a part), see packed_decode_shape: a context takes as many parts as it needs for so many blocks each, at most (and in
+    fact, where a context is longer than they hold) n_split; with n_split > 1 they meet in float32 `partials` and zeroed int32 `counters` (see packed_decode_scratch; the counters are left
+    zero).  Rows with slot −1 are left as they are."""
     what = "attention_decode_packed"
     _attention_packed_check(what, qkv, q_off, cache, block_table, (tok_slot, tok_pos), out, n_rows, n_heads, n_kv_heads, head_dim, window, dev_err)
     if qkv.dtype != torch.bfloat16 or tok_slot.shape[0] < n_rows or tok_pos.shape[0] < n_rows:
         raise KernelError(f"{what}: bfloat16 rows, each with a slot and a position")
+    few, n_split, part_tiles = shape
     scratch = (0, 0)
     if n_split > 1:
         scratch = _packed_scratch(what, packed_decode_scratch(n_rows, n_heads, n_kv_heads, head_dim, n_split), partials, counters)
     call("vlrf_attn_packed_decode", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], tok_slot.data_ptr(),
-         tok_pos.data_ptr(), out.data_ptr(), out.stride(0), n_rows, n_heads, n_kv_heads, head_dim, cache.block_tokens, float(scale), window, n_split,
-         *scratch, dev_err.data_ptr(), _stream())
+         tok_pos.data_ptr(), out.data_ptr(), out.stride(0), n_rows, n_heads, n_kv_heads, head_dim, cache.block_tokens, float(scale), window,
+         1 if few else 0, n_split, part_tiles, *scratch, dev_err.data_ptr(), _stream())
 
 
 def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ctx, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -1168,14 +1195,14 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
     """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
     already holds the step's own keys and values."""
     if ctx.max_new == 1 and _packed_decode_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
-        n_split = packed_decode_splits(ctx.n_tokens, n_heads, n_kv_heads, ctx.max_context, window)
+        shape = packed_decode_shape(ctx.n_tokens, n_heads, n_kv_heads, head_dim, ctx.max_context, window)
         partials = counters = None
-        if n_split > 1:
-            n_floats, n_counters = packed_decode_scratch(ctx.n_tokens, n_heads, n_kv_heads, head_dim, n_split)
+        if shape[1] > 1:
+            n_floats, n_counters = packed_decode_scratch(ctx.n_tokens, n_heads, n_kv_heads, head_dim, shape[1])
             partials = ctx.ws.get("packed_partials", n_floats, 1, torch.float32)
             counters = ctx.ws.get_zeroed("packed_counters", n_counters, torch.int32)
         attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
-                                window, n_split, ctx.dev_err, partials, counters)
+                                window, shape, ctx.dev_err, partials, counters)
         return
     if ctx.max_new > 1 and scale >= 0.0 and _packed_prefill_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
         groups, n_parts, part_blocks = packed_prefill_shape(ctx.host_seq_lens, ctx.host_seq_pos0, n_heads, head_dim, window)

@@ -468,16 +468,16 @@ int vlrf_packed_read(const void* Kq, const void* Kp, const void* Vq, const void*
 int vlrf_attn_packed(const void* qkv, int dtype, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp,
                      int n_blocks, const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out,
                      int T, int H, int Hkv, int dh, int BT, float scale, int window, int* dev_err, cudaStream_t stream);
-// A decode step of it on the tensor cores, bfloat16, head sizes 64, 128, 192 and 256, blocks of 64: one query a row (slot −1: skipped), every
-// context in n_split (up to 64) parts, which for more than one meet in scratch: float32 partials and int32 counters, zero before the first
-// call (every call leaves them zero), of the sizes that vlrf_attn_packed_decode_scratch gives (host pointers).
+// A decode step of it on the tensor cores, bfloat16, head sizes 64, 128, 192 and 256, blocks of 64: one query a row (slot −1: skipped).  A context takes
+// as many parts as it needs for at most part_tiles blocks each, up to n_split (of 64 at most), and longer ones where those do not hold it; contexts
+// of more than one meet in scratch: float32 partials and int32 counters, zero before the first call (every call leaves them zero), of the sizes that
+// vlrf_attn_packed_decode_scratch gives (host pointers).  few: a CTA an SM with many warps (1), or several of four (0).
 int vlrf_attn_packed_decode_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out);
 int vlrf_attn_packed_decode_scratch(int rows, int H, int Hkv, int dh, int n_split, long long* floats, long long* ints);
 int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                             const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows,
-                            int H, int Hkv, int dh, int BT, float scale, int window, int n_split, float* partials, int* counters, int* dev_err,
-                            cudaStream_t stream);
-int vlrf_attn_packed_decode_force(int few);    // for measurements and tests: a CTA an SM (1), several (0), chosen by size again (−1)
+                            int H, int Hkv, int dh, int BT, float scale, int window, int few, int n_split, int part_tiles, float* partials,
+                            int* counters, int* dev_err, cudaStream_t stream);
 // A prompt step of it on the tcgen05 tensor cores, bfloat16, head sizes 64 and 128, blocks of 64: sequences as in vlrf_attn_prefill (slot −1:
 // skipped).  A CTA takes `groups` (1 or 2) times 128 queries of a head; n_parts > 1 deals the keys of long tiles, part_blocks blocks of 64 to each or
 // more, to that many CTAs (up to vlrf_attn_packed_prefill_max_parts()), which meet in scratch: float32 partials and int32 counters, zero before the first call (every
