@@ -148,3 +148,40 @@ def test_models_say_whether_they_take_4_bits():
         with pytest.raises(ValueError, match="4 bits"):
             model.check_packed_kv()
     assert CausalSelfAttention.takes_packed_kv
+
+
+def test_scratch_sizes_are_the_library_s():
+    from vlrf_b200.csrc import library, ops
+    lib = library()
+    floats, ints = ctypes.c_longlong(0), ctypes.c_longlong(0)
+    for rows, heads, kv_heads, dim, parts in ((1, 12, 12, 64, 1), (7, 25, 25, 64, 3), (2, 32, 8, 128, 64), (3, 28, 4, 128, 5), (1, 80, 2, 256, 2), (4, 6, 3, 192, 9), (5, 24, 1, 64, 2)):
+        assert lib.vlrf_attn_packed_decode_scratch(rows, heads, kv_heads, dim, parts, ctypes.byref(floats), ctypes.byref(ints)) == 0
+        assert ops.packed_decode_scratch(rows, heads, kv_heads, dim, parts) == (floats.value, ints.value)
+    for seqs, new, heads, dim, groups, parts in ((1, 1, 12, 64, 1, 1), (3, 300, 25, 64, 2, 4), (2, 128, 8, 128, 1, 16), (1, 257, 4, 128, 2, 2)):
+        assert lib.vlrf_attn_packed_prefill_scratch(seqs, new, heads, dim, groups, parts, ctypes.byref(floats), ctypes.byref(ints)) == 0
+        assert ops.packed_prefill_scratch(seqs, new, heads, dim, groups, parts) == (floats.value, ints.value)
+    assert lib.vlrf_attn_packed_decode_scratch(1, 3, 2, 64, 1, ctypes.byref(floats), ctypes.byref(ints)) != 0
+    assert lib.vlrf_attn_packed_prefill_scratch(1, 3, 2, 96, 1, 1, ctypes.byref(floats), ctypes.byref(ints)) != 0
+
+
+def test_shapes_of_steps(monkeypatch):
+    """Shapes hold the longest context, are within what the kernels take, and are the measured best (or within a tenth of it) where several were
+    measured on 148 SMs."""
+    from vlrf_b200.csrc import ops
+    monkeypatch.setattr(ops, "_SM_COUNT", 148)
+    ops._packed_decode_shape.cache_clear(); ops._packed_prefill_shape.cache_clear()
+    for rows in (1, 2, 7, 32, 200, 5000):
+        for heads, kv_heads in ((12, 12), (32, 8), (7, 1), (48, 1)):
+            for dim in (64, 128, 192, 256):
+                for context in (0, 1, 64, 65, 1000, 8192, 200_000):
+                    few, parts, each = ops.packed_decode_shape(rows, heads, kv_heads, dim, context)
+                    assert few in (0, 1) and 1 <= parts <= 64 and each >= 1 and parts * each * 64 >= context
+    assert ops.packed_decode_shape(1, 12, 12, 64, 701)[1] == 1                        # one row of 700 tokens: not cut
+    assert ops.packed_decode_shape(32, 25, 25, 64, 1014)[:2] == (0, 1)                # the places are full
+    assert ops.packed_decode_shape(1, 32, 8, 128, 131_071)[1] >= 18                   # one long row: cut to fill the GPU
+    assert ops.packed_prefill_shape([512], [7500], 32, 128)[:2] == (2, 2)
+    assert ops.packed_prefill_shape([200], [0], 12, 64) == (1, 1, 4)
+    for lens, pos0, window in (([1], [0], 0), ([1, 5000], [100_000, 0], 0), ([300], [90_000], 100), ([2] * 40, list(range(40)), 1)):
+        groups, parts, each = ops.packed_prefill_shape(lens, pos0, 8, 128, window)
+        assert groups in (1, 2) and 1 <= parts <= 16 and each >= 1
+    ops._packed_decode_shape.cache_clear(); ops._packed_prefill_shape.cache_clear()

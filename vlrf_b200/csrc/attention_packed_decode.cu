@@ -39,8 +39,9 @@ __device__ __forceinline__ void pd_copy(void* dst, const void* src, uint32_t byt
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(pd_sm(dst)), "l"(src), "r"(bytes), "r"(pd_sm(bar)) : "memory");
 }
+// (not volatile: products of different sums change places, so that one does not wait for the other)
 __device__ __forceinline__ void pd_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -94,7 +95,11 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
     }
     __syncwarp();
     pdl_wait();
-    pdl_launch_dependents();
+    // (A large grid lets the next kernel's CTAs in when its own are done with their tiles: taken in beside them they sit on the places that are free then,
+    // three on one SM and one on another, and so they run when their turn comes.  256 CTAs of 1,983 tokens of 128, the same kernel again and again:
+    // 27.5 us, now PD_LATE.)
+    const bool small = gridDim.x * gridDim.y * gridDim.z <= 64u;
+    if (small) pdl_launch_dependents();
     const int slot = tok_slot[row], pos = tok_pos[row];
     if (slot < 0) return;                                           // padding
     const int first = window > 0 ? max(0, pos - window + 1) : 0;
@@ -199,29 +204,31 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
             float s[NP][4];
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
+                float acc[NG][CP][4];
 #pragma unroll
-                for (int a = 0; a < NG; ++a) {
-                    float acc[CP][4];
+                for (int a = 0; a < NG; ++a)
 #pragma unroll
                     for (int c = 0; c < CP; ++c) {
                         const int r0 = (n * CP + c) * 16 + g;       // tokens r0 and r0 + 8
                         const uint2 w0 = *reinterpret_cast<const uint2*>(kc + r0 * (NG * 32) + a * 32 + t * 8);
                         const uint2 w1 = *reinterpret_cast<const uint2*>(kc + (r0 + 8) * (NG * 32) + a * 32 + t * 8);
-                        acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
+                        acc[a][c][0] = acc[a][c][1] = acc[a][c][2] = acc[a][c][3] = 0.f;
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {
                             const uint32_t x0 = w ? w0.y : w0.x, x1 = w ? w1.y : w1.x, y0 = x0 >> 8, y1 = x1 >> 8;
-                            pd_mma(acc[c], x0 & PK_LOW, x1 & PK_LOW, x0 & PK_HIGH, x1 & PK_HIGH, qf[a][2 * w][0], qf[a][2 * w][1]);
-                            pd_mma(acc[c], y0 & PK_LOW, y1 & PK_LOW, y0 & PK_HIGH, y1 & PK_HIGH, qf[a][2 * w + 1][0], qf[a][2 * w + 1][1]);
+                            pd_mma(acc[a][c], x0 & PK_LOW, x1 & PK_LOW, x0 & PK_HIGH, x1 & PK_HIGH, qf[a][2 * w][0], qf[a][2 * w][1]);
+                            pd_mma(acc[a][c], y0 & PK_LOW, y1 & PK_LOW, y0 & PK_HIGH, y1 & PK_HIGH, qf[a][2 * w + 1][0], qf[a][2 * w + 1][1]);
                         }
                     }
+#pragma unroll
+                for (int a = 0; a < NG; ++a) {
                     // every column of a sub-step's result holds its query's score; this lane's columns take those of their own sub-step
                     float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        x[e] = acc[0][e];
+                        x[e] = acc[a][0][e];
 #pragma unroll
-                        for (int c = 1; c < CP; ++c) x[e] = my_sub == c ? acc[c][e] : x[e];
+                        for (int c = 1; c < CP; ++c) x[e] = my_sub == c ? acc[a][c][e] : x[e];
                     }
                     const int r0 = (n * CP + my_sub) * 16 + g;
                     const uint32_t p0 = kp[r0 * NG + a], p1 = kp[(r0 + 8) * NG + a];
@@ -302,6 +309,7 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
         if (lane == 0) atomicOr(dev_err, VLRF_DEVERR_WAIT_TIMEOUT);
         for (int j = done; j < min(n_mine, done + ST); ++j) pd_wait(&full[j % ST], (uint32_t)((j / ST) & 1));
     }
+    if (!small) pdl_launch_dependents();
     __syncthreads();                                                // every warp is done with its ring: the sums go there
     // the warp's sums: [warp][column][DH] float32 (8 columns of DH numbers are less than a warp's ring)
     float* all = reinterpret_cast<float*>(pd_raw);

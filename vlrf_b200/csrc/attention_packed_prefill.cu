@@ -154,7 +154,6 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    pdl_launch_dependents();
     const int row0 = seq_start[seq], n_new = seq_start[seq + 1] - row0, slot = seq_slot[seq], pos0 = seq_pos0[seq];
     const int hk = h / (H / Hkv);
     const int t_first = qt * ROWS, q_first = pos0 + t_first;        // the tile's first query, in the step and in the sequence
@@ -607,6 +606,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             }
         }
     }
+    pdl_launch_dependents();                                        // (CTAs of the next kernel taken in earlier would sit on the places that are free then)
     // everyone meets here on every path; then the allocating warp gives the tensor memory back
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import dataclasses
 import functools
+import math
 import os
 
 import torch
@@ -29,6 +30,7 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # (the short way: without asking whether CUDA has begun)
 
 
 def _stream() -> int:
@@ -948,12 +950,12 @@ def _packed_check(what: str, cache: PackedKV, n_kv_heads: int, head_dim: int, bl
     if not isinstance(cache, PackedKV):
         raise KernelError(f"{what}: the cache is a PackedKV, not {type(cache).__name__}")
     at = cache.index
-    if at < 0 or at != torch.cuda.current_device():
+    if at < 0 or at != _current_device():
         raise KernelError(f"{what}: the cache must live on the current CUDA device (there is no CPU path)")
     if cache.n_kv_heads != n_kv_heads or cache.head_dim != head_dim:
         raise KernelError(f"{what}: cache shape does not match the heads")
     for t in (block_table, dev_err, *tables):
-        if t.dtype != torch.int32 or t.get_device() != at or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.get_device() != at or not t.is_contiguous():
             raise KernelError(f"{what}: block table, slots, positions and error word are contiguous int32 tensors on the cache's device")
     if block_table.dim() != 2 or block_table.shape[1] == 0:
         raise KernelError(f"{what}: the block table is [slots, blocks]")
@@ -1027,20 +1029,11 @@ def attention_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, to
 PACKED_ATTENTION_MMA = True
 
 
-def _packed_decode_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
-    if not isinstance(cache, PackedKV) or qkv.dtype != torch.bfloat16 or not PACKED_ATTENTION_MMA or qkv.data_ptr() % 16 != 0 \
-            or out.data_ptr() % 16 != 0:
-        return False
-    from . import library
-    return bool(library().vlrf_attn_packed_decode_takes(n_heads, n_kv_heads, head_dim, cache.block_tokens, qkv.stride(0), q_off, out.stride(0)))
-
-
-def _packed_prefill_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
-    if not isinstance(cache, PackedKV) or qkv.dtype != torch.bfloat16 or not PACKED_ATTENTION_MMA or qkv.data_ptr() % 16 != 0 \
-            or out.data_ptr() % 16 != 0:
-        return False
-    from . import library
-    return bool(library().vlrf_attn_packed_prefill_takes(n_heads, n_kv_heads, head_dim, cache.block_tokens, qkv.stride(0), q_off, out.stride(0)))
+def _packed_mma_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
+    """Whether the tensor-core kernels take these tensors (head sizes are theirs): what the library's vlrf_attn_packed_decode_takes and
+    vlrf_attn_packed_prefill_takes ask, and tensors on 16 bytes."""
+    return PACKED_ATTENTION_MMA and isinstance(cache, PackedKV) and qkv.dtype == torch.bfloat16 and cache.block_tokens == 64 \
+        and (qkv.data_ptr() | out.data_ptr()) % 16 == 0 and (qkv.stride(0) | q_off | out.stride(0)) % 8 == 0
 
 
 #: Microseconds of a CTA of `attention_prefill_packed`, measured: its start, queries and result (with one and with two groups of queries), a block of 64 keys
@@ -1109,58 +1102,59 @@ def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_
 
 
 def packed_prefill_scratch(n_seqs: int, max_new: int, n_heads: int, head_dim: int, groups: int, n_parts: int) -> tuple:
-    """(float32 elements of `partials`, int32 elements of `counters`) that `attention_prefill_packed` wants for n_parts > 1."""
-    import ctypes
-
-    from . import call_host
-    floats, ints = ctypes.c_longlong(0), ctypes.c_longlong(0)
-    call_host("vlrf_attn_packed_prefill_scratch", n_seqs, max_new, n_heads, head_dim, groups, n_parts, ctypes.byref(floats), ctypes.byref(ints))
-    return floats.value, ints.value
+    """(float32 elements of `partials`, int32 elements of `counters`) that `attention_prefill_packed` wants for n_parts > 1: the library's
+    vlrf_attn_packed_prefill_scratch, without asking it."""
+    if n_parts <= 1:
+        return 0, 0
+    tiles = -(-max_new // (128 * groups)) * groups * n_seqs * n_heads
+    return tiles * n_parts * (128 * head_dim + 256), tiles
 
 
 #: What `attention_decode_packed` takes, in microseconds, measured: a launch, meeting other parts in scratch, and a round of its warps (a tile of 64 tokens
-#: each): the latency of one, or the time a tile takes of an SM's quarter times the warps there, by head size up to 64, 128 and above.
-PACKED_DECODE_US = dict(launch=3.5, wave=1.5, meet=4.0, tile={64: (1.0, 0.42), 128: (1.3, 0.8), 256: (2.0, 1.5)})
+#: each): the latency of one, or the time a tile takes of an SM's quarter times the warps there, by head size up to 64, 128 and above; bytes of cache a us.
+PACKED_DECODE_US = dict(launch=3.5, wave=1.5, meet=4.0, tile={64: (0.9, 0.4), 128: (1.0, 0.72), 256: (2.0, 1.5)}, bytes=5.5e6)
 #: … and its CTAs: (warps, CTAs an SM) of several an SM, and of one
 PACKED_DECODE_CTAS = {64: ((4, 6), (24, 1)), 128: ((4, 3), (12, 1)), 256: ((4, 2), (6, 1))}
 
 
-@functools.lru_cache(maxsize=1024)                # (a rule of sizes alone)
-def packed_decode_shape(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, window: int = 0) -> tuple:
+def packed_decode_shape(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, max_context: int, window: int = 0, fill: float = 0.67) -> tuple:
     """(whether a CTA has an SM to itself, into how many parts the longest context is cut, blocks of 64 tokens a part at most) for a decode step over a
-    cache of 4 bits: the shape that the measured costs of its rounds say is fastest, with contexts of a step taken as two thirds of the longest."""
+    cache of 4 bits: the shape that the measured costs of its rounds say is fastest.  fill: the rows' contexts, in all, of that many of the longest."""
     reach = min(max_context, window + 63) if window > 0 else max_context
-    tiles = -(-max(1, reach) // 64)
+    return _packed_decode_shape(n_rows * n_kv_heads * -(-(n_heads // n_kv_heads) // 8), n_rows, head_dim, -(-max(1, reach) // 64),
+                                1.0 if window > 0 or n_rows == 1 else round(8 * fill) / 8.0, os.environ.get("VLRF_B200_DECODE_SPLITS"))
+
+
+@functools.lru_cache(maxsize=1024)                # (a rule of sizes alone)
+def _packed_decode_shape(pairs: int, n_rows: int, head_dim: int, tiles: int, fill: float, forced) -> tuple:
     size = 64 if head_dim == 64 else 128 if head_dim == 128 else 256
-    pairs = max(1, n_rows * n_kv_heads * -(-(n_heads // n_kv_heads) // 8))
-    sms, cost = sm_count(), PACKED_DECODE_US
-    forced = os.environ.get("VLRF_B200_DECODE_SPLITS")
-    best = None
+    sms, cost, best = sm_count(), PACKED_DECODE_US, None
+    low, high = cost["tile"][size]
     for few in (0, 1):
         warps, at_once = PACKED_DECODE_CTAS[size][few]
         for parts in ((max(1, min(64, int(forced))),) if forced else (1, 2, 3, 4, 6, 8, 12, 18, 24, 37, 64)):
             each = -(-tiles // parts)
             if parts > 1 and (each < 2 or pairs * parts > 8 * sms * at_once):
                 break
-            ctas = pairs * (parts if pairs == 1 else max(1.0, 0.67 * parts))
-            waves = -(-ctas // (sms * at_once))
-            side = min(at_once, -(-ctas // sms))
-            low, high = cost["tile"][size]
-            rounds = -(-each // warps)
-            time = cost["launch"] + waves * (rounds * max(low, high * min(warps, each) * side / 4.0) + cost["wave"]) + (cost["meet"] if parts > 1 else 0.0)
+            ctas = pairs * (min(parts, parts * fill + (0.5 if n_rows > 1 else 0.0)) if parts > 1 else 1)
+            waves, side = max(1, math.ceil(ctas / (sms * at_once) - 0.1)), min(at_once, -(-ctas // sms))
+            rounds = waves * -(-each // warps) * max(low, high * min(warps, each) * side / 4.0) + waves * cost["wave"]
+            bytes_us = pairs * tiles * fill * 64 * 1.125 * head_dim / cost["bytes"]
+            time = cost["launch"] + max(rounds, bytes_us) + (cost["meet"] if parts > 1 else 0.0)
             if best is None or time < 0.97 * best[0]:
                 best = (time, few, parts, each)
     return best[1:]
 
 
 def packed_decode_scratch(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, n_split: int) -> tuple:
-    """(float32 elements of `partials`, int32 elements of `counters`) that `attention_decode_packed` wants for n_split > 1."""
-    import ctypes
-
-    from . import call_host
-    floats, ints = ctypes.c_longlong(0), ctypes.c_longlong(0)
-    call_host("vlrf_attn_packed_decode_scratch", n_rows, n_heads, n_kv_heads, head_dim, n_split, ctypes.byref(floats), ctypes.byref(ints))
-    return floats.value, ints.value
+    """(float32 elements of `partials`, int32 elements of `counters`) that `attention_decode_packed` wants for n_split > 1: the library's
+    vlrf_attn_packed_decode_scratch, without asking it."""
+    if n_split <= 1:
+        return 0, 0
+    share = n_heads // n_kv_heads
+    columns = 8 if head_dim > 128 or share > 4 else 4 if share > 2 else 2
+    places = n_rows * n_kv_heads * -(-share // columns)
+    return places * n_split * columns * (head_dim + 4), places
 
 
 def _packed_scratch(what: str, want: tuple, partials, counters) -> tuple:
@@ -1194,19 +1188,21 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
                           scale: float, window: int = 0) -> None:
     """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
     already holds the step's own keys and values."""
-    if ctx.max_new == 1 and _packed_decode_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
-        shape = packed_decode_shape(ctx.n_tokens, n_heads, n_kv_heads, head_dim, ctx.max_context, window)
-        partials = counters = None
+    mma = _packed_mma_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim)
+    partials = counters = None
+    if mma and ctx.max_new == 1 and head_dim % 64 == 0:
+        rows, past = ctx.n_tokens, ctx.host_seq_pos0
+        shape = packed_decode_shape(rows, n_heads, n_kv_heads, head_dim, ctx.max_context, window,
+                                    (sum(past) + rows) / (rows * ctx.max_context) if len(past) == rows else 0.67)
         if shape[1] > 1:
-            n_floats, n_counters = packed_decode_scratch(ctx.n_tokens, n_heads, n_kv_heads, head_dim, shape[1])
+            n_floats, n_counters = packed_decode_scratch(rows, n_heads, n_kv_heads, head_dim, shape[1])
             partials = ctx.ws.get("packed_partials", n_floats, 1, torch.float32)
             counters = ctx.ws.get_zeroed("packed_counters", n_counters, torch.int32)
-        attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
+        attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, rows, n_heads, n_kv_heads, head_dim, scale,
                                 window, shape, ctx.dev_err, partials, counters)
         return
-    if ctx.max_new > 1 and scale >= 0.0 and _packed_prefill_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim):
+    if mma and ctx.max_new > 1 and scale >= 0.0 and head_dim in (64, 128):
         groups, n_parts, part_blocks = packed_prefill_shape(ctx.host_seq_lens, ctx.host_seq_pos0, n_heads, head_dim, window)
-        partials = counters = None
         if n_parts > 1:
             n_floats, n_counters = packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts)
             partials = ctx.ws.get("packed_partials", n_floats, 1, torch.float32)
