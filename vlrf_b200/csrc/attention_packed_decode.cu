@@ -97,7 +97,7 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
     pdl_wait();
     // (A large grid lets the next kernel's CTAs in when its own are done with their tiles: taken in beside them they sit on the places that are free then,
     // three on one SM and one on another, and so they run when their turn comes.  256 CTAs of 1,983 tokens of 128, the same kernel again and again:
-    // 27.5 us, now PD_LATE.)
+    // 27.5 us, now 24.2.)
     const bool small = gridDim.x * gridDim.y * gridDim.z <= 64u;
     if (small) pdl_launch_dependents();
     const int slot = tok_slot[row], pos = tok_pos[row];

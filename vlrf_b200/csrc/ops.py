@@ -1190,7 +1190,7 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
     already holds the step's own keys and values."""
     mma = _packed_mma_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim)
     partials = counters = None
-    if mma and ctx.max_new == 1 and head_dim % 64 == 0:
+    if mma and ctx.max_new == 1 and head_dim % 64 == 0 and ctx.n_tokens <= 65535:
         rows, past = ctx.n_tokens, ctx.host_seq_pos0
         shape = packed_decode_shape(rows, n_heads, n_kv_heads, head_dim, ctx.max_context, window,
                                     (sum(past) + rows) / (rows * ctx.max_context) if len(past) == rows else 0.67)
@@ -1201,7 +1201,7 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
         attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, rows, n_heads, n_kv_heads, head_dim, scale,
                                 window, shape, ctx.dev_err, partials, counters)
         return
-    if mma and ctx.max_new > 1 and scale >= 0.0 and head_dim in (64, 128):
+    if mma and ctx.max_new > 1 and scale >= 0.0 and head_dim in (64, 128) and ctx.n_seqs <= 65535:
         groups, n_parts, part_blocks = packed_prefill_shape(ctx.host_seq_lens, ctx.host_seq_pos0, n_heads, head_dim, window)
         if n_parts > 1:
             n_floats, n_counters = packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts)

@@ -2,8 +2,8 @@
 //
 // Append: a thread takes 8 neighbouring entries of a token's keys and the same 8 of its values; the G / 8 threads of a group find its least
 // and largest number by shuffles (that a number is NaN goes along).  A quotient rounds by the addition of 1.5 · 2^23, whose sum's low bits are the
-// code; where one lies within 10^-4 of the border half way between two codes, the thread does its eight again by exact remainders, so the codes are
-// those of the exact quotients, and another implementation in more bits agrees with them one by one.  Read: four pieces a thread, their loads
+// code; where one lies within 10^-5 of the border half way between two codes, and is no tie, the thread does its eight again by exact remainders, so the
+// codes are those of the exact quotients, and another implementation in more bits agrees with them one by one.  Read: two pieces a thread, their loads
 // together.
 // Both are bound by their bytes: reading 2 · dh · (2 or 4) bytes a token and head and writing dh + 8 · dh / G of them, or the reverse.
 #include "common.cuh"
@@ -11,6 +11,7 @@
 
 namespace {
 constexpr int PK_THREADS = 256;
+constexpr float PK_SURE = 0.49999f;                          // quotients this near a whole number round to it, whatever float32 makes of them
 
 // n / d for n < 2^31 and a d ≥ 2 by a multiplication (m = ⌊2^(31 + l) / d⌋ + 1 with l = ⌈log2 d⌉)
 struct Divide {
@@ -113,35 +114,84 @@ __device__ __forceinline__ uint32_t pack_code(float x, float zero, float step, f
     return (uint32_t)fminf(k + (up ? 1.f : 0.f), 15.f);
 }
 
-// eight codes; CLAMP: zero may lie above the least number (it was rounded)
-template <bool CLAMP, typename E> __device__ __forceinline__ uint32_t pack_word(const E& e, uint32_t pair) {
-    const float step = pair_step(pair), zero = pair_zero(pair);
-    if (!(step > 0.f)) return 0u;
+// (out of line: hardly ever gone)
+__device__ __noinline__ uint32_t pack_word_exact(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7, float zero, float step) {
+    // (a step so small that its inverse, or half of it, leaves float32: all three by 2^100, which changes no quotient)
+    const float by = step < 1e-30f ? 0x1p100f : 1.f, inv = 1.f / (step * by), x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) word |= pack_code(x[j] * by, zero * by, step * by, inv) << (4 * j);
+    return word;
+}
+
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void apart(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// eight codes, and whether float32 could say them for sure; CLAMP: zero may lie above the least number (it was rounded)
+template <bool CLAMP, typename E> __device__ __forceinline__ uint32_t pack_word(const E& e, uint32_t pair, bool& sure) {
+    const float zero = pair_zero(pair);
+    float step = pair_step(pair);
+    const bool flat = !(step > 0.f);                         // (0, or NaN: codes are 0)
+    step = flat ? 1.f : step;
     const float inv = 1.f / step;
     float worst = 0.f;
     uint32_t word = 0;
+    // quotients to half a unit of float32's last place (exact where they are float32 numbers, as ties are), and 15.06 at most
+    auto quotient = [&](int j) {
+        const float d = e.at(j) - zero, q = d * inv;
+        return fmaf(fmaf(-step, q, d), inv, q);
+    };
+    auto from_whole = [](float q) { return fabsf(q - ((q + 12582912.f) - 12582912.f)); };
+    // (two at a time in one instruction; sm_100)
+    const uint64_t less = two(-zero, -zero), inv2 = two(inv, inv), step2 = two(-step, -step), up = two(12582912.f, 12582912.f), down = two(-12582912.f, -12582912.f);
 #pragma unroll
-    for (int j = 7; j >= 0; --j) {
-        float q = (e.at(j) - zero) * inv;                    // off by 3 · 10^-6 at most, and 15.06 at most
-        if (CLAMP) q = fmaxf(q, 0.f);
-        const float y = q + 12582912.f;
-        worst = fmaxf(worst, fabsf(q - (y - 12582912.f)));
-        word = word * 16u + __float_as_uint(y);
+    for (int j = 6; j >= 0; j -= 2) {
+        const uint64_t d = add2(two(e.at(j), e.at(j + 1)), less), q0 = mul2(d, inv2);
+        uint64_t q = fma2(fma2(step2, q0, d), inv2, q0);
+        float a, b, ya, yb, ra, rb;
+        if (CLAMP) {
+            apart(q, a, b);
+            q = two(fmaxf(a, 0.f), fmaxf(b, 0.f));
+        }
+        const uint64_t y = add2(q, up);
+        apart(add2(y, down), ra, rb);
+        apart(add2(q, two(-ra, -rb)), a, b);
+        apart(y, ya, yb);
+        worst = fmaxf(worst, fmaxf(fabsf(a), fabsf(b)));
+        word = (word * 16u + __float_as_uint(yb)) * 16u + __float_as_uint(ya);
     }
     word -= 0x4b400000u * 0x11111111u;                       // (the bits of 1.5 · 2^23, eight times)
-    if (!(worst < 0.4999f) || step < 1e-30f) {
-        // (a step so small that its inverse, or half of it, leaves float32: all three by 2^100, which changes no quotient)
-        const float by = step < 1e-30f ? 0x1p100f : 1.f, up = 1.f / (step * by);
-        word = 0;
-#pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-            float x = 0.f;
+    sure = flat || (worst < PK_SURE && step >= 1e-30f);
+    if (!sure && step >= 1e-30f) {
+        // A tie is one if nothing is left of the difference, nor of its rounding, as is nearly always so for bfloat16 numbers, whose ties are many (1.5 % of
+        // the words of normal numbers; these eight looks cost a fifth of the kernel's time, and going the exact way for them would cost more).
+        sure = true;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x = i == j ? e.at(i) : x;
-            word |= pack_code(x * by, zero * by, step * by, up) << (4 * j);
+        for (int j = 0; j < 8; ++j) {
+            const float q = CLAMP ? fmaxf(quotient(j), 0.f) : quotient(j), off = from_whole(q), d = e.at(j) - zero;
+            sure = sure && (off < PK_SURE || (off == 0.5f && fmaf(-step, q, d) == 0.f && sub_rest(e.at(j), zero, d) == 0.f));
         }
     }
-    return word;
+    return flat ? 0u : word;
 }
 
 // PIECES: threads of a group (8 entries each)
@@ -165,14 +215,28 @@ packed_append_kernel(const ET* __restrict__ qkv, int ld, int k_off, int v_off, u
     if (mine && slot >= 0 && blk < 0 && c == 0) atomicOr(dev_err, VLRF_DEVERR_NO_BLOCK);
     const unsigned h = per_head(c), piece = c - h * per_head.d;
     const size_t row = ((size_t)max(blk, 0) * Hkv + h) * BT + (pos >= 0 ? pos % BT : 0);
+    uint32_t pair[2], word[2];
+    bool sure[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         float lo, hi;
         x[s].template range<PIECES>(lo, hi);
-        const uint32_t pair = pack_pair(lo, hi), word = pack_word<sizeof(ET) == 4>(x[s], pair);
-        if (mine && blk >= 0) {
-            (s == 0 ? Kq : Vq)[row * per_head.d + piece] = word;
-            if (piece % PIECES == 0) (s == 0 ? Kp : Vp)[row * (per_head.d / PIECES) + piece / PIECES] = pair;
+        pair[s] = pack_pair(lo, hi);
+        word[s] = pack_word<sizeof(ET) == 4>(x[s], pair[s], sure[s]);
+    }
+    if (!(sure[0] && sure[1])) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            if (!sure[s])
+                word[s] = pack_word_exact(x[s].at(0), x[s].at(1), x[s].at(2), x[s].at(3), x[s].at(4), x[s].at(5), x[s].at(6), x[s].at(7), pair_zero(pair[s]),
+                                          pair_step(pair[s]));
+    }
+    if (mine && blk >= 0) {
+        Kq[row * per_head.d + piece] = word[0];
+        Vq[row * per_head.d + piece] = word[1];
+        if (piece % PIECES == 0) {
+            Kp[row * (per_head.d / PIECES) + piece / PIECES] = pair[0];
+            Vp[row * (per_head.d / PIECES) + piece / PIECES] = pair[1];
         }
     }
 }
@@ -206,7 +270,7 @@ template <int VEC> __device__ __forceinline__ void store8(__nv_bfloat16* p, cons
     }
 }
 
-constexpr int PK_READ = 4;                                   // pieces of 8 entries (of keys and of values) a thread reads
+constexpr int PK_READ = 2;                                   // pieces of 8 entries (of keys and of values) a thread reads
 template <typename ET, int VEC, int PIECES>
 __global__ void __launch_bounds__(PK_THREADS)
 packed_read_kernel(const uint32_t* __restrict__ Kq, const uint32_t* __restrict__ Kp, const uint32_t* __restrict__ Vq, const uint32_t* __restrict__ Vp,
