@@ -357,14 +357,16 @@ PROMPTS = [([1], [0]), ([5], [64]), ([128], [0]), ([129, 2], [0, 127]), ([300, 1
 @pytest.mark.parametrize("window", [0, 1, 100])
 @pytest.mark.parametrize("groups,n_parts", [(1, 1), (2, 1), (1, 3), (2, 16)])
 def test_prompt_attention_on_the_tensor_cores(heads, kv_heads, dim, new, past, window, groups, n_parts):
-    """The bound of the weights counts three roundings here: a weight, a key and a value as bfloat16."""
+    """The bound counts three roundings here: a weight, a key and a value as float16."""
     pages = Pages([a + b for a, b in zip(new, past)], kv_heads, dim, seed=heads + sum(new))
     check_prompt(prefill(pages, new, heads, kv_heads, dim, window, groups, n_parts), pages, new, heads, kv_heads, dim, window)
 
 
 def check_prompt(fn, pages, new, heads, kv_heads, dim, window):
-    """A sample of the tokens against float64.  With h = 2^-8: a key rounded to bfloat16 moves a score by at most e_k = h · scale · Σ |q| |k|, the weights by a
-    factor of exp(2 e_k) together; a value moves by h of itself, and a weight by h, both times the largest |v|."""
+    """A sample of the tokens against float64.  A number of a key or a value is off by h = 2^-11 of itself, and, where it lies below float16's normal range (2^-14
+    of its first block's, or 2^-28 of its own row's largest), by less than that of the largest; so by 2 h of the largest at the very most.  That moves a score by
+    e_k ≤ 2 h · scale · Σ |q| · |k|max, the weights by a factor of exp(2 e_k) together, and the result by 2 h |v|max.  A weight is off by h of itself, and below
+    float16's range by 2^-25 where the row's reference point has 2^4: h + n 2^-29 of |v|max."""
     T, scale = sum(new), 1 / math.sqrt(dim)
     qkv = (torch.randn((T, (heads + 2 * kv_heads) * dim), generator=torch.Generator().manual_seed(9)) * 1.2).bfloat16()
     slot = [i for i, a in enumerate(new) for _ in range(a)]
@@ -387,8 +389,8 @@ def check_prompt(fn, pages, new, heads, kv_heads, dim, window):
         want = plain.attend(q, k, v, scale, window, p)
         for h in range(heads):
             kk, vv = k[first:p + 1, h // share], v[first:p + 1, h // share]
-            e_k = (HALF_STEP + (dim + 16) * U) * scale * float((kk.abs() * q[h].abs()).sum(-1).max())
-            tol = float(vv.abs().max()) * (math.expm1(2 * e_k) + 2 * HALF_STEP + (p + 1 - first + 32) * U)
+            e_k = (2.0 ** -10 + (dim + 16) * U) * scale * float(kk.abs().max() * q[h].abs().sum())
+            tol = float(vv.abs().max()) * (math.expm1(2 * e_k) + 3 * 2.0 ** -11 + (p + 1 - first) * 2.0 ** -29 + (p + 1 - first + 32) * U)
             tol = tol + HALF_STEP * (want[h].abs() + tol)
             off = (got[t].view(heads, dim)[h] - want[h]).abs()
             assert bool((off <= tol).all()), (t, i, p, h, float(off.max()), float(tol.max()))
@@ -397,8 +399,8 @@ def check_prompt(fn, pages, new, heads, kv_heads, dim, window):
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("groups,n_parts", [(1, 1), (2, 1), (1, 4)])
 def test_prompt_attention_is_as_good_as_its_roundings_are_random(dim, groups, n_parts):
-    """The bound above takes every rounding at its worst; over many numbers they cancel.  The mean square error of 400 tokens is held to that of
-    the same roundings done in float64 on the host, plus a quarter."""
+    """The bound above takes every rounding at its worst; over many numbers they cancel, and what is left beside the result's own rounding is little.  The
+    mean square error of 400 tokens is held to that of the same roundings done in float64 on the host, plus a quarter."""
     heads, new = 2, [400]
     pages = Pages([700], heads, dim, seed=2)
     qkv = (torch.randn((400, 3 * heads * dim), generator=torch.Generator().manual_seed(9)) * 1.2).bfloat16()
@@ -412,9 +414,9 @@ def test_prompt_attention_is_as_good_as_its_roundings_are_random(dim, groups, n_
         q = qkv[:, h * dim:(h + 1) * dim].double()
         mask = torch.arange(700)[None] <= torch.arange(300, 700)[:, None]
         want = torch.softmax(((q @ k[:, h].T) / math.sqrt(dim)).masked_fill(~mask, -math.inf), 1) @ v[:, h]
-        s = ((q @ r(k[:, h]).T) / math.sqrt(dim)).masked_fill(~mask, -math.inf)
-        w = torch.exp(s - s.amax(1, keepdim=True))
-        rounded = r((r(w) @ r(v[:, h])) / w.sum(1, keepdim=True))
+        s = ((q @ k[:, h].half().double().T) / math.sqrt(dim)).masked_fill(~mask, -math.inf)
+        w = torch.exp(s - s[:, :64].amax(1, keepdim=True))
+        rounded = r((w.half().double() @ v[:, h].half().double()) / w.sum(1, keepdim=True))
         err += float(((out.double().cpu()[:, h * dim:(h + 1) * dim] - want) ** 2).mean())
         ref += float(((rounded - want) ** 2).mean())
     assert int(e.item()) == 0 and err <= 1.25 * ref, (err, ref)
@@ -519,3 +521,80 @@ def test_refusals():
             ops.PackedKV(*tensors)
     with pytest.raises(KernelError):
         ops.PackedKV.zeros(3, 2, 64, 24, DEV)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sharp,size", [(1e4, 1.0), (1e-6, 1.0), (1.0, 1e5), (1.0, 1e-6), (1e3, 1e-3), (0.0, 1.0), (1.0, 1e-30), (1e-30, 1.0), (1e12, 1e20)])
+def test_prompt_attention_with_queries_and_keys_of_many_sizes(dim, sharp, size):
+    """Queries and keys that float16 does not hold as they are."""
+    heads, new = 2, [140]
+    pages = Pages([200], heads, dim, seed=5)
+    pages.host["k_pairs"] = (pages.host["k_pairs"].float() * size).bfloat16()
+    pages.cache.k_pairs.copy_(pages.host["k_pairs"])
+    qkv = (torch.randn((140, 3 * heads * dim), generator=torch.Generator().manual_seed(9)) * sharp).bfloat16()
+    scale = 1.0 / (math.sqrt(dim) * max(sharp, 1e-9) * size)
+    out = torch.zeros((140, heads * dim), dtype=torch.bfloat16, device=DEV)
+    e = err_word()
+    prefill(pages, new, heads, heads, dim, 0, 2, 1)(qkv.to(DEV), 0, pages.table.to(DEV), None, None, out, scale, e)
+    assert int(e.item()) == 0
+    k, v = pages.context(0)
+    for t in (0, 1, 70, 139):
+        q = qkv[t, :heads * dim].double().view(heads, dim)
+        want = plain.attend(q, k, v, scale, 0, 60 + t)
+        for h in range(heads):
+            kk, vv = k[:61 + t, h], v[:61 + t, h]
+            e_k = (2.0 ** -10 + (dim + 16) * U) * scale * float(kk.abs().max() * q[h].abs().sum())
+            tol = float(vv.abs().max()) * (math.expm1(2 * e_k) + 3 * 2.0 ** -11 + 400 * U)
+            tol = tol + HALF_STEP * (want[h].abs() + tol)
+            assert bool(((out[t].double().cpu().view(heads, dim)[h] - want[h]).abs() <= tol).all()), (t, h)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("groups,n_parts", [(1, 1), (2, 1), (2, 3)])
+@pytest.mark.parametrize("which", ["k_pairs", "v_pairs", "both"])
+@pytest.mark.parametrize("far,size", [((70, 100, 101, 190), 2.0 ** 20), ((3, 150), 2.0 ** 40), (tuple(range(64)), 2.0 ** 18), ((66, 130), 2.0 ** 15),
+                                      (tuple(range(64, 128)), 2.0 ** 60), (tuple(range(0, 200, 2)), 2.0 ** 17)])
+def test_prompt_attention_with_tokens_of_many_sizes(dim, groups, n_parts, which, far, size):
+    """Tokens whose keys or values lie far above those of the others; a row that does not see them has nothing of it."""
+    heads, new, past = 2, [140], 60
+    pages = Pages([200], heads, dim, seed=6)
+    parts = ["k_pairs", "v_pairs"] if which == "both" else [which]
+    for name in parts:
+        for t in far:
+            block = int(pages.table[0, t // 64])
+            pages.host[name][block, :, t % 64] = (pages.host[name][block, :, t % 64].float() * size).bfloat16()
+        getattr(pages.cache, name).copy_(pages.host[name])
+    qkv = (torch.randn((140, 3 * heads * dim), generator=torch.Generator().manual_seed(9)) * 1.2).bfloat16()
+    scale = 1.0 / (math.sqrt(dim) * (size if "k_pairs" in parts else 1.0))
+    out = torch.zeros((140, heads * dim), dtype=torch.bfloat16, device=DEV)
+    e = err_word()
+    prefill(pages, new, heads, heads, dim, 0, groups, n_parts)(qkv.to(DEV), 0, pages.table.to(DEV), None, None, out, scale, e)
+    assert int(e.item()) == 0
+    k, v = pages.context(0)
+    for t in (0, 3, 9, 10, 40, 41, 70, 89, 90, 139):
+        q = qkv[t, :heads * dim].double().view(heads, dim)
+        want = plain.attend(q, k, v, scale, 0, past + t)
+        for h in range(heads):
+            kk, vv = k[:past + 1 + t, h], v[:past + 1 + t, h]
+            e_k = (2.0 ** -10 + (dim + 16) * U) * scale * float(kk.abs().max() * q[h].abs().sum())
+            tol = float(vv.abs().max()) * (math.expm1(2 * e_k) + 3 * 2.0 ** -11 + 400 * U)
+            tol = tol + HALF_STEP * (want[h].abs() + tol)
+            assert bool(((out[t].double().cpu().view(heads, dim)[h] - want[h]).abs() <= tol).all()), (t, h)
+
+
+def test_a_query_that_is_not_finite_leaves_the_other_rows_alone():
+    pages = Pages([150], 2, 64)
+    qkv = torch.randn(150, 6 * 64).bfloat16()
+    outs = []
+    for bad in (None, float("inf"), float("nan")):
+        x = qkv.clone()
+        if bad is not None:
+            x[77, 3] = bad                     # head 0
+        out = torch.zeros(150, 128, device=DEV, dtype=torch.bfloat16)
+        e = err_word()
+        prefill(pages, [150], 2, 2, 64, 0, 2, 1)(x.to(DEV), 0, pages.table.to(DEV), None, None, out, 0.125, e)
+        outs.append(out.cpu())
+    for o in outs[1:]:
+        assert bool(torch.isnan(o[77, :64]).any())
+        o[77, :64] = outs[0][77, :64]
+        assert torch.equal(o, outs[0])

@@ -3,24 +3,31 @@
 //
 // A CTA takes GROUPS · 128 consecutive new tokens of one sequence and one head and walks the keys they see in blocks of 64 up to the
 // diagonal.  Its warps have fixed jobs:
-//   producers      codes and pairs of a block from the cache into registers, a block ahead; from there zero + step · code as bfloat16 (one rounding)
-//                  into a ring of 64 KB of shared memory, K and V in turn, in the 128-byte swizzle that the MMA reads.  A code becomes
-//                  a bfloat16 by a mask under the exponent of 128, less 128 (exact), two at a time; pairs of entries i and i + 4 of eight
-//                  stay neighbours, so the numbers of a row lie permuted, those of the queries likewise (the sum does not care), and the
-//                  result is put in order where it is written.  Rows that no query may see, behind the sequence's last token or in
-//                  blocks wholly before the window, are zeros and are not read;
+//   producers      codes and pairs of a block from the cache into registers, a block ahead; from there zero + step · code as float16 into a ring of 64 KB of
+//                  shared memory, K and V in turn, in the 128-byte swizzle that the MMA reads.  A code becomes a number by a mask under an exponent, two
+//                  at a time; pairs of entries i and i + 4 of eight stay neighbours, so the numbers of a row lie permuted, those of the queries likewise (the
+//                  sum does not care), and the result is put in order where it is written.  Rows that no query may see, behind the sequence's last
+//                  token or in blocks wholly before the window, are zeros and are not read;
 //   MMA warps      (one a group) S = Q·Kᵀ into tensor memory and, once the probabilities are there, O += P·V (P is the operand in tensor memory, V
 //                  is read as it lies, head dimension contiguous);
 //   softmax warps  eight a group of 128 queries: a query is one lane of tensor memory, and two threads have a half of a block's keys each;
 //                  running maximum and sum in float32, O scaled where a maximum grew.
 // With GROUPS = 2 two groups share every block that the producers take apart.
 //
-// Keys and values enter the products as bfloat16, so each is off by at most 2^-8 of itself beyond the cache's own rounding, as are the weights; scores,
-// sums and results stay in float32.  A value that is not a number must not meet the weight 0 of a query that does not see it (0 · NaN is
-// not 0): its row of V becomes zeros, and its key's row of K NaN instead, which the mask hides from the same queries; so a head's row that
-// sees it is NaN throughout.
+// Queries, keys, weights and values are float16 operands (11 bits: each off by up to 2^-11 of itself), scores, sums and results float32; as bfloat16 they
+// together moved a result by 2.5 times what its own rounding does, as float16 by a tenth of that.  What float16 lacks in range powers of two give: the
+// queries' from their largest, the keys' and the values' from the CTA's first block, weights stay below 2^15; a key or a value 2^14 times as large as
+// the first block's gets a power of its own, which costs its block a slower pass.
+// A value that is not a number must not meet the weight 0 of a query that does not see it (0 · NaN is not 0): its row of V becomes zeros, and its
+// key's row of K NaN instead, which the mask hides from the same queries; so a head's row that sees it is NaN throughout.
+//
+// Bound by the chain of a block, some 2,800 cycles at head size 128 of which the tensor cores have 1,000: producers take a block's numbers apart in the issue
+// slots that softmax leaves (1,000 cycles each for K and V), and S waits for them.  More producers would take registers from the softmax warps, which then
+// spill (28 warps: 173 us where 22 take 119); blocks of 64 keys with two threads a row are what 80 registers hold.  Measured: 512 new tokens
+// behind 7500, 32 heads of 128 over 8: 119 us, 0.55 PFLOP/s; twice 1024 new tokens, 12 heads of 64: 21.8 us.
 // Every wait is bounded; a CTA that gives up sets the device error word, waits (bounded) for its MMAs, frees its tensor memory and leaves.
 #include <type_traits>
+#include <cuda_fp16.h>
 #include "common.cuh"
 #include "packed_kv.cuh"
 #include "tcgen05.cuh"
@@ -28,7 +35,9 @@
 namespace {
 constexpr int PP_CB = 64, PP_BK = 64, PP_RING = 65536;              // tokens of a cache block; keys of a block; bytes of the ring
 constexpr int PP_MAX_PARTS = 16;
-constexpr float PP_MOST = 2048.f, PP_LEAST = 4.f;                   // (64 weights that add up to 2^11: one is 2^5 at least)
+// Weights lie 2^PP_UP times as large (float16 then has them down to 2^-28 of the reference point's), and add up to PP_MOST at most before that moves: any is
+// float16 still.  (32 weights that add up to 2^15: one is 2^10 at least, 2^6 above the reference point's.)
+constexpr float PP_UP = 4.f, PP_MOST = 32768.f, PP_LEAST = 5.f;
 constexpr __host__ __device__ int pp_producers(int GROUPS) { return 2 * GROUPS; }
 constexpr __host__ __device__ int pp_threads(int GROUPS) { return (GROUPS * 8 + pp_producers(GROUPS) + GROUPS) * 32; }
 constexpr __host__ __device__ int pp_part_floats(int DH) { return DH * 128 + 256; }
@@ -66,8 +75,9 @@ __device__ __forceinline__ uint64_t pp_desc_mn(const void* tile, uint32_t chunk)
     d |= (uint64_t)2 << 61;
     return d;
 }
-__host__ __device__ constexpr uint32_t pp_idesc_mn(int M, int N) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+// instruction descriptor: D float32, A and B float16, A K-major, B K-major or (mn) MN-major
+__host__ __device__ constexpr uint32_t pp_idesc(int M, int N, bool mn) {
+    return (1u << 4) | (mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 __device__ __forceinline__ void pp_mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -93,19 +103,28 @@ __device__ __forceinline__ void pp_st32(uint32_t taddr, const uint32_t (&r)[32])
           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
-// eight codes of a word as bfloat16 numbers: entries (0, 4), (1, 5), (2, 6), (3, 7)
-__device__ __forceinline__ uint4 pp_numbers(uint32_t w, __nv_bfloat162 step, __nv_bfloat162 zero) {
+// Eight codes of a word as float16 numbers step · code + zero, entries (0, 4), (1, 5), (2, 6), (3, 7): a code under the exponent of 1024, where the upper
+// code of a byte counts sixteenfold, so half of the shifts go.
+__device__ __forceinline__ uint4 pp_numbers(uint32_t w, __half2 step, __half2 zero) {
+    const __half2 less = __float2half2_rn(-1024.f), by = __float2half2_rn(0.0625f), less16 = __float2half2_rn(-64.f);
     uint32_t r[4];
-    const uint32_t magic = 0x43004300u;                             // 128, twice
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t x = ((w >> (4 * i)) & PK_LOW) | magic;
-        const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&magic));
-        const __nv_bfloat162 v = __hfma2(c, step, zero);
-        r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t x = w >> (8 * i), lo = (x & PK_LOW) | 0x64006400u, hi = (x & PK_HIGH) | 0x64006400u;
+        const __half2 a = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&lo), less), step, zero);
+        const __half2 b = __hfma2(__hfma2(*reinterpret_cast<const __half2*>(&hi), by, less16), step, zero);
+        r[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+        r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
+// 2^e, e held to what float32 has
+__device__ __forceinline__ float pp_power(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+// the exponent of a bfloat16 (of the bits of its upper half, sign away): 2^e ≤ |x| < 2^(e + 1); −127 for zero and what is below 2^-126
+__device__ __forceinline__ int pp_exponent(uint32_t bits) { return (int)(bits >> 7 & 255u) - 127; }
+
+// what the queries are divided by, as a power of two: their largest (its bits) comes to 2^14
+__device__ __forceinline__ int pp_up(uint32_t top) { return max(pp_exponent(top), -110) - 14; }
 
 template <int DH, int GROUPS>
 __global__ void __launch_bounds__(pp_threads(GROUPS), GROUPS == 1 ? 2 : 1)
@@ -123,7 +142,10 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     unsigned char* q_tiles = smem;                                  // [GROUPS][NG][128][128 B]
     unsigned char* kv_tiles = smem + GROUPS * Q_BYTES;              // [PP_SLOTS][NG][BK][128 B]: K_0, V_0, K_1, V_1, …
     float* s_part = reinterpret_cast<float*>(kv_tiles + PP_RING);     // [GROUPS][2][128]
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(s_part + GROUPS * 256);       // [GROUPS]
+    float2* s_far = reinterpret_cast<float2*>(s_part + GROUPS * 256);            // [PP_SLOTS][64]: of block b at b % PP_SLOTS, each key's powers (see producers)
+    uint32_t* s_any_far = reinterpret_cast<uint32_t*>(s_far + PP_SLOTS * 64);    // [PP_SLOTS]: whether any of a producer's is not 0, a byte each (without: not written)
+    uint64_t* q_known = reinterpret_cast<uint64_t*>(s_any_far + PP_SLOTS);
+    uint64_t* q_full = q_known + 1;       // [GROUPS]
     uint64_t* full = q_full + GROUPS;
     uint64_t* empty = full + PP_SLOTS;
     uint64_t* s_full = empty + PP_SLOTS;                            // [GROUPS] each from here
@@ -134,7 +156,10 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
     int* s_never = s_abort + 1;                                     // stays 0: for waits that nothing calls off
-    int* s_last = s_never + 1;                                      // [GROUPS]: whether this CTA merges its tile's parts
+    int* s_top = s_never + 1;                                       // the largest of the queries' bits, sign away
+    int* s_first = s_top + 1;                                       // [2]: of the largest numbers of the first block's keys and of its values, the smallest, as bits
+    float* s_unit = reinterpret_cast<float*>(s_first + 2);          // [2]: from an MMA's result to a score in units of log2(e); from one of O to a number
+    int* s_last = reinterpret_cast<int*>(s_unit + 2);                                        // [GROUPS]: whether this CTA merges its tile's parts
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // z is the slowest index of the order in which CTAs are started: first parts first, and within a part long tiles first
@@ -143,14 +168,18 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         for (int i = 0; i < PP_SLOTS; ++i) { tbar_init(&full[i], NPROD); tbar_init(&empty[i], GROUPS); }
         for (int g = 0; g < GROUPS; ++g) {
             tbar_init(&q_full[g], 8);
-            tbar_init(&s_full[g], 1);
+            tbar_init(&s_full[g], 2);                               // the MMAs, and what the producers left beside the numbers
             tbar_init(&s_read[g], 8);
             for (int i = 0; i < NP; ++i) { tbar_init(&p_full[g * NP + i], 8); tbar_init(&o_full[g * NP + i], 1); }
             s_last[g] = 1;
         }
         tbar_init(drained, GROUPS);
+        tbar_init(q_known, SOFT);
         *s_abort = 0;
         *s_never = 0;
+        *s_top = 0;
+        s_first[0] = s_first[1] = 0x7f80;
+        for (int i = 0; i < PP_SLOTS; ++i) s_any_far[i] = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -219,23 +248,81 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                 }
             }
         };
+        // Keys and values lie divided by powers of two, 2^key_up and 2^value_up, that take to 1 … 2 the smallest of the largest numbers that the keys, or the
+        // values, of the CTA's first block have each.  Numbers up to 2^15 times that are float16 then, and those of a row whose largest is 2^-14 of it lose
+        // nothing.  A key or a value beyond (`far`) lies divided by a power of its own; its score is multiplied, or its weight, by what that is more.
+        int key_up = 0, value_up = 0;
+        auto top_of = [](uint32_t pair) {                           // the largest number of a group, as bits of a bfloat16 (NaN: 0)
+            const float zero = pair_zero(pair), top = fmaxf(fabsf(zero), fabsf(fmaf(15.f, pair_step(pair), zero)));
+            return top == top ? (int)(__float_as_uint(top) >> 16) : 0;
+        };
+        auto both = [](int e) { return NG == 2 ? max(e, __shfl_xor_sync(0xffffffffu, e, 2)) : e; };     // (a row's other group is two lanes on)
+        int value_far[UNITS];                                       // of the block that is being put
+        // a pair whose zero is below 2^14 and whose step is below 2^10 times the unit needs no power of its own (|zero| + 15 step < 2^15); both as bfloat16
+        uint32_t key_limit = 0u, value_limit = 0u;
+        auto limit_of = [](int up) { return (uint32_t)(up + 10 + 127) << 7 | (uint32_t)(up + 14 + 127) << 23; };
+        auto beyond = [](uint32_t most, uint32_t limit) {           // (NaN is not)
+            const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&most), b = *reinterpret_cast<const __nv_bfloat162*>(&limit);
+            return __hge(a.x, b.x) || __hge(a.y, b.y);
+        };
+        auto larger = [](uint32_t x, uint32_t y) {                  // of both halves, signs away
+            x &= 0x7fff7fffu;
+            const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+            return *reinterpret_cast<const uint32_t*>(&m);
+        };
+        auto far_of = [&](uint32_t pair, int up) { return max(0, pp_exponent((uint32_t)both(top_of(pair))) - up - 14); };
         auto put = [&](int t, const Piece& from) -> bool {          // tile t of this CTA: block t / 2, K or V
             const int sl = t % PP_SLOTS, use = t / PP_SLOTS;
+            int key_far[UNITS];
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) key_far[i] = 0;
+            if (!(t & 1)) {
+                uint32_t key_most = 0u, value_most = 0u;
+#pragma unroll
+                for (int i = 0; i < UNITS; ++i) {
+                    value_far[i] = 0;
+                    key_most = larger(from.pairs[i], key_most);
+                    value_most = larger(from.value_pairs[i], value_most);
+                }
+                any = __any_sync(0xffffffffu, beyond(key_most, key_limit) || beyond(value_most, value_limit));
+            }
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < UNITS; ++i) {
+                    key_far[i] = far_of(from.pairs[i], key_up);
+                    value_far[i] = far_of(from.value_pairs[i], value_up);
+                }
+            }
+            __half2 step[UNITS], zero[UNITS];
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const bool nan_value = (from.value_pairs[i] & 0x7fffu) > 0x7f80u;        // (NaN in a value's pair, both halves of it: zeros in V, NaN in K)
+                const uint32_t pair = (t & 1) ? (nan_value ? 0u : from.value_pairs[i]) : (nan_value ? 0x7fff7fffu : from.pairs[i]);
+                const float down = pp_power(-((t & 1) ? value_up + value_far[i] : key_up + key_far[i]));
+                step[i] = __float2half2_rn(pair_step(pair) * down);
+                zero[i] = __float2half2_rn(pair_zero(pair) * down);
+            }
             if (use >= 1 && !tbar_wait_warp(&empty[sl], (uint32_t)((use - 1) & 1), s_abort)) return false;
             unsigned char* tile = kv_tiles + (size_t)sl * PP_TILE;
+            if (!(t & 1)) {
+                const int at = t / 2 % PP_SLOTS;
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < UNITS; ++i) {
+                        const int u = i * 32 + lane, r = p * PR + u / (DH / 32), c = u % (DH / 32);
+                        if (c == 0) s_far[at * 64 + r] = make_float2(pp_power(key_far[i]), (float)value_far[i]);
+                    }
+                }
+                if (lane == 0) reinterpret_cast<unsigned char*>(s_any_far + at)[p] = any;
+            }
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) {
                 const int u = i * 32 + lane, r = p * PR + u / (DH / 32), c = u % (DH / 32);
-                // (NaN in a value's pair, both halves of it: zeros in V, NaN in K)
-                uint32_t pair = (t & 1) ? from.value_pairs[i] : from.pairs[i];
-                if ((from.value_pairs[i] & 0x7fffu) > 0x7f80u) pair = (t & 1) ? 0u : 0x7fff7fffu;
-                const uint32_t s2 = __byte_perm(pair, 0, 0x1010), z2 = __byte_perm(pair, 0, 0x3232);
-                const __nv_bfloat162 step = *reinterpret_cast<const __nv_bfloat162*>(&s2), zero = *reinterpret_cast<const __nv_bfloat162*>(&z2);
                 unsigned char* dst = tile + (c >> 1) * ATOM_KV + r * 128;
                 const uint32_t w[4] = {from.codes[i].x, from.codes[i].y, from.codes[i].z, from.codes[i].w};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<uint4*>(dst + ((((c & 1) * 4 + j) ^ (r & 7)) << 4)) = pp_numbers(w[j], step, zero);
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + ((((c & 1) * 4 + j) ^ (r & 7)) << 4)) = pp_numbers(w[j], step[i], zero[i]);
             }
             return true;
         };
@@ -249,21 +336,44 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             const int blk = block_of(0);
             fetch(0, blk, std::false_type{}, piece[0]);
             fetch(0, blk, std::true_type{}, piece[1]);
+            uint32_t top[2] = {0x7f80u, 0x7f80u};
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const uint32_t a = (uint32_t)both(top_of(piece[0].pairs[i])), b = (uint32_t)both(top_of(piece[1].value_pairs[i]));
+                top[0] = min(top[0], a != 0 ? a : 0x7f80u);         // (a row of zeros says nothing)
+                top[1] = min(top[1], b != 0 ? b : 0x7f80u);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                top[x] = __reduce_min_sync(0xffffffffu, top[x]);
+                if (lane == 0) atomicMin(&s_first[x], (int)top[x]);
+            }
+            asm volatile("bar.sync 11, %0;" ::"n"(NPROD * 32) : "memory");
+            // (where no row says anything: 2^0; the top of float32 is kept away from, so that sums of weights times values have room)
+            key_up = s_first[0] == 0x7f80 ? 0 : min(max(pp_exponent((uint32_t)s_first[0]), -110), 80);
+            value_up = s_first[1] == 0x7f80 ? 0 : min(max(pp_exponent((uint32_t)s_first[1]), -110), 80);
+            key_limit = limit_of(key_up);
+            value_limit = limit_of(value_up);
+            ok = tbar_wait_warp(q_known, 0, s_abort);
+            if (p == 0 && lane == 0) {
+                s_unit[0] = fminf(pp_power(key_up) * (scale * 1.4426950408889634f) * pp_power(pp_up((uint32_t)*s_top)), 3.4028235e38f);
+                s_unit[1] = pp_power(value_up);
+            }
         }
-        for (int b = 0; b < my_n; ++b) {
+        for (int b = 0; b < my_n && ok; ++b) {
             const int next = b + 1 < my_n ? block_of(b + 1) : -1;
             if (!(ok = put(2 * b, piece[0]))) break;
-            if (b + 1 < my_n) fetch(b + 1, next, std::false_type{}, piece[0]);
             hand_over(2 * b);
+            if (b + 1 < my_n) fetch(b + 1, next, std::false_type{}, piece[0]);
             if (!(ok = put(2 * b + 1, piece[1]))) break;
-            if (b + 1 < my_n) fetch(b + 1, next, std::true_type{}, piece[1]);
             hand_over(2 * b + 1);
+            if (b + 1 < my_n) fetch(b + 1, next, std::true_type{}, piece[1]);
         }
         if (!ok) atomicExch(s_abort, 1);
     } else if (warp >= SOFT + NPROD) {
         // ---- MMAs, a warp a group
         const int g = warp - SOFT - NPROD, my_lo = g == 0 ? lo[0] : lo[GROUPS - 1], my_hi = g == 0 ? hi[0] : hi[GROUPS - 1];
-        constexpr uint32_t idesc_s = umma_idesc_bf16(128, BK), idesc_o = pp_idesc_mn(128, DH);
+        constexpr uint32_t idesc_s = pp_idesc(128, BK, false), idesc_o = pp_idesc(128, DH, true);
         const uint64_t dq = umma_desc_k128(q_tiles + g * Q_BYTES), dk0 = umma_desc_k128(kv_tiles), dv0 = pp_desc_mn(kv_tiles, ATOM_KV);
         const uint32_t tmem_s = tmem + g * 256, tmem_o = tmem_s + BK, tmem_p = tmem_o + DH;
         bool ok = true;
@@ -283,6 +393,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                         umma_bf16(tmem_s, dq + (uint64_t)(((k >> 2) * ATOM_Q) >> 4) + 2 * (k & 3), dk + (uint64_t)(((k >> 2) * ATOM_KV) >> 4) + 2 * (k & 3),
                                   idesc_s, k > 0 ? 1u : 0u);
                     umma_commit(&s_full[g]);
+                    tbar_arrive(&s_full[g]);
                     umma_commit(&empty[sl]);
                 } else {
                     tbar_arrive(&empty[sl]);
@@ -326,32 +437,67 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         const uint32_t tmem_s = tmem + g * 256 + lane_addr, tmem_o = tmem_s + BK, tmem_p = tmem_o + DH;
         unsigned char* q_tile = q_tiles + g * Q_BYTES;
         float* sp = s_part + g * 256;
-        const float sl2 = scale * 1.4426950408889634f;              // scores in units of log2(e)
         const unsigned win_eff = window > 0 ? (unsigned)window : 0x7fffffffu;    // key visible: 0 ≤ q_pos − key < win_eff
-        if (n_i > 0) {
-            // the queries, eight entries a piece, in the producers' order
-            for (int idx = threadIdx.x & 255; idx < 128 * (DH / 8); idx += 256) {
-                const int rr = idx / (DH / 8), c = idx % (DH / 8);
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (rr < group_rows) v = *reinterpret_cast<const uint4*>(qkv + (size_t)(row0 + t_first + g * 128 + rr) * ld + q_off + (size_t)h * DH + c * 8);
-                *reinterpret_cast<uint4*>(q_tile + (c >> 3) * ATOM_Q + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) =
-                    make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+        {
+            // the queries, eight entries a piece, in the producers' order, as float16 divided by a power of two that takes the CTA's largest to 2^14: their
+            // eight bits are all there but for numbers 2^-31 of that
+            constexpr int PIECES = 128 * (DH / 8) / 256;
+            uint4 v[PIECES];
+            uint32_t top = 0;
+#pragma unroll
+            for (int x = 0; x < PIECES; ++x) {
+                const int idx = x * 256 + (threadIdx.x & 255), rr = idx / (DH / 8), c = idx % (DH / 8);
+                v[x] = make_uint4(0u, 0u, 0u, 0u);
+                if (rr < group_rows) v[x] = *reinterpret_cast<const uint4*>(qkv + (size_t)(row0 + t_first + g * 128 + rr) * ld + q_off + (size_t)h * DH + c * 8);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+#pragma unroll
+            for (int x = 0; x < PIECES; ++x) {
+                const uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {                       // (what is not finite stays so whatever it is divided by)
+                    const uint32_t a = w[y] & 0x7fffu, b = w[y] >> 16 & 0x7fffu;
+                    top = max(top, max(a < 0x7f80u ? a : 0u, b < 0x7f80u ? b : 0u));
+                }
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) {
+                atomicMax(s_top, (int)top);
+                tbar_arrive(q_known);
+            }
             __syncwarp();
-            if (lane == 0) tbar_arrive(&q_full[g]);
+            if (n_i > 0 && tbar_wait_warp(q_known, 0, s_abort)) {
+                const float down = pp_power(-pp_up((uint32_t)*s_top));
+#pragma unroll
+                for (int x = 0; x < PIECES; ++x) {
+                    const int idx = x * 256 + (threadIdx.x & 255), rr = idx / (DH / 8), c = idx % (DH / 8);
+                    const uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+                    uint32_t o[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {                   // entries (y, y + 4)
+                        const uint32_t lo = w[y >> 1], hi = w[2 + (y >> 1)];
+                        const __half2 two = (y & 1) ? __floats2half2_rn(__uint_as_float(lo & 0xffff0000u) * down, __uint_as_float(hi & 0xffff0000u) * down)
+                                                    : __floats2half2_rn(__uint_as_float(lo << 16) * down, __uint_as_float(hi << 16) * down);
+                        o[y] = *reinterpret_cast<const uint32_t*>(&two);
+                    }
+                    *reinterpret_cast<uint4*>(q_tile + (c >> 3) * ATOM_Q + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tbar_arrive(&q_full[g]);
+            }
         }
         float m_run = -INFINITY, l_run = 0.f;                       // the row's reference point; the sum of this half
         bool ok = true;
         auto wait_o = [&](int j) { return tbar_wait_warp(&o_full[g * NP + j % NP], (uint32_t)((j / NP) & 1), s_abort); };       // until O holds block j
-        auto block = [&](int i, auto masked_c) {
+        float unit = 0.f;                                           // (known once the first scores are there)
+        // MASKED: some key of the block may be hidden from some row, and (is_far) some key or value may have a power of its own
+        auto block = [&](int i, auto masked_c, bool there, uint32_t is_far) {
             constexpr bool MASKED = decltype(masked_c)::value;
             const int k0 = (my_lo + i) * BK + half * HK;            // the half's first key
             // chunks of 32 keys of which a row of this warp sees any (those behind lie above the diagonal)
             const int q_top = group_first + q * 32 + 31;
             const int n_live = MASKED ? (q_top < k0 ? 0 : min(NC, ((q_top - k0) >> 5) + 1)) : NC;
             // (a warp that has given up goes on meeting its neighbour, who may not have, until both have: with nothing to tell)
-            const bool there = ok && tbar_wait_warp(&s_full[g], (uint32_t)(i & 1), s_abort);
             if (!there) {
                 ok = false;
                 uint32_t any;
@@ -366,15 +512,18 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t s_at = tmem_s + (uint32_t)(half * HK), p_at = tmem_p + (uint32_t)((i % NP) * (BK / 2) + half * (HK / 2));
             uint32_t sv[NC][32];
-            // Exponentials of a chunk against m_use, P as bfloat16 into tensor memory; their sum onto `sum`.
-            auto chunk = [&](int c, const uint32_t (&x)[32], float m_use, uint64_t (&sum)[2]) {
+            unit = s_unit[0];
+            const float2* far = s_far + ((my_lo + i - my_first) % PP_SLOTS) * 64;
+            // Exponentials of a chunk, x times `by` being scores in units of log2(e), against m_use and 2^PP_UP times; P as float16 into tensor memory, their
+            // sum onto `sum`.
+            auto chunk = [&](int c, const uint32_t (&x)[32], float by, float m_use, uint64_t (&sum)[2]) {
                 uint32_t pk[16];
                 const int d0 = q_pos - (k0 + c * 32);               // q_pos − key for e = 0
-                const uint64_t by = pp_two(sl2, sl2), from = pp_two(-m_use, -m_use);
+                const uint64_t by2 = pp_two(by, by), from = pp_two(PP_UP - m_use, PP_UP - m_use);
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float p0, p1;
-                    pp_apart(pp_fma2(pp_two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), by, from), p0, p1);
+                    pp_apart(pp_fma2(pp_two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), by2, from), p0, p1);
                     p0 = pp_exp2(p0);
                     p1 = pp_exp2(p1);
                     if (MASKED) {
@@ -382,9 +531,24 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                         p1 = (unsigned)(d0 - e - 1) < win_eff ? p1 : 0.f;
                     }
                     sum[(e >> 1) & 1] = pp_add2(sum[(e >> 1) & 1], pp_two(p0, p1));
-                    pk[e >> 1] = pack2(p0, p1);
+                    const __half2 two = __floats2half2_rn(p0, p1);
+                    pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&two);
                 }
                 pp_st16(p_at + (uint32_t)(c * 16), pk);
+            };
+            // a chunk's scores with the powers of its keys and values; with m_use, returns the sum of its weights without those of the values
+            auto with_powers = [&](int c, uint32_t (&x)[32], float m_use) {
+                float plain = 0.f;
+                const int d0 = q_pos - (k0 + c * 32);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int key = half * HK + c * 32 + e;
+                    const float2 power = (is_far >> (key / (BK / NPROD) * 8) & 255u) != 0u ? far[key] : make_float2(1.f, 0.f);
+                    const float score = __uint_as_float(x[e]) * power.x * unit;
+                    plain += (unsigned)(d0 - e) < win_eff ? pp_exp2(score + (PP_UP - m_use)) : 0.f;
+                    x[e] = __float_as_uint(score + power.y);
+                }
+                return plain;
             };
             auto total = [](const uint64_t (&sum)[2]) {
                 float a0, a1, b0, b1;
@@ -423,15 +587,15 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) tbar_arrive(&s_read[g]);
-                // No maximum is looked for while the weights against the reference point stay small: they are as exact in bfloat16 and float32 up to 2^11 as
-                // up to 1.  A row whose weights of this block add up to more (for random rows hardly any behind the first block) moves its reference
+                // No maximum is looked for while the weights against the reference point stay small: they are as exact in float16 up to 2^15 as up to
+                // 1.  A row whose weights of this block add up to more (for random rows hardly any behind the first block) moves its reference
                 // point, and the two warps begin the block anew.
                 if (i > 0) {
                     if (i >= NP && !wait_o(i - NP)) ok = false;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     uint64_t s2[2] = {0ull, 0ull};
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) chunk(c, sv[c], reference(), s2);
+                    for (int c = 0; c < NC; ++c) chunk(c, sv[c], unit, reference(), s2);
                     sum = total(s2);
                 }
                 moved = either(i == 0 || m_run == -INFINITY || sum > PP_MOST);
@@ -440,13 +604,13 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(sv[c][x]));
-                    corr = move_reference(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2, PP_LEAST);
+                        for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(sv[c][x]) * unit);
+                    corr = move_reference(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), PP_LEAST);
                     if (i > 0 && !wait_o(i - 1)) ok = false;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     uint64_t s2[2] = {0ull, 0ull};
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) chunk(c, sv[c], reference(), s2);
+                    for (int c = 0; c < NC; ++c) chunk(c, sv[c], unit, reference(), s2);
                     sum = total(s2);
                 }
                 if (!ok) return;
@@ -456,11 +620,13 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                 for (int c = 0; c < n_live; ++c) {
                     tmem_ld32(s_at + (uint32_t)(c * 32), sv[0]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (is_far != 0u) with_powers(c, sv[0], 0.f);
+                    const float by = is_far != 0u ? 1.f : unit;
                     const int d0 = q_pos - (k0 + c * 32);
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], (unsigned)(d0 - x) < win_eff ? __uint_as_float(sv[0][x]) : -INFINITY);
+                    for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], (unsigned)(d0 - x) < win_eff ? __uint_as_float(sv[0][x]) * by : -INFINITY);
                 }
-                const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+                const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 moved = either(m_half > m_run + PP_LEAST);
                 if (moved) corr = move_reference(m_half, PP_LEAST);
                 const int before = moved ? i - 1 : i - NP;
@@ -469,12 +635,14 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
                 uint64_t s2[2] = {0ull, 0ull};
+                float plain = 0.f;
 #pragma unroll 1
                 for (int c = 0; c < NC; ++c) {
                     if (c < n_live) {
                         tmem_ld32(s_at + (uint32_t)(c * 32), sv[0]);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        chunk(c, sv[0], reference(), s2);
+                        if (is_far != 0u) plain += with_powers(c, sv[0], reference());
+                        chunk(c, sv[0], is_far != 0u ? 1.f : unit, reference(), s2);
                     } else {
                         uint32_t none[16];
 #pragma unroll
@@ -482,7 +650,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                         pp_st16(p_at + (uint32_t)(c * 16), none);
                     }
                 }
-                sum = total(s2);
+                sum = is_far != 0u ? plain : total(s2);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) tbar_arrive(&s_read[g]);
@@ -504,42 +672,66 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             __syncwarp();
             if (lane == 0) tbar_arrive(&p_full[g * NP + i % NP]);
         };
-        for (int i = 0; i < n_i; ++i) {
-            if (window > 0 || (my_lo + i) * BK + BK - 1 > group_first) block(i, std::true_type{});       // (uniform over the group)
-            else block(i, std::false_type{});
+        for (int i = 0; i < n_i; ++i) {                             // (uniform over the group)
+            const bool there = ok && tbar_wait_warp(&s_full[g], (uint32_t)(i & 1), s_abort);
+            const uint32_t is_far = there ? s_any_far[(my_lo + i - my_first) % PP_SLOTS] : 0u;
+            if (is_far != 0u || window > 0 || (my_lo + i) * BK + BK - 1 > group_first) block(i, std::true_type{}, there, is_far);
+            else block(i, std::false_type{}, there, 0u);
         }
-        // the row's result of this half's columns, and the sum of both halves of the keys
-        float o_acc[HD];
-#pragma unroll
-        for (int d = 0; d < HD; ++d) o_acc[d] = 0.f;
-        if (n_i > 0) {
-            if (ok && wait_o(n_i - 1)) {
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                for (int d0 = 0; d0 < HD; d0 += 32) {
-                    uint32_t ov[32];
-                    tmem_ld32(tmem_o + (uint32_t)(half * HD + d0), ov);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) o_acc[d0 + x] = __uint_as_float(ov[x]);
-                }
-            } else {
-                ok = false;
-                atomicExch(s_abort, 1);
+        // the row's result, a half of the columns a thread and 32 of them at a time, and the sum of both halves of the keys
+        const bool any_o = n_i > 0 && ok && wait_o(n_i - 1);
+        if (n_i > 0 && !any_o) {
+            ok = false;
+            atomicExch(s_abort, 1);
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        auto result = [&](int d0, float (&o)[32]) {
+            uint32_t ov[32];
+            if (any_o) {
+                tmem_ld32(tmem_o + (uint32_t)(half * HD + d0), ov);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             }
-        }
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = any_o ? __uint_as_float(ov[x]) * s_unit[1] : 0.f;
+        };
+        // as bfloat16, entries in order again, into shared memory (Q's tile: no MMA reads it any more)
+        auto leave = [&](int d0, const float (&o)[32], float inv) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 8) {
+                uint4 pk;
+                pk.x = pack2(o[d] * inv, o[d + 2] * inv); pk.y = pack2(o[d + 4] * inv, o[d + 6] * inv);
+                pk.z = pack2(o[d + 1] * inv, o[d + 3] * inv); pk.w = pack2(o[d + 5] * inv, o[d + 7] * inv);
+                const int c = (half * HD + d0 + d) >> 3;
+                *reinterpret_cast<uint4*>(q_tile + (c >> 3) * ATOM_Q + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = pk;
+            }
+        };
+        auto inverse = [&]() { return m_run == -INFINITY && l_run == 0.f ? 0.f : 1.f / l_run; };     // (values 2^126 apart: infinite rather than 0)
         asm volatile("bar.sync %0, 256;" ::"r"(9 + g) : "memory");  // (also behind the last block's maxima)
         sp[half * 128 + r] = l_run;
         asm volatile("bar.sync %0, 256;" ::"r"(9 + g) : "memory");
         l_run = sp[r] + sp[128 + r];
-        bool writes_out = true;
-        if (tile_parts > 1 && group_rows > 0) {
+        bool writes_out = group_rows > 0;
+        if (tile_parts == 1) {
+            const float inv = inverse();
+#pragma unroll 1
+            for (int d0 = 0; d0 < HD; d0 += 32) {
+                float o[32];
+                result(d0, o);
+                leave(d0, o, inv);
+            }
+        } else if (group_rows > 0) {
             // leave this part's result in scratch ([d][row], so that a warp writes whole lines), then see whether the tile's other
             // parts are all there
             const size_t tile_id = (((size_t)seq * H + h) * n_tiles + qt) * GROUPS + g;
+            const float* parts = partials + tile_id * n_parts * pp_part_floats(DH);
             float* mine = partials + (tile_id * n_parts + part) * pp_part_floats(DH);
+#pragma unroll 1
+            for (int d0 = 0; d0 < HD; d0 += 32) {
+                float o[32];
+                result(d0, o);
 #pragma unroll
-            for (int d = 0; d < HD; ++d) mine[(half * HD + d) * 128 + r] = o_acc[d];
+                for (int x = 0; x < 32; ++x) mine[(half * HD + d0 + x) * 128 + r] = o[x];
+            }
             if (half == 0) {
                 mine[DH * 128 + r] = m_run;
                 mine[DH * 128 + 128 + r] = l_run;
@@ -556,42 +748,36 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             if (writes_out) {
                 __threadfence();
                 // every part in turn, this CTA's own included: the sum does not depend on who came last
-                m_run = -INFINITY; l_run = 0.f;
+                m_run = -INFINITY;
+                for (int pt = 0; pt < tile_parts; ++pt) m_run = fmaxf(m_run, __ldcg(parts + pt * pp_part_floats(DH) + DH * 128 + r));
+                auto weight = [&](int pt) {                         // (sums that are not numbers stay so)
+                    const float m_p = __ldcg(parts + pt * pp_part_floats(DH) + DH * 128 + r);
+                    return m_p == -INFINITY ? 0.f : pp_exp2(m_p - m_run);
+                };
+                l_run = 0.f;
+                for (int pt = 0; pt < tile_parts; ++pt) l_run = fmaf(__ldcg(parts + pt * pp_part_floats(DH) + DH * 128 + 128 + r), weight(pt), l_run);
+                const float inv = inverse();
+#pragma unroll 1
+                for (int d0 = 0; d0 < HD; d0 += 32) {
+                    float o[32];
 #pragma unroll
-                for (int d = 0; d < HD; ++d) o_acc[d] = 0.f;
-                for (int pt = 0; pt < tile_parts; ++pt) {
-                    const float* theirs = partials + (tile_id * n_parts + pt) * pp_part_floats(DH);
-                    const float m_p = __ldcg(theirs + DH * 128 + r), l_p = __ldcg(theirs + DH * 128 + 128 + r);
-                    const float m_new = fmaxf(m_run, m_p), use = m_new == -INFINITY ? 0.f : m_new;
-                    const float a = (m_run == -INFINITY) ? 0.f : pp_exp2(m_run - use);
-                    const float b = (m_p == -INFINITY) ? 0.f : pp_exp2(m_p - use);       // (sums that are not numbers stay so)
-                    l_run = fmaf(l_run, a, l_p * b);
-                    m_run = m_new;
+                    for (int x = 0; x < 32; ++x) o[x] = 0.f;
+#pragma unroll 1
+                    for (int pt = 0; pt < tile_parts; ++pt) {
+                        const float* theirs = parts + pt * pp_part_floats(DH) + (half * HD + d0) * 128 + r;
+                        const float w = weight(pt);
+                        float v[32];
 #pragma unroll
-                    for (int d0 = 0; d0 < HD; d0 += 16) {
-                        float v[16];
+                        for (int x = 0; x < 32; ++x) v[x] = __ldcg(theirs + x * 128);
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) v[x] = __ldcg(theirs + (half * HD + d0 + x) * 128 + r);
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) o_acc[d0 + x] = fmaf(o_acc[d0 + x], a, v[x] * b);
+                        for (int x = 0; x < 32; ++x) o[x] = fmaf(v[x], w, o[x]);
                     }
+                    leave(d0, o, inv);
                 }
             }
         }
-        if (writes_out && group_rows > 0) {
-            // the row as bfloat16, entries in order again, into shared memory (Q's tile: no MMA reads it any more); then each warp writes
-            // whole rows, so that a store instruction fills whole lines
-            const float inv = (l_run > 0.f || l_run != l_run) ? 1.f / l_run : 0.f;
-            if (ok) {
-#pragma unroll
-                for (int d = 0; d < HD; d += 8) {
-                    uint4 pk;
-                    pk.x = pack2(o_acc[d] * inv, o_acc[d + 2] * inv); pk.y = pack2(o_acc[d + 4] * inv, o_acc[d + 6] * inv);
-                    pk.z = pack2(o_acc[d + 1] * inv, o_acc[d + 3] * inv); pk.w = pack2(o_acc[d + 5] * inv, o_acc[d + 7] * inv);
-                    const int c = (half * HD + d) >> 3;
-                    *reinterpret_cast<uint4*>(q_tile + (c >> 3) * ATOM_Q + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = pk;
-                }
-            }
+        if (writes_out) {
+            // each warp writes whole rows, so that a store instruction fills whole lines
             asm volatile("bar.sync %0, 64;" ::"r"(1 + g * 4 + q) : "memory");
             if (ok) {
                 constexpr int PIECES = DH / 8, AT_ONCE = 32 / PIECES;
@@ -627,7 +813,7 @@ template <int DH, int GROUPS>
 int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
               int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_seqs, int max_new, int H, int Hkv,
               float scale, int window, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
-    const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_RING + GROUPS * 256 * 4 + 40 * 8;
+    const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_RING + GROUPS * 256 * 4 + (PP_RING / (PP_BK * DH * 2)) * (64 * 8 + 4) + 48 * 8;
     static DeviceMarks marks;
     auto kern = attn_packed_prefill_kernel<DH, GROUPS>;
     cudaError_t e = allow_shared_memory(marks, kern, smem);
