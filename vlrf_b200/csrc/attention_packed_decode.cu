@@ -1,19 +1,24 @@
 // Decode attention over a cache of keys and values in 4 bits (packed_kv.cuh): one query a row and head, bfloat16, head sizes 64, 128,
 // 192 and 256, any number of query heads to a key/value head.
 //
-// A CTA takes one row, one key/value head, up to NT · 8 of its query heads and one of n_split parts of the context; each of its warps
-// walks tiles of 64 tokens (a cache block) of its own, which arrive in a ring of stages by bulk copies: codes and pairs of a block and head
-// are contiguous.  In tensor-core products the codes are the 16-row operand as they lie in the cache, masked but not converted
-// (packed_kv.cuh), and the queries the 8 columns:
-//     Sᵀ [16 tokens × 8 queries]:  q · k_j = Σ over groups of step_j (q · c_j) + zero_j Σ q
-//     Oᵀ [16 entries × 8 queries] += c [entries × 16 tokens] · (p_j step_j) [16 tokens × queries],   and Σ p_j zero_j beside it
+// A CTA takes one row, one key/value head, up to RC (2, 4 or 8) of its query heads and one of the parts into which a long context is cut; each of
+// its warps walks tiles of 64 tokens (a cache block) of its own, which arrive in a ring of two stages by bulk copies: codes and pairs of a block and
+// head are contiguous.  In tensor-core products the codes are the 16-row operand as they lie in the cache, masked but not converted
+// (packed_kv.cuh), and the queries the 8 columns, 8 / RC sub-steps of 16 tokens side by side:
+//     Sᵀ [16 tokens × columns]:  q · k_j = Σ over groups of step_j (q · c_j) + zero_j Σ q
+//     Oᵀ [16 entries × columns] += c [entries × 16 tokens] · (p_j step_j) [16 tokens × columns],   and Σ p_j zero_j beside it
 // The order of entries inside a product is free, so each lane takes its keys' codes in pieces of eight bytes, and its values' entries
 // pairwise from two tokens' words.  Weights change from the layout of a result to that of an operand by `movmatrix`.  Weights times steps
 // are rounded to bfloat16 (each by up to 2^-8 of itself, as in the library's other bfloat16 attention); scores, sums, zeros and results stay
 // in float32, and code products are exact.  Scales that keep code · 2^-133 in float32's range: queries by 2^90 (so |q| < 2^37), weights by 2^80 (steps of
-// values below 2^47).
+// values below 2^47; a weight times a step below 2^-73 is nothing).
 //
-// The warps of a CTA merge their sums in shared memory; the parts of a context leave theirs in scratch, and the CTA that comes last merges them.
+// The warps of a CTA merge their sums in shared memory; the parts of a context leave theirs in scratch, and the CTA that comes last merges them
+// in their order.  (A cluster a context, its CTAs merging in distributed shared memory, left SMs empty: 16 CTAs of one an SM found no room together.)
+//
+// Bound by taking codes apart and by latency rather than by bytes: 131,071 tokens of 8 heads of 128 for 32 queries (151 MB) 40 us, 3.8 TB/s, with the
+// integer pipe 47 % and the tensor pipe 23 % busy; the copies alone take 31 us, the arithmetic alone 30.  16 rows of 1 to 8,116 tokens: 27 us, 2.7 TB/s;
+// 32 rows of 300 to 1,013 tokens of 25 heads of 64: 15.6 us, 2.4 TB/s; one row of 701 tokens of 12 heads: 5.3 us, a chain of latencies.
 #include "common.cuh"
 #include "packed_kv.cuh"
 
