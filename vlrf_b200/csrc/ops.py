@@ -971,7 +971,7 @@ def _packed_check(what: str, cache: PackedKV, n_kv_heads: int, head_dim: int, bl
 def kv_append_packed(qkv, k_off: int, v_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, n_tokens: int, n_kv_heads: int,
                      head_dim: int, dev_err) -> None:
     """Quantise the K and V columns of qkv rows (float32 or bfloat16; qkv may be a range of columns of wider rows) into one layer's paged
-    cache of 4 bits.  Rows with slot −1 are skipped."""
+    cache of 4 bits.  Rows with slot −1 are skipped; no two others have slot and position alike (one's codes might meet the other's steps)."""
     what = "kv_append_packed"
     _packed_check(what, cache, n_kv_heads, head_dim, block_table, (tok_slot, tok_pos), dev_err, n_tokens, (("qkv", qkv),))
     if tok_slot.shape[0] < n_tokens or tok_pos.shape[0] < n_tokens:
@@ -1087,7 +1087,8 @@ def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_
                              part_blocks: int = 6, partials=None, counters=None) -> None:
     """Causal attention of every sequence's new tokens (rows seq_start[i] … seq_start[i+1]−1 of qkv, the first of them at position
     seq_pos0[i]) over the sequence's cache of 4 bits, which already holds these tokens; bfloat16, head size 64 or 128, on the tcgen05
-    tensor cores.  n_parts > 1 deals the keys of long tiles to that many CTAs (see packed_prefill_shape) and wants float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero."""
+    tensor cores, operands float16 under powers of two.  n_parts > 1 deals the keys of long tiles to that many CTAs (see packed_prefill_shape) and wants
+    float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero."""
     what = "attention_prefill_packed"
     _attention_packed_check(what, qkv, q_off, cache, block_table, (seq_slot, seq_start, seq_pos0), out, n_tokens, n_heads, n_kv_heads, head_dim, window,
                             dev_err)
