@@ -362,6 +362,17 @@ def test_prompt_attention_on_the_tensor_cores(heads, kv_heads, dim, new, past, w
     check_prompt(prefill(pages, new, heads, kv_heads, dim, window, groups, n_parts), pages, new, heads, kv_heads, dim, window)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 1, 64), (2, 2, 128)])
+@pytest.mark.parametrize("new,past", [([1, 1, 1, 300, 1, 2, 1, 1, 1], [5, 70, 0, 100, 64, 3, 200, 63, 9]), ([1] * 33 + [270, 3, 130] + [1] * 4, list(range(40))),
+                                      ([0, 400, 0, 0, 0, 1, 0, 0, 0], [3, 0, 1, 64, 0, 127, 0, 5, 0])])
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("groups,n_parts", [(1, 1), (2, 1), (2, 3)])
+def test_prompt_attention_of_one_long_sequence_among_single_tokens(heads, kv_heads, dim, new, past, window, groups, n_parts):
+    """More sequences than tiles of the longest: the grid has a place a tile."""
+    pages = Pages([a + b for a, b in zip(new, past)], kv_heads, dim, seed=heads + len(new))
+    check_prompt(prefill(pages, new, heads, kv_heads, dim, window, groups, n_parts), pages, new, heads, kv_heads, dim, window)
+
+
 def check_prompt(fn, pages, new, heads, kv_heads, dim, window):
     """A sample of the tokens against float64.  A number of a key or a value is off by h = 2^-11 of itself, and, where it lies below float16's normal range (2^-14
     of its first block's, or 2^-28 of its own row's largest), by less than that of the largest; so by 2 h of the largest at the very most.  That moves a score by
@@ -381,7 +392,7 @@ def check_prompt(fn, pages, new, heads, kv_heads, dim, window):
     for i, a in enumerate(new):
         s = sum(new[:i])
         edges |= {s, s + a - 1} | {s + x for x in (1, 63, 64, 127, 128, 129, 255, 256) if x < a}
-    for t in sorted(edges | set(range(0, T, 37))):
+    for t in sorted((edges | set(range(0, T, 37))) & set(range(T))):        # (a sequence that brings nothing has no rows)
         i, p = slot[t], pos[t]
         k, v = contexts[i]
         first = max(0, p - window + 1) if window else 0

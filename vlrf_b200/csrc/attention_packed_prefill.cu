@@ -132,7 +132,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                            const unsigned char* __restrict__ Vq, const uint32_t* __restrict__ Vp, int n_blocks, const int* __restrict__ block_table,
                            int max_blocks, const int* __restrict__ seq_slot, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
                            __nv_bfloat16* __restrict__ out, int ld_out, int H, int Hkv, float scale, int window, int n_parts, int part_blocks, float* __restrict__ partials,
-                           int* __restrict__ counters, int n_tiles, int* __restrict__ dev_err) {
+                           int* __restrict__ counters, int n_tiles, int n_seqs, int n_flat, int* __restrict__ dev_err) {
     constexpr int BK = PP_BK, PP_TILE = BK * DH * 2, PP_SLOTS = PP_RING / PP_TILE, ROWS = GROUPS * 128, NG = DH / 64, NPROD = pp_producers(GROUPS), SOFT = GROUPS * 8;
     constexpr int Q_BYTES = 128 * DH * 2, ATOM_Q = 16384, ATOM_KV = BK * 128;    // a 64-number chunk of 128 queries / of a block
     constexpr int NP = BK + DH + BK <= 256 ? 2 : 1;                 // buffers of P that a group's 256 columns have room for
@@ -162,8 +162,6 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     int* s_last = reinterpret_cast<int*>(s_unit + 2);                                        // [GROUPS]: whether this CTA merges its tile's parts
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // z is the slowest index of the order in which CTAs are started: first parts first, and within a part long tiles first
-    const int part = blockIdx.z / n_tiles, qt = n_tiles - 1 - blockIdx.z % n_tiles, seq = blockIdx.y, h = blockIdx.x;
     if (threadIdx.x == 0) {
         for (int i = 0; i < PP_SLOTS; ++i) { tbar_init(&full[i], NPROD); tbar_init(&empty[i], GROUPS); }
         for (int g = 0; g < GROUPS; ++g) {
@@ -183,6 +181,38 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
+    // z is the slowest index of the order in which CTAs are started: first parts first, and within a part long tiles first
+    const int h = blockIdx.x;
+    int part, qt, seq;
+    if (n_flat == 0) {
+        part = blockIdx.z / n_tiles;
+        qt = n_tiles - 1 - blockIdx.z % n_tiles;
+        seq = blockIdx.y;
+    } else {
+        // sequences of very unequal numbers of new tokens: the grid has as many places as their tiles can need, and place f is the f-th tile there is
+        part = blockIdx.z / n_flat;
+        int f = blockIdx.z % n_flat;
+        seq = -1;
+        qt = 0;
+        for (int s0 = 0; s0 < n_seqs && seq < 0; s0 += 32) {        // (every warp looks; the answer is the same)
+            const int s = s0 + lane, tiles = s < n_seqs ? min((max(seq_start[s + 1] - seq_start[s], 0) + ROWS - 1) / ROWS, n_tiles) : 0;
+            int upto = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int from = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += from;
+            }
+            const uint32_t behind = __ballot_sync(0xffffffffu, f < upto);
+            if (behind != 0u) {
+                const int l = __ffs(behind) - 1;
+                seq = s0 + l;
+                qt = __shfl_sync(0xffffffffu, upto, l) - 1 - f;     // (its long tiles first)
+            } else {
+                f -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        if (seq < 0) return;                                        // (more places than tiles; uniform over the CTA)
+    }
     const int row0 = seq_start[seq], n_new = seq_start[seq + 1] - row0, slot = seq_slot[seq], pos0 = seq_pos0[seq];
     const int hk = h / (H / Hkv);
     const int t_first = qt * ROWS, q_first = pos0 + t_first;        // the tile's first query, in the step and in the sequence
@@ -811,18 +841,25 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
 
 template <int DH, int GROUPS>
 int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
-              int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_seqs, int max_new, int H, int Hkv,
-              float scale, int window, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+              int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_tokens, int n_seqs, int max_new, int H,
+              int Hkv, float scale, int window, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
     const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_RING + GROUPS * 256 * 4 + (PP_RING / (PP_BK * DH * 2)) * (64 * 8 + 4) + 48 * 8;
     static DeviceMarks marks;
     auto kern = attn_packed_prefill_kernel<DH, GROUPS>;
     cudaError_t e = allow_shared_memory(marks, kern, smem);
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_prefill: %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     const long long tiles = (max_new + GROUPS * 128 - 1) / (GROUPS * 128);
-    VLRF_REQUIRE(tiles * n_parts <= 65535, "attn_packed_prefill: %lld tiles of %d parts are too many for one launch", tiles, n_parts);
-    e = launch_chained(kern, dim3(H, n_seqs, (unsigned)(tiles * n_parts)), dim3(pp_threads(GROUPS)), smem, stream, (const __nv_bfloat16*)qkv, ld, q_off,
+    // A place a tile that there can be (⌈len / rows⌉ over the sequences), where that is less than half of the longest sequence's tiles for every sequence: a
+    // CTA that finds nothing to do takes an SM's place for a microsecond, and one that looks its tile up starts half a microsecond later
+    // (five sequences of 1 to 640 tokens, 25 heads: 25.4 us, so 24.0; behind 60 single tokens 1,000: 118, so 108).
+    const long long flat = n_tokens / (GROUPS * 128) + n_seqs;
+    const bool use_flat = 2 * flat < tiles * n_seqs && flat * n_parts <= 65535;
+    VLRF_REQUIRE(use_flat || tiles * n_parts <= 65535, "attn_packed_prefill: %lld tiles of %d parts are too many for one launch", tiles, n_parts);
+    const dim3 grid(H, use_flat ? 1 : n_seqs, (unsigned)((use_flat ? flat : tiles) * n_parts));
+    e = launch_chained(kern, grid, dim3(pp_threads(GROUPS)), smem, stream, (const __nv_bfloat16*)qkv, ld, q_off,
                        (const unsigned char*)Kq, (const uint32_t*)Kp, (const unsigned char*)Vq, (const uint32_t*)Vp, n_blocks, block_table, max_blocks, seq_slot,
-                       seq_start, seq_pos0, (__nv_bfloat16*)out, ld_out, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, (int)tiles, dev_err);
+                       seq_start, seq_pos0, (__nv_bfloat16*)out, ld_out, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, (int)tiles, n_seqs,
+                       use_flat ? (int)flat : 0, dev_err);
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_prefill: %s", cudaGetErrorString(e));
     return vlrf_check_launch("attn_packed_prefill");
 }
@@ -844,11 +881,11 @@ extern "C" int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, 
 
 extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                                         const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out,
-                                        int ld_out, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int groups, int n_parts,
-                                        int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+                                        int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int groups,
+                                        int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
     VLRF_REQUIRE(vlrf_attn_packed_prefill_takes(H, Hkv, dh, BT, ld, q_off, ld_out),
                  "attn_packed_prefill: %d heads over %d of %d, blocks of %d, row strides %d and %d are not taken", H, Hkv, dh, BT, ld, ld_out);
-    VLRF_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && max_new >= 0 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && dev_err != nullptr,
+    VLRF_REQUIRE(n_tokens >= 0 && n_seqs >= 0 && n_seqs <= 65535 && max_new >= 0 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && dev_err != nullptr,
                  "attn_packed_prefill: bad arguments");
     VLRF_REQUIRE(scale >= 0.f, "attn_packed_prefill: a scale of %g is negative", (double)scale);       // (a row's maximum is taken of the raw scores)
     VLRF_REQUIRE(groups == 1 || groups == 2, "attn_packed_prefill: %d groups of 128 queries a CTA (1 or 2)", groups);
@@ -857,8 +894,8 @@ extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, cons
     for (const void* p : {qkv, Kq, Kp, Vq, Vp, (const void*)out})
         VLRF_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "attn_packed_prefill: tensors begin on 16 bytes");
     if (n_seqs == 0 || max_new == 0) return VLRF_OK;
-#define GO(DH, G) pp_launch<DH, G>(qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, seq_slot, seq_start, seq_pos0, out, ld_out, n_seqs, \
-                                   max_new, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, dev_err, stream)
+#define GO(DH, G) pp_launch<DH, G>(qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, seq_slot, seq_start, seq_pos0, out, ld_out, n_tokens, \
+                                   n_seqs, max_new, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, dev_err, stream)
     if (dh == 64) return groups == 1 ? GO(64, 1) : GO(64, 2);
     return groups == 1 ? GO(128, 1) : GO(128, 2);
 #undef GO

@@ -1044,9 +1044,9 @@ PACKED_PROMPT_US = dict(cta=(4.5, 5.5), block={64: 1.05, 128: 1.45}, meet=5.0)
 def packed_prefill_shape(lens, pos0, n_heads: int, head_dim: int, window: int = 0) -> tuple:
     """(groups of 128 queries a CTA of `attention_prefill_packed` takes, most CTAs to which it deals the keys of a tile, blocks of 64 that each of those
     holds at least) for sequences that bring lens[i] tokens behind pos0[i].  Two groups share the keys that a CTA takes apart; one makes twice the CTAs,
-    two an SM, which pays for small heads and few tokens (one prompt of 200 tokens of 12 heads of 64: 8.1 us against 9.5; four of 1,000 behind 4,000: 176
-    against 163).  A tile's blocks are a chain: parts shorten it where the tiles leave SMs idle (512 tokens of 32 heads of 128 behind 7,500: 172 us whole, 102
-    in two parts, 140 in three, which come in two waves)."""
+    two an SM, which pays for small heads and few tokens (one prompt of 200 tokens of 12 heads of 64: 10.2 us against 11.3; four of 1,000 behind 4,000: 204
+    against 172).  A tile's blocks are a chain: parts shorten it where the tiles leave SMs idle (512 tokens of 32 heads of 128 behind 7,500: 206 us whole, 119
+    in two parts, 163 in three, which come in two waves)."""
     return _packed_prefill_shape(tuple(lens), tuple(pos0), n_heads, head_dim, window)
 
 
@@ -1098,7 +1098,7 @@ def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_
     if n_parts > 1:
         scratch = _packed_scratch(what, packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts), partials, counters)
     call("vlrf_attn_packed_prefill", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], seq_slot.data_ptr(),
-         seq_start.data_ptr(), seq_pos0.data_ptr(), out.data_ptr(), out.stride(0), n_seqs, max_new, n_heads, n_kv_heads, head_dim, cache.block_tokens,
+         seq_start.data_ptr(), seq_pos0.data_ptr(), out.data_ptr(), out.stride(0), n_tokens, n_seqs, max_new, n_heads, n_kv_heads, head_dim, cache.block_tokens,
          float(scale), window, groups, n_parts, part_blocks, *scratch, dev_err.data_ptr(), _stream())
 
 
