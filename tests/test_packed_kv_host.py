@@ -72,13 +72,13 @@ def test_decode_attention_refuses(change):
     lib = library()
     a = dict(dict(rows=3, H=4, Hkv=2, dh=64, BT=64, max_blocks=4, window=0, n_split=1, part_tiles=1, ld=512, q_off=0, ld_out=256, qkv=4096,
                   dev_err=ctypes.c_void_p(4096)), **change)
-    assert lib.vlrf_attn_packed_decode(ctypes.c_void_p(a["qkv"]), a["ld"], a["q_off"], *pointers(4), 10, *pointers(1), a["max_blocks"], *pointers(3),
+    assert lib.vlrf_attn_packed_decode(ctypes.c_void_p(a["qkv"]), a["ld"], a["q_off"], *pointers(4), 10, *pointers(1), a["max_blocks"], *pointers(2), None, *pointers(1),
                                        a["ld_out"], a["rows"], a["H"], a["Hkv"], a["dh"], a["BT"], 0.125, a["window"], 0, a["n_split"], a["part_tiles"], None, None, a["dev_err"],
                                        None) != 0
     assert b"attn_packed_decode" in lib.vlrf_last_error()
 
 
-@pytest.mark.parametrize("change", [dict(dh=32), dict(dh=192), dict(n_seqs=-1), dict(n_seqs=70000), dict(max_new=-1), dict(H=3), dict(BT=32), dict(n_tokens=-1),
+@pytest.mark.parametrize("change", [dict(dh=32), dict(dh=192), dict(n_seqs=-1), dict(n_seqs=70000), dict(max_new=-1), dict(H=3), dict(BT=32), dict(n_tokens=-1), dict(least_new=0),
                                     dict(max_blocks=0), dict(window=-1), dict(dev_err=None), dict(n_parts=0), dict(n_parts=17), dict(n_parts=2),
                                     dict(groups=0), dict(groups=3), dict(part_blocks=0), dict(scale=-1.0), dict(ld=385), dict(q_off=4), dict(ld_out=130), dict(qkv=4100),
                                     dict(max_new=2 ** 24)])
@@ -89,7 +89,7 @@ def test_prompt_attention_refuses(change):
                   dev_err=ctypes.c_void_p(4096)), **change)
     assert lib.vlrf_attn_packed_prefill(ctypes.c_void_p(a["qkv"]), a["ld"], a["q_off"], *pointers(4), 10, *pointers(1), a["max_blocks"], *pointers(4),
                                         a["ld_out"], a.get("n_tokens", abs(a["n_seqs"] * a["max_new"]) % 2 ** 31), a["n_seqs"], a["max_new"], a["H"], a["Hkv"], a["dh"], a["BT"],
-                                        a["scale"], a["window"], a["groups"],
+                                        a["scale"], a["window"], a.get("least_new", 1), a["groups"],
                                         a["n_parts"], a["part_blocks"], None, None, a["dev_err"], None) != 0
     assert b"attn_packed_prefill" in lib.vlrf_last_error()
 

@@ -38,10 +38,10 @@ def run_step(cache, table, rows, out, ctx, H, G, d, scale=None, window=0):
     ops.attention_packed_step(rows, 0, cache, table, out, ctx, H, G, d, 1 / math.sqrt(d) if scale is None else scale, window)
 
 
-def check_against_float64(all_rows, got, at, H, G, d, scale, window=0):
+def check_against_float64(all_rows, got, at, H, G, d, scale, window=0, held=None):
     """got[i] is the attention of the row at position at[i] over all rows up to it; bounds as for bfloat16 weights times steps and a bfloat16 result, scores
-    in float32 or of float16 operands (off by 2^-10 of Σ |q| |k|max at most)."""
-    k, v = [plain.values(*plain.quantise(all_rows[:, c:c + G * d], d)) for c in (H * d, (H + G) * d)]
+    in float32 or of float16 operands (off by 2^-10 of Σ |q| |k|max at most).  held: what the cache holds, where it is known (else the rows, quantised)."""
+    k, v = held or [plain.values(*plain.quantise(all_rows[:, c:c + G * d], d)) for c in (H * d, (H + G) * d)]
     for i, p in enumerate(at):
         q = all_rows[p, :H * d].double().view(H, d)
         want = plain.attend(q, k, v, scale, window, p)
@@ -106,6 +106,55 @@ def test_offsets_past_32_bits(n_new):
     check = [0, 64, past - 1, past, past + n_new - 1]
     check_against_float64(rows, out[check], check, H, G, d, 1 / math.sqrt(d))
     assert int(cache.k[n_blocks - 1].any()) and not int(cache.k[6:n_blocks - 2].any())
+
+
+@pytest.mark.parametrize("H,G,d", [(25, 25, 64), (32, 4, 128)])
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("new", [[1] * 9 + [150], [70, 1, 0, 1, 1, 130, 1, 1, 1, 1], [3, 1, 1, 1, 1, 1, 1, 1]])
+def test_single_tokens_among_prompts_go_to_the_decode_kernel(H, G, d, window, new, monkeypatch):
+    """Many single tokens with long contexts: two kernels share the step, no row is left out or written by the wrong one."""
+    from vlrf_b200.csrc import ops
+    past = [(97 * i + 460) % 900 for i in range(len(new))]
+    seen = []
+    for name in ("attention_decode_packed", "attention_prefill_packed"):
+        inner = getattr(ops, name)
+        monkeypatch.setattr(ops, name, lambda *a, inner=inner, name=name, **kw: (seen.append(name), inner(*a, **kw)) and None)
+    cache, table = cache_for(1100, G, d, len(new))
+    whole, ws = [], Workspace(DEV)
+    for i, (a, b) in enumerate(zip(new, past)):            # the contexts, sequence by sequence
+        whole.append(qkv_rows(a + b, H, G, d, seed=i))
+        if b:
+            ctx = step_of([b], [0], slots=[i])
+            ops.kv_append_packed(whole[i][:b].to(DEV), H * d, (H + G) * d, cache, table, ctx.tok_slot, ctx.tok_pos, b, G, d, ctx.dev_err)
+    out = torch.full((sum(new) + 2, H * d), 3.0, dtype=torch.bfloat16, device=DEV)
+    ctx = step_of(new, past, ws)
+    run_step(cache, table, torch.cat([w[b:] for w, b in zip(whole, past)]).to(DEV), out[:sum(new)], ctx, H, G, d, window=window)
+    assert int(ctx.dev_err.item()) == 0 and bool((out[sum(new):] == 3).all()) and seen == ["attention_prefill_packed", "attention_decode_packed"]
+    at, host, blocks = 0, {n: getattr(cache, n).cpu() for n in ("k", "k_pairs", "v", "v_pairs")}, table.cpu().long()
+    for i, (w, a, b) in enumerate(zip(whole, new, past)):
+        if a:
+            place = torch.arange(a + b)
+            held = [plain.unpacked(host[n][blocks[i, place // 64], :, place % 64], host[n + "_pairs"][blocks[i, place // 64], :, place % 64]) for n in ("k", "v")]
+            check_against_float64(w, out[[at, at + a - 1]], [b, b + a - 1], H, G, d, 1 / math.sqrt(d), window, held)
+        at += a
+    # the same step in one kernel is no further off than the two may be from one another
+    monkeypatch.setattr(ops, "PACKED_SINGLES_APART", 10 ** 9)
+    alone = torch.zeros_like(out)
+    run_step(cache, table, torch.cat([w[b:] for w, b in zip(whole, past)]).to(DEV), alone[:sum(new)], step_of(new, past), H, G, d, window=window)
+    at = 0
+    for a in new:
+        if a != 1:
+            assert torch.equal(alone[at:at + a], out[at:at + a]) or float((alone[at:at + a] - out[at:at + a]).abs().max()) <= 2 * HALF_STEP * float(out.abs().max())
+        at += a
+
+
+def test_rows_of_entries_are_checked():
+    from vlrf_b200.csrc import KernelError, ops
+    cache, table = cache_for(64, 2, 64)
+    rows, out = qkv_rows(3, 2, 2, 64).to(DEV), torch.zeros((3, 128), dtype=torch.bfloat16, device=DEV)
+    for row_of in (ints([0, 1, 2]), torch.tensor([0, 1, 2, 3], device=DEV)):            # too few; int64
+        with pytest.raises(KernelError):
+            ops.attention_decode_packed(rows, 0, cache, table, ints([0, 0, 0]), ints([0, 1, 2]), out, 3, 2, 2, 64, 0.125, 0, (False, 1, 1), ints([0]), row_of=row_of)
 
 
 @pytest.mark.parametrize("new,past", [([1, 1, 1], [700, 3, 300]), ([90, 1, 300], [700, 64, 0])])

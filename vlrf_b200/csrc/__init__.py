@@ -199,13 +199,13 @@ _SIGNATURES = {
                          _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p, _c_void_p],
     "vlrf_attn_packed_decode_takes": [_c_int] * 7,
     "vlrf_attn_packed_decode_scratch": [_c_int] * 5 + [ctypes.POINTER(ctypes.c_longlong)] * 2,
-    "vlrf_attn_packed_decode": [_c_void_p, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int,
+    "vlrf_attn_packed_decode": [_c_void_p, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int,
                                 _c_int, _c_int, _c_int, _c_int, _c_int, _c_float] + [_c_int] * 4 + [_c_void_p] * 4,
     "vlrf_attn_packed_prefill_takes": [_c_int] * 7,
     "vlrf_attn_packed_prefill_max_parts": [],
     "vlrf_attn_packed_prefill_scratch": [_c_int] * 6 + [ctypes.POINTER(ctypes.c_longlong)] * 2,
     "vlrf_attn_packed_prefill": [_c_void_p, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 8
-                                + [_c_float] + [_c_int] * 4 + [_c_void_p] * 4,
+                                + [_c_float] + [_c_int] * 5 + [_c_void_p] * 4,
     "vlrf_moe_route": [_c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                        _c_void_p, _c_int, _c_void_p],
     "vlrf_moe_route_scored": [_c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p,

@@ -80,7 +80,7 @@ template <int NG, int RC, bool FEW>
 __global__ void __launch_bounds__(pd_warps(NG, FEW) * 32, pd_ctas(NG, FEW))
 attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_off, const unsigned char* __restrict__ Kq, const unsigned char* __restrict__ Kp,
                           const unsigned char* __restrict__ Vq, const unsigned char* __restrict__ Vp, int n_blocks, const int* __restrict__ block_table,
-                          int max_blocks, const int* __restrict__ tok_slot, const int* __restrict__ tok_pos, __nv_bfloat16* __restrict__ out, int ld_out, int R,
+                          int max_blocks, const int* __restrict__ tok_slot, const int* __restrict__ tok_pos, const int* __restrict__ row_of, __nv_bfloat16* __restrict__ out, int ld_out, int R,
                           int Hkv, int q_tiles, float scale, int window, int part_tiles, float* __restrict__ partials, int* __restrict__ counters, int* __restrict__ dev_err) {
     constexpr int DH = NG * 64, WARPS = pd_warps(NG, FEW), ST = PD_STAGES, CODES = pd_tile_codes(NG), PAIRS = pd_tile_pairs(NG), BYTES = pd_tile_bytes(NG);
     constexpr int CP = 8 / RC, NP = 4 / CP;                         // sub-steps side by side; products one after another for a tile's four sub-steps
@@ -106,7 +106,9 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
     const bool small = gridDim.x * gridDim.y * gridDim.z <= 64u;
     if (small) pdl_launch_dependents();
     const int slot = tok_slot[row], pos = tok_pos[row];
-    if (slot < 0) return;                                           // padding
+    // (with row_of, an entry stands for the rows row_of[i] … row_of[i + 1] − 1, and only those of one row are looked at)
+    const int at_row = row_of == nullptr ? row : row_of[row];
+    if (slot < 0 || (row_of != nullptr && row_of[row + 1] - at_row != 1)) return;            // padding
     const int first = window > 0 ? max(0, pos - window + 1) : 0;
     const int tile0 = first / PD_TOKENS, n_tiles = pos >= 0 ? pos / PD_TOKENS - tile0 + 1 : 0;
     // a context takes as many parts as it needs for at most part_tiles tiles each (a longer one than was said: all there are), about equally long
@@ -161,7 +163,7 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             float e[8];
-            const __nv_bfloat16* src = qkv + (size_t)row * ld + q_off + (size_t)(hk * R + q0 + qi) * DH + a * 64 + (2 * t + w) * 8;
+            const __nv_bfloat16* src = qkv + (size_t)at_row * ld + q_off + (size_t)(hk * R + q0 + qi) * DH + a * 64 + (2 * t + w) * 8;
             if (qi < n_q) {
                 const uint4 v = *reinterpret_cast<const uint4*>(src);
                 const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -365,7 +367,7 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
             }
         if (parts == 1) {
             const float inv = (L > 0.f || L != L) ? 1.f / L : 0.f;
-            *reinterpret_cast<uint2*>(out + (size_t)row * ld_out + (size_t)(hk * R + q0 + qi) * DH + c4 * 4) =
+            *reinterpret_cast<uint2*>(out + (size_t)at_row * ld_out + (size_t)(hk * R + q0 + qi) * DH + c4 * 4) =
                 make_uint2(pd_pack(acc.x * inv, acc.y * inv), pd_pack(acc.z * inv, acc.w * inv));
         } else {
             float* mine = my_parts + (size_t)(part * RC + qi) * (DH + 4);
@@ -424,14 +426,14 @@ attn_packed_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_o
             acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
         }
         const float inv = (L > 0.f || L != L) ? 1.f / L : 0.f;
-        *reinterpret_cast<uint2*>(out + (size_t)row * ld_out + (size_t)(hk * R + q0 + i4 / (DH / 4)) * DH + i4 % (DH / 4) * 4) =
+        *reinterpret_cast<uint2*>(out + (size_t)at_row * ld_out + (size_t)(hk * R + q0 + i4 / (DH / 4)) * DH + i4 % (DH / 4) * 4) =
             make_uint2(pd_pack(acc.x * inv, acc.y * inv), pd_pack(acc.z * inv, acc.w * inv));
     }
 }
 
 template <int NG, int RC, bool FEW>
 int pd_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
-              int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows, int H, int Hkv, float scale, int window, int n_split, int part_tiles,
+              int max_blocks, const int* tok_slot, const int* tok_pos, const int* row_of, void* out, int ld_out, int rows, int H, int Hkv, float scale, int window, int n_split, int part_tiles,
               float* partials, int* counters, int* dev_err, cudaStream_t stream) {
     const int R = H / Hkv, q_tiles = (R + RC - 1) / RC;
     constexpr size_t smem = pd_smem(NG, FEW);
@@ -443,7 +445,7 @@ int pd_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_decode: %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
     e = launch_chained(kern, dim3(Hkv * q_tiles, rows, n_split), dim3(pd_warps(NG, FEW) * 32), smem, stream, (const __nv_bfloat16*)qkv, ld, q_off,
                        (const unsigned char*)Kq, (const unsigned char*)Kp, (const unsigned char*)Vq, (const unsigned char*)Vp, n_blocks, block_table, max_blocks,
-                       tok_slot, tok_pos, (__nv_bfloat16*)out, ld_out, R, Hkv, q_tiles, scale, window, part_tiles, partials, counters, dev_err);
+                       tok_slot, tok_pos, row_of, (__nv_bfloat16*)out, ld_out, R, Hkv, q_tiles, scale, window, part_tiles, partials, counters, dev_err);
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_decode: %s", cudaGetErrorString(e));
     return vlrf_check_launch("attn_packed_decode");
 }
@@ -466,8 +468,8 @@ extern "C" int vlrf_attn_packed_decode_scratch(int rows, int H, int Hkv, int dh,
 }
 
 extern "C" int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
-                                       const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows,
-                                       int H, int Hkv, int dh, int BT, float scale, int window, int few, int n_split, int part_tiles, float* partials,
+                                       const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, const int* row_of, void* out,
+                                       int ld_out, int rows, int H, int Hkv, int dh, int BT, float scale, int window, int few, int n_split, int part_tiles, float* partials,
                                        int* counters, int* dev_err, cudaStream_t stream) {
     VLRF_REQUIRE(vlrf_attn_packed_decode_takes(H, Hkv, dh, BT, ld, q_off, ld_out),
                  "attn_packed_decode: %d heads over %d of %d, blocks of %d, row strides %d and %d are not taken", H, Hkv, dh, BT, ld, ld_out);
@@ -479,7 +481,7 @@ extern "C" int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const
     if (rows == 0) return VLRF_OK;
     const int R = H / Hkv, RC = pd_columns(dh, R);
 #define GO(NG, C) (few ? pd_launch<NG, C, true>(ARGS) : pd_launch<NG, C, false>(ARGS))
-#define ARGS qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, tok_slot, tok_pos, out, ld_out, rows, H, Hkv, scale, window, n_split, part_tiles, \
+#define ARGS qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, tok_slot, tok_pos, row_of, out, ld_out, rows, H, Hkv, scale, window, n_split, part_tiles, \
              partials, counters, dev_err, stream
     if (dh == 64) return RC == 2 ? GO(1, 2) : RC == 4 ? GO(1, 4) : GO(1, 8);
     if (dh == 128) return RC == 2 ? GO(2, 2) : RC == 4 ? GO(2, 4) : GO(2, 8);

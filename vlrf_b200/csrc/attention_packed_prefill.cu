@@ -132,7 +132,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                            const unsigned char* __restrict__ Vq, const uint32_t* __restrict__ Vp, int n_blocks, const int* __restrict__ block_table,
                            int max_blocks, const int* __restrict__ seq_slot, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
                            __nv_bfloat16* __restrict__ out, int ld_out, int H, int Hkv, float scale, int window, int n_parts, int part_blocks, float* __restrict__ partials,
-                           int* __restrict__ counters, int n_tiles, int n_seqs, int n_flat, int* __restrict__ dev_err) {
+                           int* __restrict__ counters, int n_tiles, int n_seqs, int n_flat, int least_new, int* __restrict__ dev_err) {
     constexpr int BK = PP_BK, PP_TILE = BK * DH * 2, PP_SLOTS = PP_RING / PP_TILE, ROWS = GROUPS * 128, NG = DH / 64, NPROD = pp_producers(GROUPS), SOFT = GROUPS * 8;
     constexpr int Q_BYTES = 128 * DH * 2, ATOM_Q = 16384, ATOM_KV = BK * 128;    // a 64-number chunk of 128 queries / of a block
     constexpr int NP = BK + DH + BK <= 256 ? 2 : 1;                 // buffers of P that a group's 256 columns have room for
@@ -195,7 +195,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         seq = -1;
         qt = 0;
         for (int s0 = 0; s0 < n_seqs && seq < 0; s0 += 32) {        // (every warp looks; the answer is the same)
-            const int s = s0 + lane, tiles = s < n_seqs ? min((max(seq_start[s + 1] - seq_start[s], 0) + ROWS - 1) / ROWS, n_tiles) : 0;
+            const int s = s0 + lane, len = s < n_seqs ? seq_start[s + 1] - seq_start[s] : 0, tiles = len >= least_new ? min((len + ROWS - 1) / ROWS, n_tiles) : 0;
             int upto = tiles;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -221,7 +221,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     const int kb_first = first_key / BK, n_kb = q_last / BK - kb_first + 1;
     // the tile's key blocks are dealt to tile_parts CTAs, of part_blocks each or more; the others of its n_parts have nothing to do
     const int tile_parts = max(1, min(n_parts, (n_kb + part_blocks - 1) / part_blocks));
-    const bool active = n_rows > 0 && slot >= 0 && pos0 >= 0 && part < tile_parts;      // uniform over the CTA
+    const bool active = n_rows > 0 && n_new >= least_new && slot >= 0 && pos0 >= 0 && part < tile_parts;      // uniform over the CTA
     if (!active) return;                                            // (before it holds anything)
     constexpr uint32_t TMEM_COLS = 256 * GROUPS;                    // a group: S BK columns, O DH, P NP times BK / 2 (two bfloat16 a column)
     if (warp == SOFT) {
@@ -842,7 +842,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
 template <int DH, int GROUPS>
 int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
               int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_tokens, int n_seqs, int max_new, int H,
-              int Hkv, float scale, int window, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+              int Hkv, float scale, int window, int least_new, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
     const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_RING + GROUPS * 256 * 4 + (PP_RING / (PP_BK * DH * 2)) * (64 * 8 + 4) + 48 * 8;
     static DeviceMarks marks;
     auto kern = attn_packed_prefill_kernel<DH, GROUPS>;
@@ -851,7 +851,7 @@ int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp
     const long long tiles = (max_new + GROUPS * 128 - 1) / (GROUPS * 128);
     // A place a tile that there can be (⌈len / rows⌉ over the sequences), where that is less than half of the longest sequence's tiles for every sequence: a
     // CTA that finds nothing to do takes an SM's place for a microsecond, and one that looks its tile up starts half a microsecond later
-    // (five sequences of 1 to 640 tokens, 25 heads: 25.4 us, so 24.0; behind 60 single tokens 1,000: 118, so 108).
+    // (five sequences of 1 to 640 tokens, 25 heads of 64, window 256: 25.4 us, so 24.0).
     const long long flat = n_tokens / (GROUPS * 128) + n_seqs;
     const bool use_flat = 2 * flat < tiles * n_seqs && flat * n_parts <= 65535;
     VLRF_REQUIRE(use_flat || tiles * n_parts <= 65535, "attn_packed_prefill: %lld tiles of %d parts are too many for one launch", tiles, n_parts);
@@ -859,7 +859,7 @@ int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp
     e = launch_chained(kern, grid, dim3(pp_threads(GROUPS)), smem, stream, (const __nv_bfloat16*)qkv, ld, q_off,
                        (const unsigned char*)Kq, (const uint32_t*)Kp, (const unsigned char*)Vq, (const uint32_t*)Vp, n_blocks, block_table, max_blocks, seq_slot,
                        seq_start, seq_pos0, (__nv_bfloat16*)out, ld_out, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, (int)tiles, n_seqs,
-                       use_flat ? (int)flat : 0, dev_err);
+                       use_flat ? (int)flat : 0, least_new, dev_err);
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_prefill: %s", cudaGetErrorString(e));
     return vlrf_check_launch("attn_packed_prefill");
 }
@@ -881,11 +881,12 @@ extern "C" int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, 
 
 extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                                         const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out,
-                                        int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int groups,
-                                        int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+                                        int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int least_new,
+                                        int groups, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
     VLRF_REQUIRE(vlrf_attn_packed_prefill_takes(H, Hkv, dh, BT, ld, q_off, ld_out),
                  "attn_packed_prefill: %d heads over %d of %d, blocks of %d, row strides %d and %d are not taken", H, Hkv, dh, BT, ld, ld_out);
-    VLRF_REQUIRE(n_tokens >= 0 && n_seqs >= 0 && n_seqs <= 65535 && max_new >= 0 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && dev_err != nullptr,
+    VLRF_REQUIRE(n_tokens >= 0 && n_seqs >= 0 && n_seqs <= 65535 && max_new >= 0 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && least_new >= 1 &&
+                     dev_err != nullptr,
                  "attn_packed_prefill: bad arguments");
     VLRF_REQUIRE(scale >= 0.f, "attn_packed_prefill: a scale of %g is negative", (double)scale);       // (a row's maximum is taken of the raw scores)
     VLRF_REQUIRE(groups == 1 || groups == 2, "attn_packed_prefill: %d groups of 128 queries a CTA (1 or 2)", groups);
@@ -895,7 +896,7 @@ extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, cons
         VLRF_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "attn_packed_prefill: tensors begin on 16 bytes");
     if (n_seqs == 0 || max_new == 0) return VLRF_OK;
 #define GO(DH, G) pp_launch<DH, G>(qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, seq_slot, seq_start, seq_pos0, out, ld_out, n_tokens, \
-                                   n_seqs, max_new, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, dev_err, stream)
+                                   n_seqs, max_new, H, Hkv, scale, window, least_new, n_parts, part_blocks, partials, counters, dev_err, stream)
     if (dh == 64) return groups == 1 ? GO(64, 1) : GO(64, 2);
     return groups == 1 ? GO(128, 1) : GO(128, 2);
 #undef GO

@@ -1084,11 +1084,12 @@ def _packed_prefill_shape(lens: tuple, pos0: tuple, n_heads: int, head_dim: int,
 
 def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_slot, seq_start, seq_pos0, out, n_tokens: int, n_seqs: int, max_new: int,
                              n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int, dev_err, groups: int = 1, n_parts: int = 1,
-                             part_blocks: int = 6, partials=None, counters=None) -> None:
+                             part_blocks: int = 6, partials=None, counters=None, least_new: int = 1) -> None:
     """Causal attention of every sequence's new tokens (rows seq_start[i] … seq_start[i+1]−1 of qkv, the first of them at position
     seq_pos0[i]) over the sequence's cache of 4 bits, which already holds these tokens; bfloat16, head size 64 or 128, on the tcgen05
     tensor cores, operands float16 under powers of two.  n_parts > 1 deals the keys of long tiles to that many CTAs (see packed_prefill_shape) and wants
-    float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero."""
+    float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero.  Sequences that bring fewer than least_new
+    tokens are skipped."""
     what = "attention_prefill_packed"
     _attention_packed_check(what, qkv, q_off, cache, block_table, (seq_slot, seq_start, seq_pos0), out, n_tokens, n_heads, n_kv_heads, head_dim, window,
                             dev_err)
@@ -1099,7 +1100,7 @@ def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_
         scratch = _packed_scratch(what, packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts), partials, counters)
     call("vlrf_attn_packed_prefill", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], seq_slot.data_ptr(),
          seq_start.data_ptr(), seq_pos0.data_ptr(), out.data_ptr(), out.stride(0), n_tokens, n_seqs, max_new, n_heads, n_kv_heads, head_dim, cache.block_tokens,
-         float(scale), window, groups, n_parts, part_blocks, *scratch, dev_err.data_ptr(), _stream())
+         float(scale), window, least_new, groups, n_parts, part_blocks, *scratch, dev_err.data_ptr(), _stream())
 
 
 def packed_prefill_scratch(n_seqs: int, max_new: int, n_heads: int, head_dim: int, groups: int, n_parts: int) -> tuple:
@@ -1167,22 +1168,31 @@ def _packed_scratch(what: str, want: tuple, partials, counters) -> tuple:
 
 
 def attention_decode_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, out, n_rows: int, n_heads: int, n_kv_heads: int,
-                            head_dim: int, scale: float, window: int, shape: tuple, dev_err, partials=None, counters=None) -> None:
+                            head_dim: int, scale: float, window: int, shape: tuple, dev_err, partials=None, counters=None, row_of=None) -> None:
     """One bfloat16 query per row and head attends the keys 0…position of its slot in a cache of 4 bits, on the tensor cores.  shape = (a CTA an SM
     or not, n_split, blocks a part), see packed_decode_shape: a context takes as many parts as it needs for so many blocks each, at most (and in
     fact, where a context is longer than they hold) n_split; with n_split > 1 they meet in float32 `partials` and zeroed int32 `counters` (see packed_decode_scratch; the counters are left
-    zero).  Rows with slot −1 are left as they are."""
+    zero).  Rows with slot −1 are left as they are.  row_of (int32, a number more than n_rows): entry i of tok_slot and tok_pos stands for the rows
+    row_of[i] … row_of[i+1]−1, and only entries of one row are looked at (of a mixed step the sequences that bring one token)."""
     what = "attention_decode_packed"
-    _attention_packed_check(what, qkv, q_off, cache, block_table, (tok_slot, tok_pos), out, n_rows, n_heads, n_kv_heads, head_dim, window, dev_err)
-    if qkv.dtype != torch.bfloat16 or tok_slot.shape[0] < n_rows or tok_pos.shape[0] < n_rows:
+    _attention_packed_check(what, qkv, q_off, cache, block_table, (tok_slot, tok_pos) if row_of is None else (tok_slot, tok_pos, row_of), out, n_rows, n_heads,
+                            n_kv_heads, head_dim, window, dev_err)
+    if qkv.dtype != torch.bfloat16 or tok_slot.shape[0] < n_rows or tok_pos.shape[0] < n_rows or (row_of is not None and row_of.shape[0] <= n_rows):
         raise KernelError(f"{what}: bfloat16 rows, each with a slot and a position")
     few, n_split, part_tiles = shape
     scratch = (0, 0)
     if n_split > 1:
         scratch = _packed_scratch(what, packed_decode_scratch(n_rows, n_heads, n_kv_heads, head_dim, n_split), partials, counters)
     call("vlrf_attn_packed_decode", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], tok_slot.data_ptr(),
-         tok_pos.data_ptr(), out.data_ptr(), out.stride(0), n_rows, n_heads, n_kv_heads, head_dim, cache.block_tokens, float(scale), window,
+         tok_pos.data_ptr(), _ptr(row_of), out.data_ptr(), out.stride(0), n_rows, n_heads, n_kv_heads, head_dim, cache.block_tokens, float(scale), window,
          1 if few else 0, n_split, part_tiles, *scratch, dev_err.data_ptr(), _stream())
+
+
+#: Single tokens among prompts: a prompt's CTA is 128 or 256 queries whether there are so many or not, so from this many heads times blocks of 64 in their
+#: contexts on they go to the decode kernel, one launch more (640 tokens of 25 heads of 64 beside 2 tokens behind 400, 350 blocks: 23.3 us together, 27.8
+#: apart; 4 tokens, 700: 24.0, 25.8; 8 tokens, 1,400: 33.1, 26.4; 16 tokens: 43.3, 28.5; 200 tokens of 8 heads of 128 beside 2 behind 3,000, 752: 32.9,
+#: 24.8; 700 of 32 heads beside 30 behind 2,000: 418, 82).
+PACKED_SINGLES_APART = 750
 
 
 def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ctx, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -1190,26 +1200,34 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
     """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
     already holds the step's own keys and values."""
     mma = _packed_mma_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim)
-    partials = counters = None
+
+    def scratch(sizes):
+        return (ctx.ws.get("packed_partials", sizes[0], 1, torch.float32), ctx.ws.get_zeroed("packed_counters", sizes[1], torch.int32)) if sizes[1] else ()
+
+    def decode(slots, positions, rows, past, longest, row_of=None):
+        shape = packed_decode_shape(len(past) or rows, n_heads, n_kv_heads, head_dim, longest, window,
+                                    (sum(past) + len(past)) / (len(past) * longest) if past else 0.67)
+        room = scratch(packed_decode_scratch(rows, n_heads, n_kv_heads, head_dim, shape[1]) if shape[1] > 1 else (0, 0))
+        attention_decode_packed(qkv, q_off, cache, block_table, slots, positions, out, rows, n_heads, n_kv_heads, head_dim, scale, window, shape, ctx.dev_err,
+                                *(room or (None, None)), row_of)
+
     if mma and ctx.max_new == 1 and head_dim % 64 == 0 and ctx.n_tokens <= 65535:
-        rows, past = ctx.n_tokens, ctx.host_seq_pos0
-        shape = packed_decode_shape(rows, n_heads, n_kv_heads, head_dim, ctx.max_context, window,
-                                    (sum(past) + rows) / (rows * ctx.max_context) if len(past) == rows else 0.67)
-        if shape[1] > 1:
-            n_floats, n_counters = packed_decode_scratch(rows, n_heads, n_kv_heads, head_dim, shape[1])
-            partials = ctx.ws.get("packed_partials", n_floats, 1, torch.float32)
-            counters = ctx.ws.get_zeroed("packed_counters", n_counters, torch.int32)
-        attention_decode_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, rows, n_heads, n_kv_heads, head_dim, scale,
-                                window, shape, ctx.dev_err, partials, counters)
+        past = ctx.host_seq_pos0
+        decode(ctx.tok_slot, ctx.tok_pos, ctx.n_tokens, past if len(past) == ctx.n_tokens else (), ctx.max_context)
         return
     if mma and ctx.max_new > 1 and scale >= 0.0 and head_dim in (64, 128) and ctx.n_seqs <= 65535:
-        groups, n_parts, part_blocks = packed_prefill_shape(ctx.host_seq_lens, ctx.host_seq_pos0, n_heads, head_dim, window)
-        if n_parts > 1:
-            n_floats, n_counters = packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts)
-            partials = ctx.ws.get("packed_partials", n_floats, 1, torch.float32)
-            counters = ctx.ws.get_zeroed("packed_counters", n_counters, torch.int32)
+        lens, pos0 = ctx.host_seq_lens, ctx.host_seq_pos0
+        single = [b for a, b in zip(lens, pos0) if a == 1]
+        apart = n_heads * sum((min(b, window + 63) if window > 0 else b) // 64 + 1 for b in single) >= PACKED_SINGLES_APART and max(lens) > 1
+        if apart:
+            lens, pos0 = [a for a in lens if a > 1], [b for a, b in zip(lens, pos0) if a > 1]
+        groups, n_parts, part_blocks = packed_prefill_shape(lens, pos0, n_heads, head_dim, window)
+        room = scratch(packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts) if n_parts > 1 else (0, 0))
         attention_prefill_packed(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_start, ctx.seq_pos0, out, ctx.n_tokens, ctx.n_seqs, ctx.max_new,
-                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, part_blocks, partials, counters)
+                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, part_blocks, *(room or (None, None)),
+                                 2 if apart else 1)
+        if apart:
+            decode(ctx.seq_slot, ctx.seq_pos0, ctx.n_seqs, single, max(single) + 1, ctx.seq_start)
         return
     attention_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
                      window, ctx.dev_err)

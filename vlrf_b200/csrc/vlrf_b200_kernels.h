@@ -472,14 +472,16 @@ int vlrf_attn_packed(const void* qkv, int dtype, int ld, int q_off, const void* 
 // as many parts as it needs for at most part_tiles blocks each, up to n_split (of 64 at most), and longer ones where those do not hold it; contexts
 // of more than one meet in scratch: float32 partials and int32 counters, zero before the first call (every call leaves them zero), of the sizes that
 // vlrf_attn_packed_decode_scratch gives (host pointers).  few: a CTA an SM with many warps (1), or several of four (0).
+// row_of (or null): entry i is the rows row_of[i] … row_of[i + 1] − 1 of qkv and out, and is skipped unless that is one row: of a mixed step the sequences that
+// bring one token.
 int vlrf_attn_packed_decode_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out);
 int vlrf_attn_packed_decode_scratch(int rows, int H, int Hkv, int dh, int n_split, long long* floats, long long* ints);
 int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
-                            const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, void* out, int ld_out, int rows,
-                            int H, int Hkv, int dh, int BT, float scale, int window, int few, int n_split, int part_tiles, float* partials,
+                            const int* block_table, int max_blocks, const int* tok_slot, const int* tok_pos, const int* row_of, void* out,
+                            int ld_out, int rows, int H, int Hkv, int dh, int BT, float scale, int window, int few, int n_split, int part_tiles, float* partials,
                             int* counters, int* dev_err, cudaStream_t stream);
 // A prompt step of it on the tcgen05 tensor cores, bfloat16, head sizes 64 and 128, blocks of 64: sequences as in vlrf_attn_prefill (slot −1:
-// skipped), of n_tokens rows at most in all.  A CTA takes `groups` (1 or 2) times 128 queries of a head; n_parts > 1 deals the keys of long tiles, part_blocks blocks of 64 to each or
+// skipped), of n_tokens rows at most in all; those that bring fewer than least_new (≥ 1) are skipped.  A CTA takes `groups` (1 or 2) times 128 queries of a head; n_parts > 1 deals the keys of long tiles, part_blocks blocks of 64 to each or
 // more, to that many CTAs (up to vlrf_attn_packed_prefill_max_parts()), which meet in scratch: float32 partials and int32 counters, zero before the first call (every
 // call leaves them zero), of the sizes that vlrf_attn_packed_prefill_scratch gives (host pointers).
 int vlrf_attn_packed_prefill_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out);
@@ -488,7 +490,7 @@ int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, int dh, int
 int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                              const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0,
                              void* out, int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window,
-                             int groups, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream);
+                             int least_new, int groups, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream);
 
 // ---- routed experts (moe.cu) ---------------------------------------------------------------------------------------
 // z: float32 router logits [T][ld_z] (column E: the logit of a shared expert's gate, if shared_gate).  ids, wts, rank
