@@ -1188,6 +1188,22 @@ def attention_decode_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_s
          1 if few else 0, n_split, part_tiles, *scratch, dev_err.data_ptr(), _stream())
 
 
+def _packed_room(ws, sizes: tuple) -> tuple:
+    return ws.get("packed_partials", sizes[0], 1, torch.float32), ws.get_zeroed("packed_counters", sizes[1], torch.int32)
+
+
+def _packed_decode_step(qkv, q_off, cache, block_table, slots, positions, out, ctx, rows, past, longest, n_heads, n_kv_heads, head_dim, scale, window,
+                        row_of=None) -> None:
+    """past: the single tokens' contexts where the host knows them."""
+    n = len(past)
+    shape = packed_decode_shape(n or rows, n_heads, n_kv_heads, head_dim, longest, window, (sum(past) + n) / (n * longest) if n > 0 else 0.67)
+    partials = counters = None
+    if shape[1] > 1:
+        partials, counters = _packed_room(ctx.ws, packed_decode_scratch(rows, n_heads, n_kv_heads, head_dim, shape[1]))
+    attention_decode_packed(qkv, q_off, cache, block_table, slots, positions, out, rows, n_heads, n_kv_heads, head_dim, scale, window, shape, ctx.dev_err,
+                            partials, counters, row_of)
+
+
 #: Single tokens among prompts: a prompt's CTA is 128 or 256 queries whether there are so many or not, so from this many heads times blocks of 64 in their
 #: contexts on they go to the decode kernel, one launch more (640 tokens of 25 heads of 64 beside 2 tokens behind 400, 350 blocks: 23.3 us together, 27.8
 #: apart; 4 tokens, 700: 24.0, 25.8; 8 tokens, 1,400: 33.1, 26.4; 16 tokens: 43.3, 28.5; 200 tokens of 8 heads of 128 beside 2 behind 3,000, 752: 32.9,
@@ -1200,20 +1216,10 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
     """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
     already holds the step's own keys and values."""
     mma = _packed_mma_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim)
-
-    def scratch(sizes):
-        return (ctx.ws.get("packed_partials", sizes[0], 1, torch.float32), ctx.ws.get_zeroed("packed_counters", sizes[1], torch.int32)) if sizes[1] else ()
-
-    def decode(slots, positions, rows, past, longest, row_of=None):
-        shape = packed_decode_shape(len(past) or rows, n_heads, n_kv_heads, head_dim, longest, window,
-                                    (sum(past) + len(past)) / (len(past) * longest) if past else 0.67)
-        room = scratch(packed_decode_scratch(rows, n_heads, n_kv_heads, head_dim, shape[1]) if shape[1] > 1 else (0, 0))
-        attention_decode_packed(qkv, q_off, cache, block_table, slots, positions, out, rows, n_heads, n_kv_heads, head_dim, scale, window, shape, ctx.dev_err,
-                                *(room or (None, None)), row_of)
-
     if mma and ctx.max_new == 1 and head_dim % 64 == 0 and ctx.n_tokens <= 65535:
         past = ctx.host_seq_pos0
-        decode(ctx.tok_slot, ctx.tok_pos, ctx.n_tokens, past if len(past) == ctx.n_tokens else (), ctx.max_context)
+        _packed_decode_step(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx, ctx.n_tokens, past if len(past) == ctx.n_tokens else (),
+                            ctx.max_context, n_heads, n_kv_heads, head_dim, scale, window)
         return
     if mma and ctx.max_new > 1 and scale >= 0.0 and head_dim in (64, 128) and ctx.n_seqs <= 65535:
         lens, pos0 = ctx.host_seq_lens, ctx.host_seq_pos0
@@ -1222,12 +1228,15 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
         if apart:
             lens, pos0 = [a for a in lens if a > 1], [b for a, b in zip(lens, pos0) if a > 1]
         groups, n_parts, part_blocks = packed_prefill_shape(lens, pos0, n_heads, head_dim, window)
-        room = scratch(packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts) if n_parts > 1 else (0, 0))
+        partials = counters = None
+        if n_parts > 1:
+            partials, counters = _packed_room(ctx.ws, packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts))
         attention_prefill_packed(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_start, ctx.seq_pos0, out, ctx.n_tokens, ctx.n_seqs, ctx.max_new,
-                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, part_blocks, *(room or (None, None)),
+                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, part_blocks, partials, counters,
                                  2 if apart else 1)
         if apart:
-            decode(ctx.seq_slot, ctx.seq_pos0, ctx.n_seqs, single, max(single) + 1, ctx.seq_start)
+            _packed_decode_step(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_pos0, out, ctx, ctx.n_seqs, single, max(single) + 1, n_heads, n_kv_heads,
+                                head_dim, scale, window, ctx.seq_start)
         return
     attention_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
                      window, ctx.dev_err)
