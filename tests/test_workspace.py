@@ -1,40 +1,58 @@
-"""Scratch that lives across steps: how it grows, and what is left when it cannot."""
+"""Scratch that outlives a step: what a capture may leave behind."""
 import pytest
 import torch
 
 from vlrf_b200.parts.context import Workspace
 
 
-def test_buffers_that_must_not_double_take_what_is_asked_for():
-    ws = Workspace("cpu")
-    ws.get("small", 1, 1000, torch.float32)
-    ws.get("small", 1, 1500, torch.float32)
-    assert ws.bytes() == 4 * 2000
-    ws.get("large", 1, 1000, torch.float32, exact=True)
-    ws.get("large", 1, 1500, torch.float32, exact=True)
-    assert ws.bytes() == 4 * (2000 + 1500)
-    generation = ws.generation
-    view = ws.get("large", 1, 1200, torch.float32, exact=True)
-    assert view.shape == (1, 1200) and ws.bytes() == 4 * 3500 and ws.generation == generation
-    ws.frozen = True
-    with pytest.raises(RuntimeError):
-        ws.get("large", 1, 1600, torch.float32, exact=True)
-    assert ws.get("large", 1, 1500, torch.float32).shape == (1, 1500)
+class Capture:
+    """Stands for a stream that is capturing: a fill is recorded, and memory holds what it held."""
+
+    def __init__(self, monkeypatch):
+        self.on = False
+        zeros, fill = torch.zeros, torch.Tensor.zero_
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.on)
+        monkeypatch.setattr(torch, "zeros", lambda *a, **kw: zeros(*a, **kw).fill_(7) if self.on else zeros(*a, **kw))
+        monkeypatch.setattr(torch.Tensor, "zero_", lambda t: t if self.on else fill(t))
 
 
-def test_a_buffer_that_cannot_grow_is_given_back_first(monkeypatch):
-    """The old buffer is not held beside the new one; a failure leaves no view of it, and captured steps see that it went."""
-    ws = Workspace("cpu")
-    ws.get("large", 1, 1000, torch.float32, exact=True)
-    generation, real = ws.generation, torch.empty
-    held = []
+def test_counters_first_made_in_a_capture_that_never_runs_are_zero_afterwards(monkeypatch):
+    ws, capture = Workspace("cpu"), Capture(monkeypatch)
+    capture.on = True
+    ws.get_zeroed("counters", 5, torch.int32)
+    ws.get_zeroed("counters", 3, torch.int32)              # (the step's other layers)
+    capture.on = False
+    assert not ws.get_zeroed("counters", 5, torch.int32).any()
+    ws.get_zeroed("counters", 5, torch.int32)[2] = 9       # whoever uses it leaves it zero: it is not filled again and again
+    assert int(ws.get_zeroed("counters", 5, torch.int32)[2]) == 9
 
-    def full(*a, **k):
-        held.append(ws.bytes())
-        raise torch.OutOfMemoryError("no room")
-    monkeypatch.setattr(torch, "empty", full)
-    with pytest.raises(torch.OutOfMemoryError):
-        ws.get("large", 1, 2000, torch.float32, exact=True)
-    monkeypatch.setattr(torch, "empty", real)
-    assert held == [0] and ws.generation > generation and ws.bytes() == 0
-    assert ws.get("large", 1, 1000, torch.float32, exact=True).shape == (1, 1000)
+
+def test_counters_that_grow_in_a_capture_that_never_runs_are_zero_afterwards(monkeypatch):
+    ws, capture = Workspace("cpu"), Capture(monkeypatch)
+    ws.get_zeroed("counters", 2, torch.int32)
+    capture.on = True
+    ws.get_zeroed("counters", 8, torch.int32)
+    capture.on = False
+    assert not ws.get_zeroed("counters", 8, torch.int32).any()
+
+
+@pytest.mark.gpu
+def test_counters_made_in_a_dropped_capture_on_the_device():
+    """Two captures that are dropped unplayed, one that is kept, and a plain step behind them."""
+    from vlrf_b200.engine.capture import capture_into
+    ws = Workspace("cuda:0")
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with capture_into(graph):
+            ws.get_zeroed("counters", 1 << 20, torch.int32)
+        del graph
+        buf = ws._bufs["counters"]
+        buf.fill_(3)                                       # as whatever lay there before
+    seen = torch.empty(1 << 20, dtype=torch.int32, device="cuda:0")
+    kept = torch.cuda.CUDAGraph()
+    with capture_into(kept):
+        seen.copy_(ws.get_zeroed("counters", 1 << 20, torch.int32))
+    kept.replay()
+    assert not bool(seen.any())
+    ws._bufs["counters"].fill_(3)
+    assert not bool(ws.get_zeroed("counters", 1 << 20, torch.int32).any())

@@ -21,6 +21,7 @@ class Workspace:
     def __init__(self, device):
         self.device = torch.device(device)
         self._bufs: dict[str, torch.Tensor] = {}
+        self._unfilled: set = set()      # zeroed buffers that were made in a capture: their fill is part of a graph that may never run
         self._side = None        # the second stream of `beside`
         self._views: dict = {}   # (name, rows, cols, dtype) -> the view handed out last time (making one costs 2 to 3 us)
         self.frozen = False  # set while a captured graph depends on the addresses
@@ -68,7 +69,8 @@ class Workspace:
 
     def get_zeroed(self, name: str, n: int, dtype: torch.dtype) -> torch.Tensor:
         """A flat buffer that is zero when first handed out (and again after it had to grow); whoever uses
-        it leaves it zero."""
+        it leaves it zero.  Made in a capture, it is filled by the graph, and filled again outside, where that graph may
+        have been dropped."""
         buf = self._bufs.get(name)
         if buf is None or buf.dtype != dtype or buf.numel() < n:
             if self.frozen:
@@ -76,6 +78,13 @@ class Workspace:
             buf = torch.zeros(max(n, 1), dtype=dtype, device=self.device)
             self._bufs[name] = buf
             self.generation += 1
+            self._unfilled.discard(name)
+            if torch.cuda.is_current_stream_capturing():
+                self._unfilled.add(name)
+        elif name in self._unfilled:
+            buf.zero_()
+            if not torch.cuda.is_current_stream_capturing():
+                self._unfilled.discard(name)
         return buf[:n]
 
     @contextlib.contextmanager
