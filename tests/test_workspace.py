@@ -11,6 +11,7 @@ class Capture:
     def __init__(self, monkeypatch):
         self.on = False
         zeros, fill = torch.zeros, torch.Tensor.zero_
+        monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
         monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.on)
         monkeypatch.setattr(torch, "zeros", lambda *a, **kw: zeros(*a, **kw).fill_(7) if self.on else zeros(*a, **kw))
         monkeypatch.setattr(torch.Tensor, "zero_", lambda t: t if self.on else fill(t))
@@ -34,6 +35,11 @@ def test_counters_that_grow_in_a_capture_that_never_runs_are_zero_afterwards(mon
     ws.get_zeroed("counters", 8, torch.int32)
     capture.on = False
     assert not ws.get_zeroed("counters", 8, torch.int32).any()
+
+
+def test_a_workspace_without_a_device():
+    ws = Workspace("cpu")
+    assert not ws.get_zeroed("counters", 4, torch.int32).any() and not ws.get_zeroed("counters", 9, torch.int32).any()
 
 
 @pytest.mark.gpu

@@ -13,6 +13,10 @@ import dataclasses
 import torch
 
 
+def _capturing() -> bool:
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 class Workspace:
     """Named scratch tensors that live across steps, so steps allocate nothing once warm and a
     captured step sees stable addresses.  `get` returns a [rows, cols] view of the named buffer, which
@@ -79,11 +83,11 @@ class Workspace:
             self._bufs[name] = buf
             self.generation += 1
             self._unfilled.discard(name)
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing():
                 self._unfilled.add(name)
         elif name in self._unfilled:
             buf.zero_()
-            if not torch.cuda.is_current_stream_capturing():
+            if not _capturing():
                 self._unfilled.discard(name)
         return buf[:n]
 
