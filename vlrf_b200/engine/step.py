@@ -220,9 +220,7 @@ class Engine:
         """Run the model on the step, replaying a captured graph when a step of the same shape ran before."""
         if not self.capture_repeated_steps or ctx.max_new == 1 or not self.model.replayable:
             return self.model.forward(ctx, self.cache)     # single-token steps have DecodeSession's graph
-        if self._graph_generation != self.ws.generation:
-            self._graphs.clear()                           # scratch moved: captured addresses are stale
-            self._graph_generation = self.ws.generation
+        self._drop_stale_graphs()
         hit = self._graphs.get(signature)
         if hit is not None:
             hit[0].replay()
@@ -231,18 +229,25 @@ class Engine:
         self._seen[signature] = n + 1
         if n == 0 or len(self._graphs) >= 16:
             logits = self.model.forward(ctx, self.cache)   # first time: plain launches (they size the scratch)
-            self._graph_generation = self.ws.generation
+            self._drop_stale_graphs()
             return logits
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         with capture_into(graph):
             logits = self.model.forward(ctx, self.cache)
-        if self.ws.generation != self._graph_generation:   # the capture itself had to allocate: do not keep it
-            self._graph_generation = self.ws.generation
+        if self._drop_stale_graphs():                      # the capture itself had to allocate: do not keep it
             return self.model.forward(ctx, self.cache)
         self._graphs[signature] = (graph, logits)
         graph.replay()
         return logits
+
+    def _drop_stale_graphs(self) -> bool:
+        """Forget the captured steps where scratch has moved since: they go to addresses that have been given back."""
+        if self._graph_generation == self.ws.generation:
+            return False
+        self._graphs.clear()
+        self._graph_generation = self.ws.generation
+        return True
 
     def check_device_errors(self) -> None:
         """Read the device's error word (synchronises) and raise if a kernel set a bit."""
