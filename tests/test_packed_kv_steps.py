@@ -1,0 +1,93 @@
+"""Steps over a cache of 4 bits as a whole: the scratch they take.  On the CPU the kernels' launches are the test's stand-ins; the plans and the scratch are
+the library's own."""
+import random
+
+import pytest
+import torch
+
+from vlrf_b200.parts.context import StepContext, Workspace
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """What a step launches, as (name, positional arguments, others), on a device of 148 SMs."""
+    from vlrf_b200.csrc import ops
+    seen = []
+    monkeypatch.setattr(ops, "_SM_COUNT", 148)
+    ops._packed_decode_shape.cache_clear(); ops._packed_prefill_shape.cache_clear()
+    for name in ("attention_packed", "attention_decode_packed", "attention_prefill_packed"):
+        monkeypatch.setattr(ops, name, lambda *a, name=name, **kw: seen.append((name, a, kw)))
+    yield seen
+    ops._packed_decode_shape.cache_clear(); ops._packed_prefill_shape.cache_clear()
+
+
+def step(new, past, H, G, d, window=0, ws=None, lists=True, scale=0.125):
+    from vlrf_b200.csrc import ops
+    T, B = sum(new), len(new)
+    t = torch.zeros(B + 1, dtype=torch.int32)
+    ws = ws or Workspace("cpu")
+    ctx = StepContext(n_tokens=T, tokens=t, tok_slot=t, tok_pos=t, n_seqs=B, seq_slot=t, seq_start=t, seq_pos0=t, max_new=max(new),
+                      max_context=max(a + b for a, b in zip(new, past)), logit_rows=t, n_logit_rows=0, act_dtype=torch.bfloat16, dev_err=t, ws=ws,
+                      host_seq_slots=list(range(B)), min_new=min(new))
+    if lists:
+        ctx.host_seq_lens, ctx.host_seq_pos0 = list(new), list(past)
+    rows = torch.empty((T, (H + 2 * G) * d), dtype=torch.bfloat16)
+    out = torch.empty((T, H * d), dtype=torch.bfloat16)
+    ops.attention_packed_step(rows, 0, ops.PackedKV.zeros(1, G, 64, d, "cpu"), t.view(1, -1), out, ctx, H, G, d, scale, window)
+    return ws
+
+
+@pytest.mark.parametrize("new,past,H,G,d,window", [([1000] + [1] * 60, [0] + [400] * 60, 25, 25, 64, 0), ([700] + [1] * 30, [0] + [2000] * 30, 32, 8, 128, 0),
+                                                    ([512] + [1] * 63, [7500] + [1000] * 63, 32, 8, 128, 0), ([1000] + [1] * 255, [4000] + [500] * 255, 12, 12, 64, 0),
+                                                    ([1000] + [30] * 60, [0] * 61, 25, 25, 64, 0), ([1] * 30 + [512, 2, 2], [900] * 30 + [6000, 10, 10], 32, 8, 128, 3000)])
+def test_scratch_of_a_step_is_what_its_tiles_fill(launches, new, past, H, G, d, window):
+    """One long prompt among many sequences: parts of a tile meet in scratch, and only tiles that are dealt to several CTAs have any."""
+    ws = step(new, past, H, G, d, window)
+    assert any(name == "attention_prefill_packed" for name, _, _ in launches)
+    assert ws.bytes() <= 30e6
+
+
+def test_every_tile_that_parts_share_has_a_place():
+    """Against the tiles one by one: those that reach more than part_blocks blocks are dealt; without a window nothing else has a place."""
+    from vlrf_b200.csrc import ops
+    rng = random.Random(5)
+    for _ in range(400):
+        n = rng.randint(1, 6)
+        new, past = [rng.choice([0, 1, 2, rng.randint(1, 700)]) for _ in range(n)], [rng.choice([0, rng.randint(0, 3000)]) for _ in range(n)]
+        groups, each, window = rng.choice([1, 2]), rng.randint(1, 30), rng.choice([0, 0, rng.randint(1, 2500)])
+        dealt, rows = 0, 128 * groups
+        for a, b in zip(new, past):
+            for t in range(0, a, rows):
+                first = max(0, b + t - window + 1) if window > 0 else 0
+                dealt += (b + min(t + rows, a) - 1) // 64 - first // 64 + 1 > each
+        places = ops.packed_prefill_places(new, past, groups, 2, each, window)
+        assert places == dealt if window == 0 else places >= dealt
+        assert ops.packed_prefill_places(new, past, groups, 1, each, window) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim", [(3, 3, 64), (4, 2, 128)])
+@pytest.mark.parametrize("new,past", [([300, 1, 64], [77, 700, 0]), ([1] * 33 + [270, 3, 130] + [1] * 4, list(range(40))), ([2, 0, 513], [900, 50, 200]),
+                                      ([1, 400, 90] * 30, [7, 300, 0] * 30)])
+@pytest.mark.parametrize("window", [0, 90, 400])
+@pytest.mark.parametrize("groups,n_parts,part_blocks", [(1, 3, 2), (2, 16, 1), (2, 2, 5)])
+@pytest.mark.parametrize("short", [0, 1, 100])
+def test_prompt_attention_with_scratch_for_the_tiles_that_are_dealt(heads, kv_heads, dim, new, past, window, groups, n_parts, part_blocks, short):
+    """Scratch of exactly the size, and of less: tiles without a place are not dealt, and nothing lies outside it."""
+    from test_packed_kv_kernels import DEV, Pages, check_prompt
+    from vlrf_b200.csrc import ops
+    pages = Pages([a + b for a, b in zip(new, past)], kv_heads, dim, seed=heads + sum(new))
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)   # noqa: E731
+    start = [sum(new[:i]) for i in range(len(new) + 1)]
+    places = max(0, ops.packed_prefill_places(new, past, groups, n_parts, part_blocks, window) - short)
+    floats, counts = ops.packed_prefill_scratch(len(new), max(new), heads, dim, groups, n_parts, places)
+    partials, counters = torch.full((floats + 1024,), 77.0, device=DEV), torch.full((counts + 64,), 5, dtype=torch.int32, device=DEV)
+    counters[:counts] = 0
+
+    def fn(qkv, q_off, table, slot, pos, out, scale, e):
+        ops.attention_prefill_packed(qkv, q_off, pages.cache, table, ints(list(range(len(new)))), ints(start), ints(past), out, sum(new), len(new), max(new), heads,
+                                     kv_heads, dim, scale, window, e, groups, n_parts, part_blocks, partials, counters, n_places=places)
+        assert not bool(counters[:counts].any()) and bool((counters[counts:] == 5).all()) and bool((partials[floats:] == 77).all())
+        if places and window == 0 and not short:
+            assert bool((partials[:floats] != 77).any())
+    check_prompt(fn, pages, new, heads, kv_heads, dim, window)

@@ -204,6 +204,8 @@ _SIGNATURES = {
     "vlrf_attn_packed_prefill_takes": [_c_int] * 7,
     "vlrf_attn_packed_prefill_max_parts": [],
     "vlrf_attn_packed_prefill_scratch": [_c_int] * 6 + [ctypes.POINTER(ctypes.c_longlong)] * 2,
+    "vlrf_attn_packed_prefill_places": [_c_void_p, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 8
+                                       + [_c_float] + [_c_int] * 6 + [_c_void_p] * 4,
     "vlrf_attn_packed_prefill": [_c_void_p, _c_int, _c_int] + [_c_void_p] * 4 + [_c_int, _c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 8
                                 + [_c_float] + [_c_int] * 5 + [_c_void_p] * 4,
     "vlrf_moe_route": [_c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,

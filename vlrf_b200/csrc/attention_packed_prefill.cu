@@ -132,7 +132,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
                            const unsigned char* __restrict__ Vq, const uint32_t* __restrict__ Vp, int n_blocks, const int* __restrict__ block_table,
                            int max_blocks, const int* __restrict__ seq_slot, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
                            __nv_bfloat16* __restrict__ out, int ld_out, int H, int Hkv, float scale, int window, int n_parts, int part_blocks, float* __restrict__ partials,
-                           int* __restrict__ counters, int n_tiles, int n_seqs, int n_flat, int least_new, int* __restrict__ dev_err) {
+                           int* __restrict__ counters, int n_tiles, int n_seqs, int n_flat, int n_places, int least_new, int* __restrict__ dev_err) {
     constexpr int BK = PP_BK, PP_TILE = BK * DH * 2, PP_SLOTS = PP_RING / PP_TILE, ROWS = GROUPS * 128, NG = DH / 64, NPROD = pp_producers(GROUPS), SOFT = GROUPS * 8;
     constexpr int Q_BYTES = 128 * DH * 2, ATOM_Q = 16384, ATOM_KV = BK * 128;    // a 64-number chunk of 128 queries / of a block
     constexpr int NP = BK + DH + BK <= 256 ? 2 : 1;                 // buffers of P that a group's 256 columns have room for
@@ -160,6 +160,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     int* s_first = s_top + 1;                                       // [2]: of the largest numbers of the first block's keys and of its values, the smallest, as bits
     float* s_unit = reinterpret_cast<float*>(s_first + 2);          // [2]: from an MMA's result to a score in units of log2(e); from one of O to a number
     int* s_last = reinterpret_cast<int*>(s_unit + 2);                                        // [GROUPS]: whether this CTA merges its tile's parts
+    int* s_place = s_last + GROUPS;                                 // the tile's place in scratch
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -220,7 +221,20 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     const int first_key = window > 0 ? max(0, q_first - window + 1) : 0;
     const int kb_first = first_key / BK, n_kb = q_last / BK - kb_first + 1;
     // the tile's key blocks are dealt to tile_parts CTAs, of part_blocks each or more; the others of its n_parts have nothing to do
-    const int tile_parts = max(1, min(n_parts, (n_kb + part_blocks - 1) / part_blocks));
+    int tile_parts = max(1, min(n_parts, (n_kb + part_blocks - 1) / part_blocks));
+    if (tile_parts > 1) {
+        // Scratch has places for tiles that reach part_blocks blocks or more from their sequence's first token only, which are its last ones: this tile's is
+        // behind those of the sequences before.  (Where there is none left the tile is not dealt; uniform over the CTA.)
+        const int whole = min(part_blocks, 1 << 24) * BK;           // tokens that a CTA takes by itself whatever the rest
+        int place = min((n_new + ROWS - 1) / ROWS, n_tiles) - 1 - qt;
+        for (int s0 = 0; s0 < seq; s0 += 32) {
+            const int s = s0 + lane, len = s < seq ? seq_start[s + 1] - seq_start[s] : 0, tiles = len >= least_new ? min((len + ROWS - 1) / ROWS, n_tiles) : 0;
+            const int alone = tiles > 0 ? whole - seq_pos0[s] : len;             // new tokens that end before that many positions
+            place += (int)__reduce_add_sync(0xffffffffu, (unsigned)(alone < len ? max(tiles - max(alone, 0) / ROWS, 0) : 0));
+        }
+        if (place >= n_places) tile_parts = 1;
+        if (threadIdx.x == 0) *s_place = place;
+    }
     const bool active = n_rows > 0 && n_new >= least_new && slot >= 0 && pos0 >= 0 && part < tile_parts;      // uniform over the CTA
     if (!active) return;                                            // (before it holds anything)
     constexpr uint32_t TMEM_COLS = 256 * GROUPS;                    // a group: S BK columns, O DH, P NP times BK / 2 (two bfloat16 a column)
@@ -752,7 +766,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         } else if (group_rows > 0) {
             // leave this part's result in scratch ([d][row], so that a warp writes whole lines), then see whether the tile's other
             // parts are all there
-            const size_t tile_id = (((size_t)seq * H + h) * n_tiles + qt) * GROUPS + g;
+            const size_t tile_id = ((size_t)*s_place * H + h) * GROUPS + g;
             const float* parts = partials + tile_id * n_parts * pp_part_floats(DH);
             float* mine = partials + (tile_id * n_parts + part) * pp_part_floats(DH);
 #pragma unroll 1
@@ -842,7 +856,8 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
 template <int DH, int GROUPS>
 int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks, const int* block_table,
               int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out, int ld_out, int n_tokens, int n_seqs, int max_new, int H,
-              int Hkv, float scale, int window, int least_new, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+              int Hkv, float scale, int window, int least_new, int n_parts, int part_blocks, int n_places, float* partials, int* counters, int* dev_err,
+              cudaStream_t stream) {
     const size_t smem = 1024 + (size_t)GROUPS * 128 * DH * 2 + (size_t)PP_RING + GROUPS * 256 * 4 + (PP_RING / (PP_BK * DH * 2)) * (64 * 8 + 4) + 48 * 8;
     static DeviceMarks marks;
     auto kern = attn_packed_prefill_kernel<DH, GROUPS>;
@@ -859,7 +874,7 @@ int pp_launch(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp
     e = launch_chained(kern, grid, dim3(pp_threads(GROUPS)), smem, stream, (const __nv_bfloat16*)qkv, ld, q_off,
                        (const unsigned char*)Kq, (const uint32_t*)Kp, (const unsigned char*)Vq, (const uint32_t*)Vp, n_blocks, block_table, max_blocks, seq_slot,
                        seq_start, seq_pos0, (__nv_bfloat16*)out, ld_out, H, Hkv, scale, window, n_parts, part_blocks, partials, counters, (int)tiles, n_seqs,
-                       use_flat ? (int)flat : 0, least_new, dev_err);
+                       use_flat ? (int)flat : 0, n_places, least_new, dev_err);
     if (e != cudaSuccess) return vlrf_fail(VLRF_ERR_CUDA, "attn_packed_prefill: %s", cudaGetErrorString(e));
     return vlrf_check_launch("attn_packed_prefill");
 }
@@ -879,10 +894,12 @@ extern "C" int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, 
     return VLRF_OK;
 }
 
-extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
-                                        const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out,
-                                        int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int least_new,
-                                        int groups, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+// With scratch for n_places tiles (of a head): n_places · H · groups · n_parts · (128 dh + 256) float32 numbers, n_places · H · groups int32 numbers.
+extern "C" int vlrf_attn_packed_prefill_places(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
+                                               const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0,
+                                               void* out, int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale,
+                                               int window, int least_new, int groups, int n_parts, int part_blocks, int n_places, float* partials,
+                                               int* counters, int* dev_err, cudaStream_t stream) {
     VLRF_REQUIRE(vlrf_attn_packed_prefill_takes(H, Hkv, dh, BT, ld, q_off, ld_out),
                  "attn_packed_prefill: %d heads over %d of %d, blocks of %d, row strides %d and %d are not taken", H, Hkv, dh, BT, ld, ld_out);
     VLRF_REQUIRE(n_tokens >= 0 && n_seqs >= 0 && n_seqs <= 65535 && max_new >= 0 && max_blocks > 0 && n_blocks >= 0 && window >= 0 && least_new >= 1 &&
@@ -892,12 +909,25 @@ extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, cons
     VLRF_REQUIRE(groups == 1 || groups == 2, "attn_packed_prefill: %d groups of 128 queries a CTA (1 or 2)", groups);
     VLRF_REQUIRE(n_parts >= 1 && n_parts <= PP_MAX_PARTS && part_blocks >= 1 && (n_parts == 1 || (partials != nullptr && counters != nullptr)),
                  "attn_packed_prefill: %d parts (1 to %d; more than one wants scratch)", n_parts, PP_MAX_PARTS);
+    VLRF_REQUIRE(n_places >= 0, "attn_packed_prefill: scratch for %d tiles", n_places);
     for (const void* p : {qkv, Kq, Kp, Vq, Vp, (const void*)out})
         VLRF_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "attn_packed_prefill: tensors begin on 16 bytes");
     if (n_seqs == 0 || max_new == 0) return VLRF_OK;
 #define GO(DH, G) pp_launch<DH, G>(qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, seq_slot, seq_start, seq_pos0, out, ld_out, n_tokens, \
-                                   n_seqs, max_new, H, Hkv, scale, window, least_new, n_parts, part_blocks, partials, counters, dev_err, stream)
+                                   n_seqs, max_new, H, Hkv, scale, window, least_new, n_parts, part_blocks, n_places, partials, counters, dev_err, stream)
     if (dh == 64) return groups == 1 ? GO(64, 1) : GO(64, 2);
     return groups == 1 ? GO(128, 1) : GO(128, 2);
 #undef GO
+}
+
+// With scratch for every tile that the sequences may have (vlrf_attn_packed_prefill_scratch).
+extern "C" int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
+                                        const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0, void* out,
+                                        int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window, int least_new,
+                                        int groups, int n_parts, int part_blocks, float* partials, int* counters, int* dev_err, cudaStream_t stream) {
+    VLRF_REQUIRE(groups == 1 || groups == 2, "attn_packed_prefill: %d groups of 128 queries a CTA (1 or 2)", groups);
+    const long long tiles = (long long)max(n_seqs, 0) * ((max(max_new, 0) + groups * 128ll - 1) / (groups * 128));
+    return vlrf_attn_packed_prefill_places(qkv, ld, q_off, Kq, Kp, Vq, Vp, n_blocks, block_table, max_blocks, seq_slot, seq_start, seq_pos0, out, ld_out, n_tokens,
+                                           n_seqs, max_new, H, Hkv, dh, BT, scale, window, least_new, groups, n_parts, part_blocks,
+                                           (int)min(tiles, 0x7fffffffll), partials, counters, dev_err, stream);
 }

@@ -1084,31 +1084,43 @@ def _packed_prefill_shape(lens: tuple, pos0: tuple, n_heads: int, head_dim: int,
 
 def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_slot, seq_start, seq_pos0, out, n_tokens: int, n_seqs: int, max_new: int,
                              n_heads: int, n_kv_heads: int, head_dim: int, scale: float, window: int, dev_err, groups: int = 1, n_parts: int = 1,
-                             part_blocks: int = 6, partials=None, counters=None, least_new: int = 1) -> None:
+                             part_blocks: int = 6, partials=None, counters=None, least_new: int = 1, n_places: int | None = None) -> None:
     """Causal attention of every sequence's new tokens (rows seq_start[i] … seq_start[i+1]−1 of qkv, the first of them at position
     seq_pos0[i]) over the sequence's cache of 4 bits, which already holds these tokens; bfloat16, head size 64 or 128, on the tcgen05
     tensor cores, operands float16 under powers of two.  n_parts > 1 deals the keys of long tiles to that many CTAs (see packed_prefill_shape) and wants
-    float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero.  Sequences that bring fewer than least_new
-    tokens are skipped."""
+    float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero.  n_places: how many of the tiles that may be dealt
+    have scratch (see packed_prefill_places; those behind them are not dealt); None: every tile that there can be.  Sequences that bring fewer than
+    least_new tokens are skipped."""
     what = "attention_prefill_packed"
     _attention_packed_check(what, qkv, q_off, cache, block_table, (seq_slot, seq_start, seq_pos0), out, n_tokens, n_heads, n_kv_heads, head_dim, window,
                             dev_err)
     if qkv.dtype != torch.bfloat16 or seq_slot.shape[0] < n_seqs or seq_start.shape[0] < n_seqs + 1 or seq_pos0.shape[0] < n_seqs:
         raise KernelError(f"{what}: bfloat16 rows, and a slot, a first row and a first position for every sequence")
     scratch = (0, 0)
+    if n_places is None:
+        n_places = n_seqs * -(-max_new // (128 * groups)) if groups > 0 else 0
     if n_parts > 1:
-        scratch = _packed_scratch(what, packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts), partials, counters)
-    call("vlrf_attn_packed_prefill", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], seq_slot.data_ptr(),
+        scratch = _packed_scratch(what, packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts, n_places), partials, counters)
+    call("vlrf_attn_packed_prefill_places", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], seq_slot.data_ptr(),
          seq_start.data_ptr(), seq_pos0.data_ptr(), out.data_ptr(), out.stride(0), n_tokens, n_seqs, max_new, n_heads, n_kv_heads, head_dim, cache.block_tokens,
-         float(scale), window, least_new, groups, n_parts, part_blocks, *scratch, dev_err.data_ptr(), _stream())
+         float(scale), window, least_new, groups, n_parts, part_blocks, n_places, *scratch, dev_err.data_ptr(), _stream())
 
 
-def packed_prefill_scratch(n_seqs: int, max_new: int, n_heads: int, head_dim: int, groups: int, n_parts: int) -> tuple:
-    """(float32 elements of `partials`, int32 elements of `counters`) that `attention_prefill_packed` wants for n_parts > 1: the library's
-    vlrf_attn_packed_prefill_scratch, without asking it."""
+def packed_prefill_places(lens, pos0, groups: int, n_parts: int, part_blocks: int, window: int = 0) -> int:
+    """How many tiles of a step `attention_prefill_packed` may deal to several CTAs, and so wants scratch for: sequences that bring lens[i] tokens behind
+    pos0[i], 128 · groups of them a tile; those tiles whose last token lies part_blocks blocks of 64 or more into its sequence."""
+    rows, whole = 128 * groups, part_blocks * 64
+    if n_parts <= 1 or (window > 0 and (window + rows - 2) // 64 + 2 <= part_blocks):
+        return 0
+    return sum(-(-a // rows) - max(whole - b, 0) // rows for a, b in zip(lens, pos0) if a + b > whole)
+
+
+def packed_prefill_scratch(n_seqs: int, max_new: int, n_heads: int, head_dim: int, groups: int, n_parts: int, n_places: int | None = None) -> tuple:
+    """(float32 elements of `partials`, int32 elements of `counters`) that `attention_prefill_packed` wants for n_parts > 1 and n_places of them, or (None) every
+    tile that n_seqs sequences of max_new tokens at most can have: the library's vlrf_attn_packed_prefill_scratch, without asking it."""
     if n_parts <= 1:
         return 0, 0
-    tiles = -(-max_new // (128 * groups)) * groups * n_seqs * n_heads
+    tiles = (n_seqs * -(-max_new // (128 * groups)) if n_places is None else n_places) * groups * n_heads
     return tiles * n_parts * (128 * head_dim + 256), tiles
 
 
@@ -1229,11 +1241,14 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
             lens, pos0 = [a for a in lens if a > 1], [b for a, b in zip(lens, pos0) if a > 1]
         groups, n_parts, part_blocks = packed_prefill_shape(lens, pos0, n_heads, head_dim, window)
         partials = counters = None
-        if n_parts > 1:
-            partials, counters = _packed_room(ctx.ws, packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts))
+        n_places = packed_prefill_places(lens, pos0, groups, n_parts, part_blocks, window)
+        if n_places > 0:
+            partials, counters = _packed_room(ctx.ws, packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts, n_places))
+        else:
+            n_parts = 1
         attention_prefill_packed(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_start, ctx.seq_pos0, out, ctx.n_tokens, ctx.n_seqs, ctx.max_new,
                                  n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, part_blocks, partials, counters,
-                                 2 if apart else 1)
+                                 2 if apart else 1, n_places)
         if apart:
             _packed_decode_step(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_pos0, out, ctx, ctx.n_seqs, single, max(single) + 1, n_heads, n_kv_heads,
                                 head_dim, scale, window, ctx.seq_start)

@@ -481,12 +481,21 @@ int vlrf_attn_packed_decode(const void* qkv, int ld, int q_off, const void* Kq, 
                             int ld_out, int rows, int H, int Hkv, int dh, int BT, float scale, int window, int few, int n_split, int part_tiles, float* partials,
                             int* counters, int* dev_err, cudaStream_t stream);
 // A prompt step of it on the tcgen05 tensor cores, bfloat16, head sizes 64 and 128, blocks of 64: sequences as in vlrf_attn_prefill (slot −1:
-// skipped), of n_tokens rows at most in all; those that bring fewer than least_new (≥ 1) are skipped.  A CTA takes `groups` (1 or 2) times 128 queries of a head; n_parts > 1 deals the keys of long tiles, part_blocks blocks of 64 to each or
-// more, to that many CTAs (up to vlrf_attn_packed_prefill_max_parts()), which meet in scratch: float32 partials and int32 counters, zero before the first call (every
-// call leaves them zero), of the sizes that vlrf_attn_packed_prefill_scratch gives (host pointers).
+// skipped), of n_tokens rows at most in all; those that bring fewer than least_new (≥ 1) are skipped.  A CTA takes `groups` (1 or 2) times 128 queries of a
+// head, a tile; n_parts > 1 deals the keys of long tiles, part_blocks blocks of 64 to each or more, to that many CTAs (up to
+// vlrf_attn_packed_prefill_max_parts()), which meet in scratch: float32 partials and int32 counters, zero before the first call (every call leaves them
+// zero).  Scratch has a place for each of the first n_places tiles whose last query lies part_blocks · 64 positions or more into its sequence (tiles counted
+// sequence by sequence, a sequence's last one first); others are not dealt.  A place is H · groups · n_parts ·
+// (128 dh + 256) numbers of partials and H · groups counters.  vlrf_attn_packed_prefill takes scratch for every tile that there can be, of the
+// sizes that vlrf_attn_packed_prefill_scratch gives (host pointers).
 int vlrf_attn_packed_prefill_takes(int H, int Hkv, int dh, int BT, int ld, int q_off, int ld_out);
 int vlrf_attn_packed_prefill_max_parts();
 int vlrf_attn_packed_prefill_scratch(int n_seqs, int max_new, int H, int dh, int groups, int n_parts, long long* floats, long long* ints);
+int vlrf_attn_packed_prefill_places(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
+                                    const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0,
+                                    void* out, int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window,
+                                    int least_new, int groups, int n_parts, int part_blocks, int n_places, float* partials, int* counters, int* dev_err,
+                                    cudaStream_t stream);
 int vlrf_attn_packed_prefill(const void* qkv, int ld, int q_off, const void* Kq, const void* Kp, const void* Vq, const void* Vp, int n_blocks,
                              const int* block_table, int max_blocks, const int* seq_slot, const int* seq_start, const int* seq_pos0,
                              void* out, int ld_out, int n_tokens, int n_seqs, int max_new, int H, int Hkv, int dh, int BT, float scale, int window,
