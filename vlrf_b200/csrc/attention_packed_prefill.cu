@@ -17,7 +17,8 @@
 // Queries, keys, weights and values are float16 operands (11 bits: each off by up to 2^-11 of itself), scores, sums and results float32; as bfloat16 they
 // together moved a result by 2.5 times what its own rounding does, as float16 by a tenth of that.  What float16 lacks in range powers of two give: the
 // queries' from their largest, the keys' and the values' from the CTA's first block, weights stay below 2^15; a key or a value 2^14 times as large as
-// the first block's gets a power of its own, which costs its block a slower pass.
+// the first block's, or 2^-10, gets a power of its own, which costs its block a slower pass: what a query attends is as exact whatever the first block
+// holds, which, with a window, it may not see.
 // A value that is not a number must not meet the weight 0 of a query that does not see it (0 · NaN is not 0): its row of V becomes zeros, and its
 // key's row of K NaN instead, which the mask hides from the same queries; so a head's row that sees it is NaN throughout.
 //
@@ -35,6 +36,7 @@
 namespace {
 constexpr int PP_CB = 64, PP_BK = 64, PP_RING = 65536;              // tokens of a cache block; keys of a block; bytes of the ring
 constexpr int PP_MAX_PARTS = 16;
+constexpr int PP_FAR = 80;                                          // powers of their own of small keys and values: 2^-80 of the first block's at least
 // Weights lie 2^PP_UP times as large (float16 then has them down to 2^-28 of the reference point's), and add up to PP_MOST at most before that moves: any is
 // float16 still.  (32 weights that add up to 2^15: one is 2^10 at least, 2^6 above the reference point's.)
 constexpr float PP_UP = 4.f, PP_MOST = 32768.f, PP_LEAST = 5.f;
@@ -293,8 +295,10 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             }
         };
         // Keys and values lie divided by powers of two, 2^key_up and 2^value_up, that take to 1 … 2 the smallest of the largest numbers that the keys, or the
-        // values, of the CTA's first block have each.  Numbers up to 2^15 times that are float16 then, and those of a row whose largest is 2^-14 of it lose
-        // nothing.  A key or a value beyond (`far`) lies divided by a power of its own; its score is multiplied, or its weight, by what that is more.
+        // values, of the CTA's first block have each.  Numbers up to 2^15 times that are float16 then, and those of a row whose largest is 2^-10 of it are off by
+        // 2^-11 of that largest (15 steps by 2^-25 each).  A key or a value beyond, either way (`far`), lies divided by a power of its own; its score is
+        // multiplied, or its weight, by what that is more or less: the reference point is one of weights times powers, so the weights keep their bits.  (No
+        // less than 2^-PP_FAR, so that sums of weights alone are float32 numbers.)
         int key_up = 0, value_up = 0;
         auto top_of = [](uint32_t pair) {                           // the largest number of a group, as bits of a bfloat16 (NaN: 0)
             const float zero = pair_zero(pair), top = fmaxf(fabsf(zero), fabsf(fmaf(15.f, pair_step(pair), zero)));
@@ -302,9 +306,11 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
         };
         auto both = [](int e) { return NG == 2 ? max(e, __shfl_xor_sync(0xffffffffu, e, 2)) : e; };     // (a row's other group is two lanes on)
         int value_far[UNITS];                                       // of the block that is being put
-        // a pair whose zero is below 2^14 and whose step is below 2^10 times the unit needs no power of its own (|zero| + 15 step < 2^15); both as bfloat16
+        // a pair whose zero is below 2^14 and whose step is below 2^10 times the unit needs no power of its own (|zero| + 15 step < 2^15), nor does one whose
+        // zero is 2^-10 of it or more; both as bfloat16, the zero's in the upper half, so that words compare as their zeros do
         uint32_t key_limit = 0u, value_limit = 0u;
         auto limit_of = [](int up) { return (uint32_t)(up + 10 + 127) << 7 | (uint32_t)(up + 14 + 127) << 23; };
+        auto floor_of = [](uint32_t limit) { return limit - (24u << 23); };     // (2^14 to 2^-10)
         auto beyond = [](uint32_t most, uint32_t limit) {           // (NaN is not)
             const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&most), b = *reinterpret_cast<const __nv_bfloat162*>(&limit);
             return __hge(a.x, b.x) || __hge(a.y, b.y);
@@ -314,7 +320,10 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
             const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
             return *reinterpret_cast<const uint32_t*>(&m);
         };
-        auto far_of = [&](uint32_t pair, int up) { return max(0, pp_exponent((uint32_t)both(top_of(pair))) - up - 14); };
+        auto far_of = [&](uint32_t pair, int up) {
+            const int top = both(top_of(pair)), e = pp_exponent((uint32_t)top) - up;
+            return e > 14 ? e - 14 : e < -10 && top != 0 ? max(e, -PP_FAR) : 0;
+        };
         auto put = [&](int t, const Piece& from) -> bool {          // tile t of this CTA: block t / 2, K or V
             const int sl = t % PP_SLOTS, use = t / PP_SLOTS;
             int key_far[UNITS];
@@ -322,21 +331,27 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) key_far[i] = 0;
             if (!(t & 1)) {
-                uint32_t key_most = 0u, value_most = 0u;
+                uint32_t key_most = 0u, value_most = 0u, key_least = 0xffffffffu, value_least = 0xffffffffu;
 #pragma unroll
                 for (int i = 0; i < UNITS; ++i) {
                     value_far[i] = 0;
                     key_most = larger(from.pairs[i], key_most);
                     value_most = larger(from.value_pairs[i], value_most);
+                    key_least = min(key_least, from.pairs[i] & 0x7fff7fffu);
+                    value_least = min(value_least, from.value_pairs[i] & 0x7fff7fffu);
                 }
-                any = __any_sync(0xffffffffu, beyond(key_most, key_limit) || beyond(value_most, value_limit));
+                any = __any_sync(0xffffffffu, beyond(key_most, key_limit) || beyond(value_most, value_limit) || key_least < floor_of(key_limit) ||
+                                                  value_least < floor_of(value_limit));
             }
             if (any) {
+                int most = 0;
 #pragma unroll
                 for (int i = 0; i < UNITS; ++i) {
                     key_far[i] = far_of(from.pairs[i], key_up);
                     value_far[i] = far_of(from.value_pairs[i], value_up);
+                    most |= key_far[i] | value_far[i];
                 }
+                any = __any_sync(0xffffffffu, most != 0);           // (a zero may be small in a row that is not, or where nothing is)
             }
             __half2 step[UNITS], zero[UNITS];
 #pragma unroll
