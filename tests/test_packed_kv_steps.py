@@ -1,4 +1,4 @@
-"""Steps over a cache of 4 bits as a whole: the scratch they take.  On the CPU the kernels' launches are the test's stand-ins; the plans and the scratch are
+"""Steps over a cache of 4 bits as a whole: the scratch they take, and lengths that the host does not know.  On the CPU the kernels' launches are the test's stand-ins; the plans and the scratch are
 the library's own."""
 import random
 
@@ -47,6 +47,13 @@ def test_scratch_of_a_step_is_what_its_tiles_fill(launches, new, past, H, G, d, 
     assert ws.bytes() <= 30e6
 
 
+@pytest.mark.parametrize("new,past,H,G,d", [([70, 3], [0, 10], 4, 4, 64), ([512], [7500], 32, 8, 128), ([300] + [1] * 40, [100] + [900] * 40, 25, 25, 64), ([2, 1], [0, 0], 2, 2, 96)])
+def test_a_step_whose_lengths_the_host_does_not_know(launches, new, past, H, G, d):
+    """The lists are there for plans; without them a step runs all the same, planned from what its context says."""
+    step(new, past, H, G, d, lists=False)
+    assert launches and launches[0][0] == ("attention_prefill_packed" if d in (64, 128) else "attention_packed")
+
+
 def test_every_tile_that_parts_share_has_a_place():
     """Against the tiles one by one: those that reach more than part_blocks blocks are dealt; without a window nothing else has a place."""
     from vlrf_b200.csrc import ops
@@ -91,3 +98,28 @@ def test_prompt_attention_with_scratch_for_the_tiles_that_are_dealt(heads, kv_he
         if places and window == 0 and not short:
             assert bool((partials[:floats] != 77).any())
     check_prompt(fn, pages, new, heads, kv_heads, dim, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,past,H,G,d", [([70, 3], [0, 10], 4, 4, 64), ([300, 1, 9], [1500, 900, 0], 8, 2, 128), ([1, 1, 1], [5, 700, 64], 4, 2, 128), ([40] + [1] * 30, [0] + [900] * 30, 25, 25, 64)])
+def test_lengths_that_the_host_does_not_know_change_the_plan_alone(new, past, H, G, d):
+    """Two plans of a step are apart by their roundings: a weight and a result of 2^-8 each, of numbers below the values' largest."""
+    from test_packed_kv_uses import DEV, HALF_STEP, cache_for, qkv_rows, run_step, step_of
+    from vlrf_b200.csrc import ops
+    cache, table = cache_for(2000, G, d, len(new))
+    whole = [qkv_rows(a + b, H, G, d, seed=i) for i, (a, b) in enumerate(zip(new, past))]
+    for i, b in enumerate(past):
+        if b:
+            ctx = step_of([b], [0], slots=[i])
+            ops.kv_append_packed(whole[i][:b].to(DEV), H * d, (H + G) * d, cache, table, ctx.tok_slot, ctx.tok_pos, b, G, d, ctx.dev_err)
+    rows = torch.cat([w[b:] for w, b in zip(whole, past)]).to(DEV)
+    outs = []
+    for known in (True, False):
+        ctx = step_of(new, past)
+        if not known:
+            ctx.host_seq_lens, ctx.host_seq_pos0 = [], []
+        outs.append(torch.full((sum(new), H * d), 3.0, dtype=torch.bfloat16, device=DEV))
+        run_step(cache, table, rows, outs[-1], ctx, H, G, d)
+        assert int(ctx.dev_err.item()) == 0
+    largest = max(float(w[:, (H + G) * d:].abs().max()) for w in whole)
+    assert float((outs[0].float() - outs[1].float()).abs().max()) <= 4 * HALF_STEP * largest

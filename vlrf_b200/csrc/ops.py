@@ -1223,6 +1223,16 @@ def _packed_decode_step(qkv, q_off, cache, block_table, slots, positions, out, c
 PACKED_SINGLES_APART = 750
 
 
+def _packed_lengths(ctx) -> tuple:
+    """The step's new tokens and those before them, sequence by sequence, as far as the host knows: else a step of its size, with the longest contexts that it
+    may have (for plans; what a sequence brings the kernels read on the device)."""
+    if len(ctx.host_seq_lens) == ctx.n_seqs and len(ctx.host_seq_pos0) == ctx.n_seqs:
+        return ctx.host_seq_lens, ctx.host_seq_pos0
+    rest, others = max(0, ctx.n_tokens - ctx.max_new), ctx.n_seqs - 1
+    lens = [ctx.max_new] + [rest // others + (i < rest % others) for i in range(others)]
+    return lens, [max(0, ctx.max_context - a) for a in lens]
+
+
 def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ctx, n_heads: int, n_kv_heads: int, head_dim: int,
                           scale: float, window: int = 0) -> None:
     """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
@@ -1234,7 +1244,7 @@ def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ct
                             ctx.max_context, n_heads, n_kv_heads, head_dim, scale, window)
         return
     if mma and ctx.max_new > 1 and scale >= 0.0 and head_dim in (64, 128) and ctx.n_seqs <= 65535:
-        lens, pos0 = ctx.host_seq_lens, ctx.host_seq_pos0
+        lens, pos0 = _packed_lengths(ctx)
         single = [b for a, b in zip(lens, pos0) if a == 1]
         apart = n_heads * sum((min(b, window + 63) if window > 0 else b) // 64 + 1 for b in single) >= PACKED_SINGLES_APART and max(lens) > 1
         if apart:
