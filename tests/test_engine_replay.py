@@ -35,6 +35,79 @@ class Model:
         return object()
 
 
+class Layer:
+    def __init__(self, mixer):
+        self.mixer = mixer
+
+    def cache_need(self):
+        return self.mixer.cache_need()
+
+
+@pytest.fixture
+def stepping(monkeypatch):
+    """An engine over layers of plain attention with a cache of 4 bits that says what it would go by: steps are planned and booked, not run."""
+    from vlrf_b200.cache import SequenceCache
+    from vlrf_b200.csrc import ops
+    from vlrf_b200.engine.model import DecoderModel
+    from vlrf_b200.parts.mixer import CausalSelfAttention
+    monkeypatch.setattr(ops, "_SM_COUNT", 148)
+    ops._packed_decode_shape.cache_clear(); ops._packed_prefill_shape.cache_clear()
+
+    def make(heads, kv_heads, dim, kv_bits=4, window=0):
+        mixers = [CausalSelfAttention(torch.zeros((heads + 2 * kv_heads) * dim, 1), None, torch.zeros(1, heads * dim), None, n_heads=heads,
+                                      n_kv_heads=kv_heads, head_dim=dim, scale=0.125, window=window) for _ in range(2)]
+        model = object.__new__(DecoderModel)
+        model.layers, model.schedule, model.embedding, model.act_dtype = [Layer(m) for m in mixers], [], None, torch.bfloat16
+        model.vocab_size, model.max_seq_len = 100, 100_000
+        eng = object.__new__(Engine)
+        eng.model, eng.ws, eng.dev_err, eng.steps_run = model, Workspace("cpu"), None, 0
+        eng.cache = SequenceCache([m.cache_need() for m in mixers], max_tokens=200_000, max_seq_len=100_000, dtype=torch.bfloat16, device="cpu", n_slots=64,
+                                  kv_bits=kv_bits)
+        monkeypatch.setattr(eng.cache, "sync_tables", lambda: None)
+        eng._meta_views, eng._meta_copied = {}, types.SimpleNamespace(synchronize=lambda: None, record=lambda: None)
+        tables = torch.empty(100_000, dtype=torch.int32)
+        eng._meta = lambda n: (tables, tables)
+        eng.went_by = []
+        eng._forward = lambda ctx, signature: eng.went_by.append(signature)
+        return eng
+    yield make
+    ops._packed_decode_shape.cache_clear(); ops._packed_prefill_shape.cache_clear()
+
+
+def goes_by(eng, new, past):
+    """What a step is known by that brings new[i] tokens behind past[i]."""
+    import numpy as np
+    slots = [eng.start_sequence() for _ in new]
+    for s, b in zip(slots, past):
+        if b:
+            eng.cache.reserve(s, b)
+            eng.cache.advance(s, b)
+    eng.step([step_module.StepEntry(s, np.ones(a, dtype=np.int64), [0]) for s, a in zip(slots, new)])
+    for s in slots:
+        eng.end_sequence(s)
+    return eng.went_by[-1]
+
+
+def test_steps_of_one_size_whose_contexts_ask_for_other_launches_are_captured_apart(stepping):
+    eng = stepping(12, 12, 64)
+    short, long = goes_by(eng, [256], [256]), goes_by(eng, [256], [20_000])              # the tiles whole; in parts
+    assert short != long
+    eng = stepping(32, 8, 128)
+    short, long = goes_by(eng, [700] + [1] * 5, [1] + [10] * 5), goes_by(eng, [700] + [1] * 5, [1] + [2000] * 5)         # single tokens apart
+    assert short != long
+
+
+def test_steps_of_one_size_and_like_contexts_are_one_captured_step(stepping):
+    eng = stepping(32, 8, 128)
+    assert goes_by(eng, [700] + [1] * 30, [300] + [2000] * 30) == goes_by(eng, [700] + [1] * 30, [310] + [2005] * 30)
+    assert goes_by(eng, [512], [7500]) == goes_by(eng, [512], [7600])
+    assert len({goes_by(eng, [512], [512 * i]) for i in range(1, 65)}) <= step_module.MAX_CAPTURED       # one long prompt in pieces
+    for eng in (stepping(3, 3, 32), stepping(2, 2, 192)):                                # (sizes that the general kernel takes)
+        assert goes_by(eng, [70, 1], [0, 500]) == goes_by(eng, [70, 1], [9, 5000]) != goes_by(eng, [70, 1], [0, 0])
+    plain = stepping(32, 8, 128, kv_bits=None)
+    assert goes_by(plain, [512], [7500]) == goes_by(plain, [512], [100])
+
+
 @pytest.fixture
 def engine(monkeypatch):
     eng = object.__new__(Engine)

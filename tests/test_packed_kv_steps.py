@@ -75,10 +75,9 @@ def test_every_tile_that_parts_share_has_a_place():
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads,kv_heads,dim", [(3, 3, 64), (4, 2, 128)])
 @pytest.mark.parametrize("new,past", [([300, 1, 64], [77, 700, 0]), ([1] * 33 + [270, 3, 130] + [1] * 4, list(range(40))), ([2, 0, 513], [900, 50, 200]),
-                                      ([1, 400, 90] * 30, [7, 300, 0] * 30)])
+                                      ([1, 400, 90] * 12, [7, 300, 0] * 12)])
 @pytest.mark.parametrize("window", [0, 90, 400])
-@pytest.mark.parametrize("groups,n_parts,part_blocks", [(1, 3, 2), (2, 16, 1), (2, 2, 5)])
-@pytest.mark.parametrize("short", [0, 1, 100])
+@pytest.mark.parametrize("groups,n_parts,part_blocks,short", [(1, 3, 2, 0), (1, 3, 2, 1), (2, 16, 1, 0), (2, 2, 5, 0), (2, 2, 5, 100)])
 def test_prompt_attention_with_scratch_for_the_tiles_that_are_dealt(heads, kv_heads, dim, new, past, window, groups, n_parts, part_blocks, short):
     """Scratch of exactly the size, and of less: tiles without a place are not dealt, and nothing lies outside it."""
     from test_packed_kv_kernels import DEV, Pages, check_prompt
@@ -103,7 +102,8 @@ def test_prompt_attention_with_scratch_for_the_tiles_that_are_dealt(heads, kv_he
 @pytest.mark.gpu
 @pytest.mark.parametrize("new,past,H,G,d", [([70, 3], [0, 10], 4, 4, 64), ([300, 1, 9], [1500, 900, 0], 8, 2, 128), ([1, 1, 1], [5, 700, 64], 4, 2, 128), ([40] + [1] * 30, [0] + [900] * 30, 25, 25, 64)])
 def test_lengths_that_the_host_does_not_know_change_the_plan_alone(new, past, H, G, d):
-    """Two plans of a step are apart by their roundings: a weight and a result of 2^-8 each, of numbers below the values' largest."""
+    """Two plans of a step are apart by their roundings.  The decode kernel's weights times steps: 2^-8 of 15 steps, twice the values' largest at most; the prompt
+    kernel's operands: less; every result: 2^-8 of the largest.  So by 6 times 2^-8 of it (scores in float32, or of float16 operands, move weights by less)."""
     from test_packed_kv_uses import DEV, HALF_STEP, cache_for, qkv_rows, run_step, step_of
     from vlrf_b200.csrc import ops
     cache, table = cache_for(2000, G, d, len(new))
@@ -122,4 +122,36 @@ def test_lengths_that_the_host_does_not_know_change_the_plan_alone(new, past, H,
         run_step(cache, table, rows, outs[-1], ctx, H, G, d)
         assert int(ctx.dev_err.item()) == 0
     largest = max(float(w[:, (H + G) * d:].abs().max()) for w in whole)
-    assert float((outs[0].float() - outs[1].float()).abs().max()) <= 4 * HALF_STEP * largest
+    assert float((outs[0].float() - outs[1].float()).abs().max()) <= 6 * HALF_STEP * largest
+
+
+@pytest.mark.gpu
+def test_steps_of_one_size_behind_short_and_long_contexts_captured_and_replayed(tmp_path):
+    """256 tokens behind 256 (tiles taken whole) and behind 640 (dealt to parts that meet in scratch), 40 beside single tokens of short and long contexts, each
+    several times in an engine that replays what it has seen: the same bits as without replaying, and the counters of the parts are left zero."""
+    from conftest import random_ids
+    from test_engine import GPT2_WIDE
+    from vlrf_b200.engine import Engine, StepEntry, load_model
+    from vlrf_b200.weights import write_random_model
+    d = write_random_model(dict(GPT2_WIDE, vocab_size=1003, bos_token_id=1, eos_token_id=2), 79, tmp_path / "small")
+    ids, runs = [random_ids(1003, 1024, 600 + i) for i in range(9)], []
+    for capture in (True, False):
+        eng = Engine(load_model(d, "bfloat16"), max_tokens=9 * 1024, kv_cache="int4")
+        eng.capture_repeated_steps = capture
+        logits = []
+        for past in (256, 256, 640, 256, 640, 640, 256, 700, 300):
+            slot = eng.start_sequence()
+            eng.step([StepEntry(slot, ids[0][:past], [])])
+            logits.append(eng.step([StepEntry(slot, ids[0][past:past + 256], [0, 200, 255])]).clone())
+            eng.end_sequence(slot)
+        for past in (9, 9, 900, 9, 900, 900, 9):
+            slots = [eng.start_sequence() for _ in ids]
+            eng.step([StepEntry(s, x[:past], []) for s, x in zip(slots[1:], ids[1:])])
+            logits.append(eng.step([StepEntry(slots[0], ids[0][:40], [0, 39])] + [StepEntry(s, x[past:past + 1], [0]) for s, x in zip(slots[1:], ids[1:])]).clone())
+            for s in slots:
+                eng.end_sequence(s)
+        eng.check_device_errors()
+        assert not bool(eng.ws._bufs["packed_counters"].any())
+        assert (len(eng._graphs) >= 4) == capture
+        runs.append(logits)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

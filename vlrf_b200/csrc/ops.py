@@ -1029,10 +1029,11 @@ def attention_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, to
 PACKED_ATTENTION_MMA = True
 
 
-def _packed_mma_takes(qkv, q_off: int, cache: PackedKV, out, n_heads: int, n_kv_heads: int, head_dim: int) -> bool:
-    """Whether the tensor-core kernels take these tensors (head sizes are theirs): what the library's vlrf_attn_packed_decode_takes and
+def _packed_mma_takes(qkv, q_off: int, cache: PackedKV, out, n_kv_heads: int, head_dim: int) -> bool:
+    """Whether the tensor-core kernels take these tensors (which head sizes, the plan says): what the library's vlrf_attn_packed_decode_takes and
     vlrf_attn_packed_prefill_takes ask, and tensors on 16 bytes."""
     return PACKED_ATTENTION_MMA and isinstance(cache, PackedKV) and qkv.dtype == torch.bfloat16 and cache.block_tokens == 64 \
+        and cache.n_kv_heads == n_kv_heads and cache.head_dim == head_dim \
         and (qkv.data_ptr() | out.data_ptr()) % 16 == 0 and (qkv.stride(0) | q_off | out.stride(0)) % 8 == 0
 
 
@@ -1204,11 +1205,8 @@ def _packed_room(ws, sizes: tuple) -> tuple:
     return ws.get("packed_partials", sizes[0], 1, torch.float32), ws.get_zeroed("packed_counters", sizes[1], torch.int32)
 
 
-def _packed_decode_step(qkv, q_off, cache, block_table, slots, positions, out, ctx, rows, past, longest, n_heads, n_kv_heads, head_dim, scale, window,
+def _packed_decode_step(qkv, q_off, cache, block_table, slots, positions, out, ctx, rows, shape, n_heads, n_kv_heads, head_dim, scale, window,
                         row_of=None) -> None:
-    """past: the single tokens' contexts where the host knows them."""
-    n = len(past)
-    shape = packed_decode_shape(n or rows, n_heads, n_kv_heads, head_dim, longest, window, (sum(past) + n) / (n * longest) if n > 0 else 0.67)
     partials = counters = None
     if shape[1] > 1:
         partials, counters = _packed_room(ctx.ws, packed_decode_scratch(rows, n_heads, n_kv_heads, head_dim, shape[1]))
@@ -1233,35 +1231,75 @@ def _packed_lengths(ctx) -> tuple:
     return lens, [max(0, ctx.max_context - a) for a in lens]
 
 
+@dataclasses.dataclass(frozen=True)
+class PackedPlan:
+    """What `attention_packed_step` launches for a step that the tensor-core kernels take.  decode: the shape of the decode kernel, for a step of single tokens
+    or those beside prompts (else None); prompt: (groups, n_parts, part_blocks) of the prompt kernel, or None; n_places: tiles that have scratch."""
+    decode: tuple | None
+    prompt: tuple | None = None
+    n_places: int = 0
+
+    def key(self) -> tuple:
+        """The same for plans that may stand for one another: blocks a part to a quarter (the kernels cut a longer context into as many parts, equally long)."""
+        decode, prompt = [t and (t[0], t[1], _coarse(t[2]) if t[1] > 1 else 0) for t in (self.decode, self.prompt)]
+        return decode, prompt, self.n_places
+
+
+def _coarse(n: int) -> int:
+    """n rounded up to three bits."""
+    unit = 1 << max(0, n.bit_length() - 3)
+    return -(-n // unit) * unit
+
+
+def packed_step_plan(ctx, n_heads: int, n_kv_heads: int, head_dim: int, window: int = 0) -> PackedPlan | None:
+    """The plan of a step (see `attention_packed_step`), from its sizes and the lengths that the host knows, worked out once a step for each kind of heads; None
+    where the tensor-core kernels do not take the step's sizes (the general kernel goes by sizes alone)."""
+    which = (n_heads, n_kv_heads, head_dim, window)
+    if which not in ctx.plans:
+        ctx.plans[which] = _packed_step_plan(ctx, *which)
+    return ctx.plans[which]
+
+
+def _packed_step_plan(ctx, n_heads: int, n_kv_heads: int, head_dim: int, window: int) -> PackedPlan | None:
+    if (head_dim % 64 != 0 or ctx.n_tokens > 65535) if ctx.max_new == 1 else (head_dim not in (64, 128) or ctx.n_seqs > 65535):
+        return None
+
+    def decode(rows, past, longest):               # past: the single tokens' contexts where the host knows them
+        n = len(past)
+        return packed_decode_shape(n or rows, n_heads, n_kv_heads, head_dim, longest, window, (sum(past) + n) / (n * longest) if n > 0 else 0.67)
+
+    if ctx.max_new == 1:
+        past = ctx.host_seq_pos0
+        return PackedPlan(decode(ctx.n_tokens, past if len(past) == ctx.n_tokens else (), ctx.max_context))
+    lens, pos0 = _packed_lengths(ctx)
+    single = [b for a, b in zip(lens, pos0) if a == 1]
+    apart = n_heads * sum((min(b, window + 63) if window > 0 else b) // 64 + 1 for b in single) >= PACKED_SINGLES_APART and max(lens) > 1
+    if apart:
+        lens, pos0 = [a for a in lens if a > 1], [b for a, b in zip(lens, pos0) if a > 1]
+    groups, n_parts, part_blocks = packed_prefill_shape(lens, pos0, n_heads, head_dim, window)
+    n_places = packed_prefill_places(lens, pos0, groups, n_parts, part_blocks, window)
+    return PackedPlan(decode(ctx.n_seqs, single, max(single) + 1) if apart else None, (groups, n_parts if n_places > 0 else 1, part_blocks), _coarse(n_places))
+
+
 def attention_packed_step(qkv, q_off: int, cache: PackedKV, block_table, out, ctx, n_heads: int, n_kv_heads: int, head_dim: int,
                           scale: float, window: int = 0) -> None:
     """The attention of a step (prompt tokens, single tokens or a mix) over a cache of 4 bits, with the kernel that suits it; the cache
     already holds the step's own keys and values."""
-    mma = _packed_mma_takes(qkv, q_off, cache, out, n_heads, n_kv_heads, head_dim)
-    if mma and ctx.max_new == 1 and head_dim % 64 == 0 and ctx.n_tokens <= 65535:
-        past = ctx.host_seq_pos0
-        _packed_decode_step(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx, ctx.n_tokens, past if len(past) == ctx.n_tokens else (),
-                            ctx.max_context, n_heads, n_kv_heads, head_dim, scale, window)
+    plan = packed_step_plan(ctx, n_heads, n_kv_heads, head_dim, window) if _packed_mma_takes(qkv, q_off, cache, out, n_kv_heads, head_dim) else None
+    if plan is not None and ctx.max_new == 1:
+        _packed_decode_step(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx, ctx.n_tokens, plan.decode, n_heads, n_kv_heads, head_dim,
+                            scale, window)
         return
-    if mma and ctx.max_new > 1 and scale >= 0.0 and head_dim in (64, 128) and ctx.n_seqs <= 65535:
-        lens, pos0 = _packed_lengths(ctx)
-        single = [b for a, b in zip(lens, pos0) if a == 1]
-        apart = n_heads * sum((min(b, window + 63) if window > 0 else b) // 64 + 1 for b in single) >= PACKED_SINGLES_APART and max(lens) > 1
-        if apart:
-            lens, pos0 = [a for a in lens if a > 1], [b for a, b in zip(lens, pos0) if a > 1]
-        groups, n_parts, part_blocks = packed_prefill_shape(lens, pos0, n_heads, head_dim, window)
+    if plan is not None and ctx.max_new > 1 and scale >= 0.0:
         partials = counters = None
-        n_places = packed_prefill_places(lens, pos0, groups, n_parts, part_blocks, window)
-        if n_places > 0:
-            partials, counters = _packed_room(ctx.ws, packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, groups, n_parts, n_places))
-        else:
-            n_parts = 1
+        if plan.prompt[1] > 1:
+            partials, counters = _packed_room(ctx.ws, packed_prefill_scratch(ctx.n_seqs, ctx.max_new, n_heads, head_dim, *plan.prompt[:2], plan.n_places))
         attention_prefill_packed(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_start, ctx.seq_pos0, out, ctx.n_tokens, ctx.n_seqs, ctx.max_new,
-                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, groups, n_parts, part_blocks, partials, counters,
-                                 2 if apart else 1, n_places)
-        if apart:
-            _packed_decode_step(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_pos0, out, ctx, ctx.n_seqs, single, max(single) + 1, n_heads, n_kv_heads,
-                                head_dim, scale, window, ctx.seq_start)
+                                 n_heads, n_kv_heads, head_dim, scale, window, ctx.dev_err, *plan.prompt, partials, counters,
+                                 1 if plan.decode is None else 2, plan.n_places)
+        if plan.decode is not None:
+            _packed_decode_step(qkv, q_off, cache, block_table, ctx.seq_slot, ctx.seq_pos0, out, ctx, ctx.n_seqs, plan.decode, n_heads, n_kv_heads, head_dim,
+                                scale, window, ctx.seq_start)
         return
     attention_packed(qkv, q_off, cache, block_table, ctx.tok_slot, ctx.tok_pos, out, ctx.n_tokens, n_heads, n_kv_heads, head_dim, scale,
                      window, ctx.dev_err)

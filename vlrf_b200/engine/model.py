@@ -93,6 +93,10 @@ class DecoderModel:
             if kv(layer.cache_need()) and not getattr(getattr(layer, "mixer", None), "takes_packed_kv", False):
                 raise ValueError(f"layer {i}: {type(getattr(layer, 'mixer', layer)).__name__} does not take keys and values in 4 bits")
 
+    def packed_plans(self, ctx: StepContext) -> tuple:
+        """What the attention of a step over a cache in 4 bits launches, which goes by the sequences' contexts too (see the mixers' `packed_plan`)."""
+        return tuple({p: None for p in (layer.mixer.packed_plan(ctx) for layer in self.layers if hasattr(getattr(layer, "mixer", None), "packed_plan"))})
+
     def cache_needs(self) -> list:
         """For every schedule entry what it keeps per sequence (None for entries that read another's); behind them, where
         the embedding keeps something per sequence (say, the token before), one more entry with its need."""

@@ -26,6 +26,8 @@ DEVERR_TEXT = {1: "a token id outside the vocabulary", 2: "a position outside th
 
 #: how keys and values may be held -> bits a number (None: the model's dtype)
 KV_CACHES = {None: None, "int4": 4}
+#: captured steps that an engine keeps (a long prompt in pieces over a cache in 4 bits is one for every quarter by which its context grows)
+MAX_CAPTURED = 32
 
 
 @dataclasses.dataclass
@@ -67,7 +69,7 @@ class Engine:
         # Steps of a shape seen before are replayed from a captured CUDA graph: the step's integer tables
         # live at fixed device addresses, so only their contents change from step to step.
         self.capture_repeated_steps = True
-        self._graphs: dict = {}        # (tokens, sequences, longest and shortest run, wanted rows, from the start) -> (graph, logits)
+        self._graphs: dict = {}        # (tokens, sequences, longest and shortest run, wanted rows, from the start, plans) -> (graph, logits)
         self._seen: dict = {}
         self._graph_generation = -1
         from ..csrc import ops
@@ -209,8 +211,10 @@ class Engine:
             n_logit_rows=n_want, act_dtype=self.model.act_dtype, dev_err=self.dev_err, ws=self.ws,
             host_seq_slots=[e.slot for e in entries], host_seq_lens=p["lens"], host_seq_pos0=p["pos0"], min_new=min(p["lens"]))
         # (a captured step is replayed for steps of the same sizes; whether every sequence begins at its first token
-        # belongs to them, since parts may launch other kernels for such a step, as do the longest and the shortest run)
-        logits = self._forward(ctx, (T, B, ctx.max_new, ctx.min_new, n_want, not any(p["pos0"])))
+        # belongs to them, since parts may launch other kernels for such a step, as do the longest and the shortest run;
+        # so does what attention over a cache in 4 bits plans from the contexts)
+        plans = () if self.cache.kv_bits is None or ctx.max_new == 1 else self.model.packed_plans(ctx)
+        logits = self._forward(ctx, (T, B, ctx.max_new, ctx.min_new, n_want, not any(p["pos0"]), *plans))
         for e in entries:
             self.cache.advance(e.slot, len(e.tokens))
         self.steps_run += 1
@@ -227,7 +231,7 @@ class Engine:
             return hit[1]
         n = self._seen.get(signature, 0)
         self._seen[signature] = n + 1
-        if n == 0 or len(self._graphs) >= 16:
+        if n == 0 or len(self._graphs) >= MAX_CAPTURED:
             logits = self.model.forward(ctx, self.cache)   # first time: plain launches (they size the scratch)
             self._drop_stale_graphs()
             return logits
