@@ -21,18 +21,18 @@ def launches(monkeypatch):
     ops._packed_decode_shape.cache_clear(); ops._packed_prefill_shape.cache_clear()
 
 
-def step(new, past, H, G, d, window=0, ws=None, lists=True, scale=0.125):
+def step(new, past, H, G, d, window=0, ws=None, lists=True, scale=0.125, dtype=torch.bfloat16):
     from vlrf_b200.csrc import ops
     T, B = sum(new), len(new)
     t = torch.zeros(B + 1, dtype=torch.int32)
     ws = ws or Workspace("cpu")
     ctx = StepContext(n_tokens=T, tokens=t, tok_slot=t, tok_pos=t, n_seqs=B, seq_slot=t, seq_start=t, seq_pos0=t, max_new=max(new),
-                      max_context=max(a + b for a, b in zip(new, past)), logit_rows=t, n_logit_rows=0, act_dtype=torch.bfloat16, dev_err=t, ws=ws,
+                      max_context=max(a + b for a, b in zip(new, past)), logit_rows=t, n_logit_rows=0, act_dtype=dtype, dev_err=t, ws=ws,
                       host_seq_slots=list(range(B)), min_new=min(new))
     if lists:
         ctx.host_seq_lens, ctx.host_seq_pos0 = list(new), list(past)
-    rows = torch.empty((T, (H + 2 * G) * d), dtype=torch.bfloat16)
-    out = torch.empty((T, H * d), dtype=torch.bfloat16)
+    rows = torch.empty((T, (H + 2 * G) * d), dtype=dtype)
+    out = torch.empty((T, H * d), dtype=dtype)
     ops.attention_packed_step(rows, 0, ops.PackedKV.zeros(1, G, 64, d, "cpu"), t.view(1, -1), out, ctx, H, G, d, scale, window)
     return ws
 
@@ -52,6 +52,41 @@ def test_a_step_whose_lengths_the_host_does_not_know(launches, new, past, H, G, 
     """The lists are there for plans; without them a step runs all the same, planned from what its context says."""
     step(new, past, H, G, d, lists=False)
     assert launches and launches[0][0] == ("attention_prefill_packed" if d in (64, 128) else "attention_packed")
+
+
+@pytest.mark.parametrize("dim", [16, 64, 80, 128, 192, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [0.125, -1.0])
+def test_the_kernels_that_a_layer_names_are_those_that_its_steps_launch(launches, dim, dtype, scale):
+    from vlrf_b200.csrc import ops
+    from vlrf_b200.engine.model import DecoderModel
+    from vlrf_b200.parts.mixer import CausalSelfAttention
+    H, G = 6, 3
+    mixer = CausalSelfAttention(torch.zeros((H + 2 * G) * dim, 1), None, torch.zeros(1, H * dim), None, n_heads=H, n_kv_heads=G, head_dim=dim, scale=scale)
+    model = object.__new__(DecoderModel)
+    model.act_dtype, model.layers = dtype, [type("Layer", (), dict(mixer=mixer))(), object()]
+    (layer, name, kinds), = model.describe_kernels(kv_bits=4)
+    assert (layer, name) == (0, "CausalSelfAttention")
+    for kind, new, past in (("prompt", [70, 3], [0, 10]), ("decode", [1, 1], [9, 700])):
+        launches.clear()
+        step(new, past, H, G, dim, scale=scale, dtype=dtype)
+        assert [n for n, _, _ in launches] == [{"tcgen05": "attention_prefill_packed", "mma.sync": "attention_decode_packed", "CUDA cores": "attention_packed"}[kinds[kind]]]
+
+
+def test_a_layer_off_the_tensor_cores_is_said_of_the_cache_that_it_has(capsys, monkeypatch):
+    """Heads of 192: decode over 4 bits is on the tensor cores, prompts are not; the plain cache's kernels are not spoken of."""
+    from vlrf_b200 import log
+    from vlrf_b200.engine.loading import say_kernels
+    from vlrf_b200.engine.model import DecoderModel
+    from vlrf_b200.parts.mixer import CausalSelfAttention
+    monkeypatch.setattr(log, "_level", log.LEVELS["warn"])
+    model = object.__new__(DecoderModel)
+    model.act_dtype = torch.bfloat16
+    model.layers = [type("Layer", (), dict(mixer=CausalSelfAttention(torch.zeros(3 * 192, 1), None, torch.zeros(1, 192), None, n_heads=1, n_kv_heads=1, head_dim=192,
+                                                                     scale=0.1)))() for _ in range(2)]
+    say_kernels(model, 4)
+    said = capsys.readouterr().err
+    assert "layers 0…1 (CausalSelfAttention): prompt attention on CUDA cores, decode attention on mma.sync, keys and values in 4 bits" in said
 
 
 def test_every_tile_that_parts_share_has_a_place():

@@ -38,7 +38,7 @@ class Model:
              n_slots: int | None = None, kv_cache: str | None = None) -> "Model":
         """A folder with config.json and model.safetensors (vlrf_load_weights, vlrf.h:124).  kv_cache "int4": keys and values in 4 bits
         (vlrf_set_kv_cache_type there), for models whose attention takes it (GPT-2)."""
-        return cls(load_model(model_dir, dtype, device), max_tokens=max_tokens, n_slots=n_slots, kv_cache=kv_cache)
+        return cls(load_model(model_dir, dtype, device, kv_cache), max_tokens=max_tokens, n_slots=n_slots, kv_cache=kv_cache)
 
     @classmethod
     def init_random(cls, config: dict, seed: int = 1234, dtype="bfloat16", device="cuda:0",

@@ -1231,6 +1231,14 @@ def _packed_lengths(ctx) -> tuple:
     return lens, [max(0, ctx.max_context - a) for a in lens]
 
 
+def attention_packed_kinds(dtype: torch.dtype, head_dim: int, block_tokens: int, row_width: int, q_off: int, out_width: int, scale: float) -> dict:
+    """Which kernels the steps of these sizes over a cache of 4 bits run on: {"prompt": …, "decode": …}, each "tcgen05", "mma.sync" or "CUDA cores" (the general
+    kernel)."""
+    mma = PACKED_ATTENTION_MMA and dtype == torch.bfloat16 and block_tokens == 64 and (row_width | q_off | out_width) % 8 == 0
+    return {"prompt": "tcgen05" if mma and head_dim in (64, 128) and scale >= 0.0 else "CUDA cores",
+            "decode": "mma.sync" if mma and head_dim % 64 == 0 else "CUDA cores"}
+
+
 @dataclasses.dataclass(frozen=True)
 class PackedPlan:
     """What `attention_packed_step` launches for a step that the tensor-core kernels take.  decode: the shape of the decode kernel, for a step of single tokens

@@ -23,9 +23,22 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"unknown dtype '{name}'; choose bfloat16 or float32") from None
 
 
-def load_model(model_dir, dtype="bfloat16", device="cuda:0") -> DecoderModel:
+def say_kernels(model: DecoderModel, kv_bits: int | None = None) -> None:
+    """Which attention kernels the model's layers get, over a cache in the model's dtype or (4) in 4 bits."""
+    kinds = {}
+    for i, name, k in model.describe_kernels(kv_bits=kv_bits):
+        kinds.setdefault((name, k["prompt"], k["decode"]), []).append(i)
+    for (name, prompt, decode), layers in kinds.items():
+        say = log.warn if model.act_dtype == torch.bfloat16 and "CUDA cores" in (prompt, decode) else log.info
+        say(f"layers {layers[0]}…{layers[-1]} ({name}): prompt attention on {prompt}, decode attention on {decode}"
+            + ("" if kv_bits is None else f", keys and values in {kv_bits} bits")
+            + (" (no tensor-core kernel takes this head size)" if say is log.warn else ""))
+
+
+def load_model(model_dir, dtype="bfloat16", device="cuda:0", kv_cache: str | None = None) -> DecoderModel:
     """Read config.json, pick the architecture it names, check model.safetensors against that
-    architecture's tensor list and assemble the model on the device."""
+    architecture's tensor list and assemble the model on the device.  (kv_cache: as the model's engine will have it, which then says
+    which kernels attention gets.)"""
     import vlrf_b200.models  # noqa: F401  (registers the architectures)
     arch, cfg, weights = open_model_dir(model_dir)
     options = BuildOptions(dtype=parse_dtype(dtype), device=torch.device(device))
@@ -38,11 +51,6 @@ def load_model(model_dir, dtype="bfloat16", device="cuda:0") -> DecoderModel:
     log.info(f"{model_dir}: {arch.name}, {len(model.layers)} layers, width {model.width}, vocabulary {model.vocab_size}, "
              f"{model.weight_bytes() / 2**20:.1f} MiB of weights as {options.dtype} on {options.device} "
              f"in {time.perf_counter() - started:.2f} s")
-    kinds = {}
-    for i, name, k in model.describe_kernels():
-        kinds.setdefault((name, k["prompt"], k["decode"]), []).append(i)
-    for (name, prompt, decode), layers in kinds.items():
-        say = log.warn if options.dtype == torch.bfloat16 and "CUDA cores" in (prompt, decode) else log.info
-        say(f"layers {layers[0]}…{layers[-1]} ({name}): prompt attention on {prompt}, decode attention on {decode}"
-            + (" (no tensor-core kernel takes this head size)" if say is log.warn else ""))
+    if kv_cache is None:
+        say_kernels(model)
     return model

@@ -74,13 +74,14 @@ class DecoderModel:
         self.__dict__["_replayable"] = all(ok(p) for p in parts)
         return self.__dict__["_replayable"]
 
-    def describe_kernels(self, block_tokens: int = 64) -> list:
-        """For every layer whose mixer can say, which attention kernels its sizes get (see the mixers' `kernels`)."""
+    def describe_kernels(self, block_tokens: int = 64, kv_bits: int | None = None) -> list:
+        """For every layer whose mixer can say, which attention kernels its sizes get (see the mixers' `kernels`); kv_bits: as for the cache."""
         out = []
         for i, layer in enumerate(self.layers):
             mixer = getattr(layer, "mixer", None)
             if mixer is not None and hasattr(mixer, "kernels"):
-                out.append((i, type(mixer).__name__, mixer.kernels(self.act_dtype, block_tokens)))
+                more = (kv_bits,) if kv_bits is not None and getattr(mixer, "takes_packed_kv", False) else ()
+                out.append((i, type(mixer).__name__, mixer.kernels(self.act_dtype, block_tokens, *more)))
         return out
 
     def check_packed_kv(self) -> None:

@@ -54,6 +54,9 @@ class Engine:
         if not torch.cuda.is_available():
             raise KernelError("no CUDA device: this framework runs on the GPU only")
         library()  # fail now, loudly, if the kernels cannot be built or loaded
+        if kv_cache is not None:
+            from .loading import say_kernels
+            say_kernels(model, KV_CACHES[kv_cache])
         self.model = model
         self.device = model.device
         self.cache = SequenceCache(model.cache_needs(), max_tokens=max_tokens, max_seq_len=model.max_seq_len,

@@ -125,10 +125,12 @@ class CausalSelfAttention:
                           n_kv_heads=self.n_kv_heads, head_dim=self.head_dim, scale=self.scale, window=self.window)
         program.product(merged, self.w_out, self.b_out, x, residual=x)
 
-    def kernels(self, act_dtype: torch.dtype, block_tokens: int) -> dict:
+    def kernels(self, act_dtype: torch.dtype, block_tokens: int, kv_bits: int | None = None) -> dict:
         """Which attention kernels these sizes get: {"prompt": …, "decode": …}, each "tcgen05", "mma.sync" or
         "CUDA cores".  Said once when a model is built, so that a head size that leaves the tensor cores is a
-        visible fact."""
+        visible fact.  kv_bits 4: over a cache in 4 bits."""
+        if kv_bits is not None:
+            return ops.attention_packed_kinds(act_dtype, self.head_dim, block_tokens, self.qkv_width, self.q_off, self.n_heads * self.head_dim, self.scale)
         return {"prompt": ops.attention_prefill_kind(act_dtype, self.head_dim, block_tokens, self.qkv_width, self.q_off,
                                                      self.n_heads * self.head_dim),
                 "decode": ops.attention_decode_kind(act_dtype, self.head_dim)}
