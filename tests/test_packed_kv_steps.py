@@ -107,6 +107,38 @@ def test_every_tile_that_parts_share_has_a_place():
         assert ops.packed_prefill_places(new, past, groups, 1, each, window) == 0
 
 
+#: us of the prompt kernel, measured on 148 SMs: new tokens, those before them, heads, head size, window, {(groups, parts, blocks a part): time}
+MEASURED = [
+    ([1024, 1024], [0, 0], 12, 64, 0, {(1, 1, 16): 28.4, (1, 2, 8): 27.3, (1, 2, 12): 28.5, (1, 3, 6): 35.9, (2, 1, 16): 26.1, (2, 2, 8): 22.1, (2, 2, 12): 22.1, (2, 3, 6): 34.4}),
+    ([512], [7500], 32, 128, 0, {(2, 1, 126): 204.8, (2, 2, 63): 119.7, (2, 2, 95): 119.5, (2, 3, 42): 163.8, (2, 4, 32): 135.9, (2, 8, 16): 166.3, (2, 16, 8): 226.4}),
+    ([1, 17, 300, 640, 1], [900, 0, 129, 384, 77], 25, 64, 256, {(1, 1, 7): 24.0, (2, 1, 8): 33.4, (2, 2, 6): 39.8}),
+    ([200], [0], 12, 64, 0, {(1, 1, 4): 10.9, (2, 1, 4): 11.5}),
+    ([1000], [0], 25, 64, 0, {(1, 1, 16): 28.8, (1, 2, 8): 29.1, (1, 2, 12): 28.1, (1, 3, 6): 36.0, (2, 1, 16): 25.8, (2, 2, 8): 29.5, (2, 2, 12): 22.0, (2, 3, 6): 34.1}),
+    ([1000] * 4, [0] * 4, 25, 64, 0, {(1, 1, 16): 66.4, (1, 2, 8): 93.6, (1, 2, 12): 84.1, (1, 3, 6): 103.7, (2, 1, 16): 59.8, (2, 2, 8): 84.6, (2, 2, 12): 72.7, (2, 3, 6): 97.4}),
+    ([1000] * 4, [4000] * 4, 12, 64, 0, {(1, 1, 79): 243.7, (1, 2, 40): 212.7, (1, 2, 60): 212.8, (1, 3, 27): 214.0, (1, 4, 20): 227.9, (1, 8, 10): 275.5, (2, 1, 79): 182.3, (2, 2, 40): 166.5, (2, 2, 60): 166.5, (2, 3, 27): 167.6, (2, 4, 20): 189.9, (2, 8, 10): 244.4}),
+    ([1000] * 4, [0] * 4, 32, 128, 0, {(2, 1, 16): 106.2, (2, 2, 8): 151.2, (2, 2, 12): 128.2, (2, 3, 6): 178.1}),
+    ([17], [6000], 12, 64, 0, {(1, 1, 95): 122.1, (1, 2, 48): 70.1, (1, 2, 72): 69.9, (1, 3, 32): 51.4, (1, 4, 24): 41.1, (1, 8, 12): 29.2, (1, 16, 6): 30.4, (2, 1, 95): 92.8, (2, 2, 48): 54.9, (2, 2, 72): 55.2, (2, 3, 32): 41.9, (2, 4, 24): 34.5, (2, 8, 12): 26.3, (2, 12, 8): 26.5, (2, 16, 6): 37.7}),
+    ([400, 30, 90], [1000, 3000, 0], 28, 128, 0, {(2, 1, 48): 74.8, (2, 2, 24): 55.3, (2, 2, 36): 55.2, (2, 3, 16): 72.1, (2, 4, 12): 71.8, (2, 8, 6): 97.9}),
+    ([1000, 600], [5000, 300], 12, 64, 300, {(1, 1, 8): 26.0, (1, 2, 6): 30.9, (2, 1, 10): 23.9, (2, 2, 8): 34.6}),
+    ([2, 2], [50, 900], 8, 128, 0, {(2, 1, 15): 28.6, (2, 2, 8): 25.7, (2, 2, 12): 25.7}),
+    ([256], [640], 12, 64, 0, {(1, 1, 14): 23.8, (1, 2, 7): 18.8, (1, 2, 11): 18.9, (2, 1, 14): 23.2, (2, 2, 7): 20.3, (2, 2, 11): 20.4}),
+    ([64], [2000], 32, 128, 0, {(2, 1, 33): 53.6, (2, 2, 17): 38.1, (2, 2, 25): 37.9, (2, 3, 11): 32.5, (2, 4, 9): 31.1}),
+    ([2000], [0], 8, 128, 0, {(2, 1, 32): 59.2, (2, 2, 16): 42.0, (2, 2, 24): 47.7, (2, 3, 11): 36.7, (2, 4, 8): 51.3}),
+    ([700], [100], 32, 128, 0, {(2, 1, 13): 31.4, (2, 2, 7): 44.8, (2, 2, 10): 30.1}),
+    ([100] * 8, [0, 50, 100, 150, 200, 250, 300, 350], 12, 64, 0, {(1, 1, 8): 15.7, (1, 2, 6): 20.0, (2, 1, 8): 14.3, (2, 2, 6): 17.8}),
+]
+
+
+@pytest.mark.parametrize("lens,pos0,heads,dim,window,times", MEASURED)
+def test_the_shape_of_a_prompt_step_is_the_fastest_or_within_a_tenth_of_it(monkeypatch, lens, pos0, heads, dim, window, times):
+    from vlrf_b200.csrc import ops
+    monkeypatch.setattr(ops, "_SM_COUNT", 148)
+    ops._packed_prefill_shape.cache_clear()
+    shape = ops.packed_prefill_shape(lens, pos0, heads, dim, window)
+    ops._packed_prefill_shape.cache_clear()
+    assert times[shape] <= 1.1 * min(times.values())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads,kv_heads,dim", [(3, 3, 64), (4, 2, 128)])
 @pytest.mark.parametrize("new,past", [([300, 1, 64], [77, 700, 0]), ([1] * 33 + [270, 3, 130] + [1] * 4, list(range(40))), ([2, 0, 513], [900, 50, 200]),

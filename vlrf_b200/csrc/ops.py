@@ -1037,26 +1037,29 @@ def _packed_mma_takes(qkv, q_off: int, cache: PackedKV, out, n_kv_heads: int, he
         and (qkv.data_ptr() | out.data_ptr()) % 16 == 0 and (qkv.stride(0) | q_off | out.stride(0)) % 8 == 0
 
 
-#: Microseconds of a CTA of `attention_prefill_packed`, measured: its start, queries and result (with one and with two groups of queries), a block of 64 keys
-#: (head sizes 64 and 128), and meeting the other parts of a tile in scratch.
-PACKED_PROMPT_US = dict(cta=(4.5, 5.5), block={64: 1.05, 128: 1.45}, meet=5.0)
+#: Microseconds of a CTA of `attention_prefill_packed` by (head size, groups of queries), measured: its start, queries and result; a block of 64 keys, alone
+#: on the GPU.  By head size: meeting the other parts of a tile in scratch, and so much for each of them.  What a block takes more (factors): where every SM
+#: has a CTA, where every SM has two, and with a window, whose blocks are all masked.  158 shapes of 25 steps are predicted to 8 % (root mean square), those taken to 17 %.
+PACKED_PROMPT_US = dict(cta={(64, 1): 6.3, (64, 2): 7.3, (128, 2): 8.9}, block={(64, 1): 1.2, (64, 2): 0.95, (128, 2): 1.4}, meet={64: (4.4, 0.3), 128: (7.4, 0.3)},
+                        busy=0.2, crowded=0.12, window=0.46)
 
 
 def packed_prefill_shape(lens, pos0, n_heads: int, head_dim: int, window: int = 0) -> tuple:
     """(groups of 128 queries a CTA of `attention_prefill_packed` takes, most CTAs to which it deals the keys of a tile, blocks of 64 that each of those
     holds at least) for sequences that bring lens[i] tokens behind pos0[i].  Two groups share the keys that a CTA takes apart; one makes twice the CTAs,
-    two an SM, which pays for small heads and few tokens (one prompt of 200 tokens of 12 heads of 64: 10.2 us against 11.3; four of 1,000 behind 4,000: 204
-    against 172).  A tile's blocks are a chain: parts shorten it where the tiles leave SMs idle (512 tokens of 32 heads of 128 behind 7,500: 206 us whole, 119
-    in two parts, 163 in three, which come in two waves)."""
+    two an SM, which pays for few tokens (one prompt of 200 tokens of 12 heads of 64: 10.9 us against 11.5; four of 1,000: 66.4 against 59.8; four of 1,000
+    behind 4,000: 244 against 182).  A tile's blocks are a chain: parts shorten it where the tiles leave SMs idle (512 tokens of 32 heads of 128 behind
+    7,500: 205 us whole, 119.5 in two parts, 164 in three, which come in two waves), or only the longest quarter of them (1,000 tokens of 25 heads of 64: 25.8 us
+    whole, 29.5 with all tiles of more than 8 blocks in two, 22.0 with those of more than 12)."""
     return _packed_prefill_shape(tuple(lens), tuple(pos0), n_heads, head_dim, window)
 
 
 @functools.lru_cache(maxsize=1024)                # (a rule of sizes alone; worked out anew it takes longer than a launch)
 def _packed_prefill_shape(lens: tuple, pos0: tuple, n_heads: int, head_dim: int, window: int) -> tuple:
-    best = None
+    cost, sms, best = PACKED_PROMPT_US, sm_count(), None
+    meet_first, meet_each = cost["meet"][head_dim]
     for groups in (1, 2) if head_dim == 64 else (2,):
-        places, rows = sm_count() * (3 - groups), 128 * groups
-        cta, block, meet = PACKED_PROMPT_US["cta"][groups - 1], PACKED_PROMPT_US["block"][head_dim], PACKED_PROMPT_US["meet"]
+        places, rows, cta = sms * (3 - groups), 128 * groups, cost["cta"][head_dim, groups]
         lengths: dict = {}                         # blocks of a tile -> tiles of a head that have so many
         for a, b in zip(lens, pos0):
             for t in range(0, a, rows):
@@ -1069,14 +1072,18 @@ def _packed_prefill_shape(lens: tuple, pos0: tuple, n_heads: int, head_dim: int,
             if each < min(chain, 6):
                 break
             parts = {n: min(16, -(-n // each)) for n in lengths}
+            meet = {n: meet_first + meet_each * p if p > 1 else 0.0 for n, p in parts.items()}
             ctas = n_heads * sum(k * parts[n] for n, k in lengths.items())
-            longest = max(cta + -(-n // p) * block + (meet if p > 1 else 0.0) for n, p in parts.items())
+            block = cost["block"][head_dim, groups] * (1.0 + cost["busy"] * min(1.0, ctas / sms)) * (1.0 + (cost["window"] if window > 0 else 0.0))
+            if groups == 1:
+                block *= 1.0 + cost["crowded"] * max(0.0, min(1.0, ctas / sms - 1.0))
+            longest = max(cta + -(-n // p) * block + meet[n] for n, p in parts.items())
             if ctas <= places:
                 time = longest
             elif even:
                 time = -(-ctas // places) * longest
             else:
-                busy = sum(k * (n * block + parts[n] * (0.6 * cta + (meet if parts[n] > 1 else 0.0))) for n, k in lengths.items())
+                busy = sum(k * (n * block + parts[n] * (cta + meet[n])) for n, k in lengths.items())
                 time = max(longest, n_heads * busy / places + longest / 2)
             if best is None or time < 0.97 * best[0]:
                 best = (time, groups, max(parts.values()), each)
