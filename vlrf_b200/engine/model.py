@@ -95,8 +95,13 @@ class DecoderModel:
                 raise ValueError(f"layer {i}: {type(getattr(layer, 'mixer', layer)).__name__} does not take keys and values in 4 bits")
 
     def packed_plans(self, ctx: StepContext) -> tuple:
-        """What the attention of a step over a cache in 4 bits launches, which goes by the sequences' contexts too (see the mixers' `packed_plan`)."""
-        return tuple({p: None for p in (layer.mixer.packed_plan(ctx) for layer in self.layers if hasattr(getattr(layer, "mixer", None), "packed_plan"))})
+        """What the attention of a step over a cache in 4 bits launches, which goes by the sequences' contexts too: a key for each kind of heads (the mixers'
+        `packed_heads`), the same for steps of one size that may replay one another."""
+        kinds = self.__dict__.get("_packed_heads")         # (asked at every step; the parts of a model do not change)
+        if kinds is None:
+            kinds = self.__dict__["_packed_heads"] = tuple(dict.fromkeys(
+                layer.mixer.packed_heads for layer in self.layers if hasattr(getattr(layer, "mixer", None), "packed_heads")))
+        return tuple(plan and plan.key() for plan in (ops.packed_step_plan(ctx, *heads) for heads in kinds))
 
     def cache_needs(self) -> list:
         """For every schedule entry what it keeps per sequence (None for entries that read another's); behind them, where

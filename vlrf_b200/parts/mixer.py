@@ -135,10 +135,10 @@ class CausalSelfAttention:
                                                      self.n_heads * self.head_dim),
                 "decode": ops.attention_decode_kind(act_dtype, self.head_dim)}
 
-    def packed_plan(self, ctx: StepContext):
-        """What the attention of a step over a cache in 4 bits launches: a key that is the same for steps of one size that may replay one another."""
-        plan = ops.packed_step_plan(ctx, self.n_heads, self.n_kv_heads, self.head_dim, self.window)
-        return plan and plan.key()
+    @property
+    def packed_heads(self) -> tuple:
+        """What steps over a cache in 4 bits are planned from beside their lengths (see csrc.ops.packed_step_plan)."""
+        return self.n_heads, self.n_kv_heads, self.head_dim, self.window
 
     def _attend(self, qkv, view, merged, ctx: StepContext) -> None:
         T = ctx.n_tokens
