@@ -89,6 +89,24 @@ def test_a_layer_off_the_tensor_cores_is_said_of_the_cache_that_it_has(capsys, m
     assert "layers 0…1 (CausalSelfAttention): prompt attention on CUDA cores, decode attention on mma.sync, keys and values in 4 bits" in said
 
 
+@pytest.mark.parametrize("lists", [True, False])
+@pytest.mark.parametrize("new", [[0, 0], [0]])
+def test_a_step_that_brings_nothing(launches, new, lists):
+    step(new, [5] * len(new), 4, 2, 64, lists=lists)
+    assert [name for name, _, _ in launches] in ([], ["attention_packed"])
+
+
+def test_scratch_for_a_number_of_tiles_that_is_none():
+    import ctypes
+    from vlrf_b200.csrc import library
+    lib = library()
+    p = [ctypes.c_void_p(4096)] * 4
+    for groups, n_parts, places in ((1, 1, -1), (2, 2, -5), (0, 1, 0), (3, 1, 0)):
+        assert lib.vlrf_attn_packed_prefill_places(p[0], 512, 0, *p, 10, p[0], 4, *p, 256, 210, 3, 70, 4, 2, 64, 64, 0.125, 0, 1, groups, n_parts, 1, places, p[0], p[0],
+                                                   p[0], None) != 0
+        assert b"attn_packed_prefill" in lib.vlrf_last_error()
+
+
 def test_every_tile_that_parts_share_has_a_place():
     """Against the tiles one by one: those that reach more than part_blocks blocks are dealt; without a window nothing else has a place."""
     from vlrf_b200.csrc import ops

@@ -1106,7 +1106,7 @@ def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_
         raise KernelError(f"{what}: bfloat16 rows, and a slot, a first row and a first position for every sequence")
     scratch = (0, 0)
     if n_places is None:
-        n_places = n_seqs * -(-max_new // (128 * groups)) if groups > 0 else 0
+        n_places = min(n_seqs * -(-max_new // (128 * groups)), 2 ** 31 - 1) if groups > 0 else 0
     if n_parts > 1:
         scratch = _packed_scratch(what, packed_prefill_scratch(n_seqs, max_new, n_heads, head_dim, groups, n_parts, n_places), partials, counters)
     call("vlrf_attn_packed_prefill_places", qkv.data_ptr(), qkv.stride(0), q_off, *cache.args, block_table.data_ptr(), block_table.shape[1], seq_slot.data_ptr(),
@@ -1276,7 +1276,7 @@ def packed_step_plan(ctx, n_heads: int, n_kv_heads: int, head_dim: int, window: 
 
 
 def _packed_step_plan(ctx, n_heads: int, n_kv_heads: int, head_dim: int, window: int) -> PackedPlan | None:
-    if (head_dim % 64 != 0 or ctx.n_tokens > 65535) if ctx.max_new == 1 else (head_dim not in (64, 128) or ctx.n_seqs > 65535):
+    if ctx.max_new < 1 or ((head_dim % 64 != 0 or ctx.n_tokens > 65535) if ctx.max_new == 1 else (head_dim not in (64, 128) or ctx.n_seqs > 65535)):
         return None
 
     def decode(rows, past, longest):               # past: the single tokens' contexts where the host knows them
