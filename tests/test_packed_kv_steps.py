@@ -107,6 +107,13 @@ def test_scratch_for_a_number_of_tiles_that_is_none():
         assert b"attn_packed_prefill" in lib.vlrf_last_error()
 
 
+@pytest.mark.parametrize("heads,tokens", [(0, 64), (2, 0)])
+def test_a_cache_without_heads_or_tokens_is_refused(heads, tokens):
+    from vlrf_b200.csrc import KernelError, ops
+    with pytest.raises(KernelError):
+        ops.PackedKV.zeros(3, heads, tokens, 64, "cpu")
+
+
 def test_every_tile_that_parts_share_has_a_place():
     """Against the tiles one by one: those that reach more than part_blocks blocks are dealt; without a window nothing else has a place."""
     from vlrf_b200.csrc import ops

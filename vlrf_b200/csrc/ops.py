@@ -916,7 +916,7 @@ class PackedKV:
     def __post_init__(self):
         shape = tuple(self.k.shape)
         group = packed_group(2 * shape[3]) if len(shape) == 4 else 0
-        if group == 0:
+        if group == 0 or shape[1] == 0 or shape[2] == 0:
             raise KernelError(f"a cache in 4 bits is [block, kv_head, block_tokens, head_dim/2] with head sizes that are multiples of {HEAD_DIM_STEP} up "
                               f"to {HEAD_DIM_MAX}, not {list(shape)}")
         pairs = shape[:3] + (2 * shape[3] // group, 2)
