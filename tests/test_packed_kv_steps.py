@@ -114,6 +114,17 @@ def test_a_cache_without_heads_or_tokens_is_refused(heads, tokens):
         ops.PackedKV.zeros(3, heads, tokens, 64, "cpu")
 
 
+@pytest.mark.parametrize("entry", [1, 2, 3, -1, 99, (2, 1), (7, 0)])
+def test_reading_back_an_entry_that_is_not_there(entry):
+    from vlrf_b200.cache import KVNeed, SequenceCache, StateNeed
+    from vlrf_b200.engine.step import Engine, StepError
+    eng = object.__new__(Engine)
+    eng.cache = SequenceCache([KVNeed(3, 64), None, (KVNeed(2, 32), StateNeed((4,)))], max_tokens=128, max_seq_len=128, dtype=torch.bfloat16, device="cpu", kv_bits=4)
+    slot = eng.start_sequence()
+    with pytest.raises(StepError, match="cache entry"):
+        eng.keys_values(slot, entry)
+
+
 def test_every_tile_that_parts_share_has_a_place():
     """Against the tiles one by one: those that reach more than part_blocks blocks are dealt; without a window nothing else has a place."""
     from vlrf_b200.csrc import ops

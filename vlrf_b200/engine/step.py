@@ -14,7 +14,7 @@ import dataclasses
 import numpy as np
 import torch
 
-from ..cache import SequenceCache
+from ..cache import CacheError, SequenceCache
 from ..csrc import KernelError, library
 from .capture import capture_into
 from ..parts.context import StepContext, Workspace
@@ -94,7 +94,10 @@ class Engine:
         from ..csrc import ops
         if not self.cache.slots.is_held(slot):
             raise StepError(f"slot {slot} is not held by a sequence")
-        view = self.cache.view(entry)
+        try:
+            view = self.cache.view(entry)
+        except (CacheError, IndexError):
+            raise StepError(f"there is no cache entry {entry} that keeps anything") from None
         if view.packed is None:
             raise StepError(f"cache entry {entry} does not hold keys and values in 4 bits")
         last = self.cache.lengths[slot] if last is None else last
