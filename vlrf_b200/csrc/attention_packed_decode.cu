@@ -18,7 +18,9 @@
 //
 // Bound by taking codes apart and by latency rather than by bytes: 131,071 tokens of 8 heads of 128 for 32 queries (151 MB) 40 us, 3.8 TB/s, with the
 // integer pipe 47 % and the tensor pipe 23 % busy; the copies alone take 31 us, the arithmetic alone 30.  16 rows of 1 to 8,116 tokens: 27 us, 2.7 TB/s;
-// 32 rows of 300 to 1,013 tokens of 25 heads of 64: 15.6 us, 2.4 TB/s; one row of 701 tokens of 12 heads: 5.3 us, a chain of latencies.
+// 32 rows of 300 to 1,013 tokens of 25 heads of 64: 15.6 us, 2.4 TB/s; one row of 701 tokens of 12 heads: 5.3 us, a chain of latencies.  A window of 512, 32 rows
+// of 8 heads of 128 for 32 queries: 11.1 us, 1.7 TB/s; heads of 192 and 256 (8 over 2, 16 rows of 2,001 tokens): 12.8 and 20.6 us, 1.1 and 0.9 TB/s (two CTAs of four
+// warps an SM are what 192 to 239 registers leave).
 #include "common.cuh"
 #include "packed_kv.cuh"
 

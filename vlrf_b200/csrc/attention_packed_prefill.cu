@@ -23,9 +23,10 @@
 // key's row of K NaN instead, which the mask hides from the same queries; so a head's row that sees it is NaN throughout.
 //
 // Bound by the chain of a block, some 2,800 cycles at head size 128 of which the tensor cores have 1,000: producers take a block's numbers apart in the issue
-// slots that softmax leaves (1,000 cycles each for K and V), and S waits for them.  More producers would take registers from the softmax warps, which then
-// spill (28 warps: 173 us where 22 take 119); blocks of 64 keys with two threads a row are what 80 registers hold.  Measured: 512 new tokens
-// behind 7500, 32 heads of 128 over 8: 119 us, 0.55 PFLOP/s; twice 1024 new tokens, 12 heads of 64: 21.8 us.
+// slots that softmax leaves (1,000 cycles each for K and V), and S waits for them.  More producers would take registers from the softmax warps (28 warps: 173 us
+// where 22 took 119); blocks of 64 keys with two threads a row are what 80 registers hold, all but 28 to 138 bytes of a thread that are spilled.  Measured: 512 new
+// tokens behind 7500, 32 heads of 128 over 8: 123 us, 0.53 PFLOP/s (of them 2 for looking for small keys and values, 2.5 for the tile's place in scratch); twice
+// 1024 new tokens, 12 heads of 64: 22.1 us.
 // Every wait is bounded; a CTA that gives up sets the device error word, waits (bounded) for its MMAs, frees its tensor memory and leaves.
 #include <type_traits>
 #include <cuda_fp16.h>
@@ -239,7 +240,7 @@ attn_packed_prefill_kernel(const __nv_bfloat16* __restrict__ qkv, int ld, int q_
     }
     const bool active = n_rows > 0 && n_new >= least_new && slot >= 0 && pos0 >= 0 && part < tile_parts;      // uniform over the CTA
     if (!active) return;                                            // (before it holds anything)
-    constexpr uint32_t TMEM_COLS = 256 * GROUPS;                    // a group: S BK columns, O DH, P NP times BK / 2 (two bfloat16 a column)
+    constexpr uint32_t TMEM_COLS = 256 * GROUPS;                    // a group: S BK columns, O DH, P NP times BK / 2 (two float16 a column)
     if (warp == SOFT) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tsm(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");

@@ -1095,7 +1095,9 @@ def attention_prefill_packed(qkv, q_off: int, cache: PackedKV, block_table, seq_
                              part_blocks: int = 6, partials=None, counters=None, least_new: int = 1, n_places: int | None = None) -> None:
     """Causal attention of every sequence's new tokens (rows seq_start[i] … seq_start[i+1]−1 of qkv, the first of them at position
     seq_pos0[i]) over the sequence's cache of 4 bits, which already holds these tokens; bfloat16, head size 64 or 128, on the tcgen05
-    tensor cores, operands float16 under powers of two.  n_parts > 1 deals the keys of long tiles to that many CTAs (see packed_prefill_shape) and wants
+    tensor cores, operands float16 under powers of two: a number of a key or a value is off by 2^-10 of the largest of its row and head, for rows down to 2^-80 of
+    the first block's that its CTA reads.  A query that sees a value group that is NaN (one that held a number that is not finite) has NaN in its whole head
+    here, in that group's columns only in `attention_packed` and `attention_decode_packed`.  n_parts > 1 deals the keys of long tiles to that many CTAs (see packed_prefill_shape) and wants
     float32 `partials` and zeroed int32 `counters` (see packed_prefill_scratch); the counters are left zero.  n_places: how many of the tiles that may be dealt
     have scratch (see packed_prefill_places; those behind them are not dealt); None: every tile that there can be.  Sequences that bring fewer than
     least_new tokens are skipped."""
@@ -1189,7 +1191,8 @@ def _packed_scratch(what: str, want: tuple, partials, counters) -> tuple:
 
 def attention_decode_packed(qkv, q_off: int, cache: PackedKV, block_table, tok_slot, tok_pos, out, n_rows: int, n_heads: int, n_kv_heads: int,
                             head_dim: int, scale: float, window: int, shape: tuple, dev_err, partials=None, counters=None, row_of=None) -> None:
-    """One bfloat16 query per row and head attends the keys 0…position of its slot in a cache of 4 bits, on the tensor cores.  shape = (a CTA an SM
+    """One bfloat16 query per row and head attends the keys 0…position of its slot in a cache of 4 bits, on the tensor cores: weights times steps are bfloat16
+    numbers.  Queries are below 2^37 and steps of values below 2^47; a weight times a step below 2^-73 is nothing (`attention_packed` has float32's range).  shape = (a CTA an SM
     or not, n_split, blocks a part), see packed_decode_shape: a context takes as many parts as it needs for so many blocks each, at most (and in
     fact, where a context is longer than they hold) n_split; with n_split > 1 they meet in float32 `partials` and zeroed int32 `counters` (see packed_decode_scratch; the counters are left
     zero).  Rows with slot −1 are left as they are.  row_of (int32, a number more than n_rows): entry i of tok_slot and tok_pos stands for the rows
