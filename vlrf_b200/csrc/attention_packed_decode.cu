@@ -10,7 +10,8 @@
 // The order of entries inside a product is free, so each lane takes its keys' codes in pieces of eight bytes, and its values' entries
 // pairwise from two tokens' words.  Weights change from the layout of a result to that of an operand by `movmatrix`.  Weights times steps
 // are rounded to bfloat16 (each by up to 2^-8 of itself, as in the library's other bfloat16 attention); scores, sums, zeros and results stay
-// in float32, and code products are exact.  Scales that keep code · 2^-133 in float32's range: queries by 2^90 (so |q| < 2^37), weights by 2^80 (steps of
+// in float32, and code products are exact.  (As two bfloat16 numbers each they would leave results as near to 64 bits as the plain form, 0.0017 of them against 0.0019
+// to 0.0024, for 4 to 7 % of the time.)  Scales that keep code · 2^-133 in float32's range: queries by 2^90 (so |q| < 2^37), weights by 2^80 (steps of
 // values below 2^47; a weight times a step below 2^-73 is nothing).
 //
 // The warps of a CTA merge their sums in shared memory; the parts of a context leave theirs in scratch, and the CTA that comes last merges them
